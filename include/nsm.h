@@ -500,6 +500,55 @@ int nsm_lm_head_nf4(const void* x, int32_t x_dtype, int32_t tokens, const uint8_
                     const void* bias, int32_t bias_dtype, void* out, int32_t out_dtype, void* workspace,
                     size_t workspace_bytes, nsm_stream_t stream);
 
+/* ---- 4-bit linear layers ---------------------------------------------------
+ * y[r][n] = bias[n] + sum_k x[r][k] * (T[q[n][k]] - z[n][k / group_size]) * scale[n][k / group_size]
+ * for 1..nsm_linear4bit_max_rows(x_dtype) rows of x and a weight [N =
+ * out_features, K = in_features] of 4-bit values q.  With `code` (16 fp32
+ * values) T is that codebook and there are no zero points: NF4 weights with
+ * their absmax as scales.  Without it T[q] = q and z is the group's zero
+ * point (`zeros`, 0..255), 8 when `zeros` is NULL.  The attention projections,
+ * dense MLPs and heads of a 4-bit checkpoint (the reference dequantises them
+ * and calls F.linear, streaming_llama_runtime.py:4765).
+ *
+ * The kernels read a tiled layout that nsm_linear4bit_pack writes once from the
+ * row-major bytes (row n at packed + n * packed_row_bytes, column 2i in the
+ * high nibble of byte i; scales and zeros [N][ceil(K / group_size)], the last
+ * group may be partial).  packed_out takes nsm_linear4bit_packed_bytes(N, K)
+ * bytes, scales_out nsm_linear4bit_scale_count(N, K, group_size) floats and
+ * zeros_out as many bytes, each 16-byte aligned; the row-major source is not
+ * read afterwards.  N up to 2^24, K even and up to 2^20, group_size a
+ * multiple of 32.
+ *
+ * x rows are x_row_stride elements apart, out rows out_row_stride (each row
+ * contiguous).  x, bias and out may be fp32 / fp16 / bf16.  Accumulation is
+ * fp32; x enters as fp16 scaled by a power of two per row (fp32 x as value +
+ * remainder), the codebook as fp16 for fp16 / bf16 outputs and to 22 bits for
+ * fp32 ones.  Results do not depend on the other rows of the call and are the
+ * same bits every time.  The workspace needs no initialisation; calls that
+ * share one must not overlap on the GPU. */
+typedef struct nsm_linear4bit_weights {
+  const uint8_t* packed; /* tiled, from nsm_linear4bit_pack */
+  const float* scales;   /* tiled */
+  const uint8_t* zeros;  /* tiled, or NULL */
+  const float* code;     /* [16] or NULL */
+  const void* bias;      /* [N] or NULL */
+  int32_t bias_dtype;
+  int32_t out_features;
+  int32_t in_features;
+  int32_t group_size;
+} nsm_linear4bit_weights;
+size_t nsm_linear4bit_packed_bytes(int32_t out_features, int32_t in_features);
+size_t nsm_linear4bit_scale_count(int32_t out_features, int32_t in_features, int32_t group_size);
+int nsm_linear4bit_max_rows(int32_t x_dtype);
+int nsm_linear4bit_pack(const uint8_t* packed, int64_t packed_row_bytes, const void* scales, int32_t scale_dtype,
+                        const uint8_t* zeros, int32_t out_features, int32_t in_features, int32_t group_size,
+                        int32_t codebook, uint8_t* packed_out, float* scales_out, uint8_t* zeros_out,
+                        nsm_stream_t stream);
+size_t nsm_linear4bit_workspace_bytes(int32_t rows, int32_t x_dtype, int32_t out_features, int32_t in_features);
+int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_stride,
+                   const nsm_linear4bit_weights* weights, void* out, int32_t out_dtype, int64_t out_row_stride,
+                   void* workspace, size_t workspace_bytes, nsm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -45,6 +45,8 @@ EXPORTED = (
     "nsm_route_rows", "nsm_workspace_selection", "nsm_exchange_connect_local", "nsm_exchange_set_spin_limit",
     "nsm_set_copy_wait_limit", "nsm_static_error", "nsm_token_workspace_bytes", "nsm_token_set_layers",
     "nsm_decode_token", "nsm_token_profile",
+    "nsm_linear4bit_packed_bytes", "nsm_linear4bit_scale_count", "nsm_linear4bit_max_rows", "nsm_linear4bit_pack",
+    "nsm_linear4bit_workspace_bytes", "nsm_linear4bit",
 )
 
 
@@ -84,6 +86,12 @@ class LayerIoC(ctypes.Structure):
         ("norm_weight", c_void_p), ("eps", c_float), ("flags", c_int32), ("reserved2", c_int32),
         ("exchange", c_void_p), ("stage_events", c_void_p),
     ]
+
+
+class Linear4bitWeightsC(ctypes.Structure):
+    _fields_ = [("packed", c_void_p), ("scales", c_void_p), ("zeros", c_void_p), ("code", c_void_p),
+                ("bias", c_void_p), ("bias_dtype", c_int32), ("out_features", c_int32), ("in_features", c_int32),
+                ("group_size", c_int32)]
 
 
 _SIGS = {
@@ -148,6 +156,14 @@ _SIGS = {
                                 c_void_p]),
     "nsm_cache_promote": (c_int, [POINTER(MlpWeightsC), c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int32,
                                   c_void_p, c_void_p]),
+    "nsm_linear4bit_packed_bytes": (c_size_t, [c_int32, c_int32]),
+    "nsm_linear4bit_scale_count": (c_size_t, [c_int32, c_int32, c_int32]),
+    "nsm_linear4bit_max_rows": (c_int, [c_int32]),
+    "nsm_linear4bit_pack": (c_int, [c_void_p, c_int64, c_void_p, c_int32, c_void_p, c_int32, c_int32, c_int32, c_int32,
+                                    c_void_p, c_void_p, c_void_p, c_void_p]),
+    "nsm_linear4bit_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32]),
+    "nsm_linear4bit": (c_int, [c_void_p, c_int32, c_int32, c_int64, POINTER(Linear4bitWeightsC), c_void_p, c_int32,
+                               c_int64, c_void_p, c_size_t, c_void_p]),
 }
 
 _lock = threading.Lock()
