@@ -549,6 +549,57 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
                    const nsm_linear4bit_weights* weights, void* out, int32_t out_dtype, int64_t out_row_stride,
                    void* workspace, size_t workspace_bytes, nsm_stream_t stream);
 
+/* ---- beam search: selection and reordering -------------------------------
+ * What follows the logits of a head (nsm_lm_head_nf4, nsm_linear4bit) when
+ * `beams` continuations of each of `batch` prompts are decoded together.  The
+ * reference decodes one sequence; these have no counterpart there.
+ *
+ * nsm_beam_select: for each batch item the `candidates` best (beam w, token v) by
+ *   scores[w] + logits[w][v] - logsumexp(logits[w][:]),
+ * best first, equal scores in the order of w, then v.  logits [batch][beams]
+ * [vocab] (fp32 / fp16 / bf16; strides in elements, each row contiguous),
+ * scores [batch][beams] fp32.  A beam whose score is -infinity or NaN is out: its logits
+ * are not read.  finished [batch][beams] (bytes, may be NULL): a finished beam is one
+ * candidate, pad_token at its own score; its logits are not read either.  A logit
+ * of -infinity or NaN is no candidate; +infinity counts as the largest finite
+ * value.  Sums and scores are compared in 64 bits.  Outputs [batch]
+ * [candidates]: scores, tokens and parents (the beam w); where fewer candidates
+ * exist, score -infinity, token -1, parent 0.  1..32 beams, 1..64 candidates.  The
+ * workspace needs no initialisation. */
+size_t nsm_beam_select_workspace_bytes(int32_t batch, int32_t beams, int32_t vocab, int32_t candidates);
+int nsm_beam_select(const void* logits, int32_t logits_dtype, int64_t batch_stride, int64_t beam_stride,
+                    const float* scores, const uint8_t* finished, int32_t batch, int32_t beams, int32_t vocab,
+                    int32_t candidates, int32_t pad_token, float* out_scores, int64_t* out_tokens,
+                    int64_t* out_parents, void* workspace, size_t workspace_bytes, nsm_stream_t stream);
+
+/* One per-beam state: row b * beams + w (row_stride bytes apart) holds outer0 x
+ * outer1 runs of run_bytes contiguous bytes.  With position_bytes > 0 a run is
+ * `positions` entries of that size (a cache's or a history's positions), of which
+ * a call may move the first `length` only.  Rows must not overlap. */
+typedef struct nsm_beam_state {
+  void* data;
+  int64_t row_stride;
+  int64_t outer0;
+  int64_t outer0_stride;
+  int64_t outer1;
+  int64_t outer1_stride;
+  int64_t run_bytes;
+  int64_t position_bytes;
+  int64_t positions;
+} nsm_beam_state;
+size_t nsm_beam_states_bytes(int32_t count);
+/* Checks the states and copies them to a device table (16-byte aligned,
+ * nsm_beam_states_bytes(count)); synchronises `stream`, not capturable. */
+int nsm_beam_states_set(const nsm_beam_state* states, int32_t count, void* table, size_t table_bytes,
+                        nsm_stream_t stream);
+/* state[b][w] = state[b][parents[b][w]] for every state and beam, in place, in
+ * one launch; `states` and `table` are what nsm_beam_states_set was given.
+ * parents [batch][beams] (device): a value outside 0..beams-1 leaves its row as it
+ * is.  length >= 0 moves the first `length` positions of the states that have
+ * positions, a negative one everything. */
+int nsm_beam_reorder(const nsm_beam_state* states, const void* table, int32_t count, int32_t batch, int32_t beams,
+                     const int64_t* parents, int64_t length, nsm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

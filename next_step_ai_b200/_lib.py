@@ -47,6 +47,8 @@ EXPORTED = (
     "nsm_decode_token", "nsm_token_profile",
     "nsm_linear4bit_packed_bytes", "nsm_linear4bit_scale_count", "nsm_linear4bit_max_rows", "nsm_linear4bit_pack",
     "nsm_linear4bit_workspace_bytes", "nsm_linear4bit",
+    "nsm_beam_select_workspace_bytes", "nsm_beam_select", "nsm_beam_states_bytes", "nsm_beam_states_set",
+    "nsm_beam_reorder",
 )
 
 
@@ -92,6 +94,12 @@ class Linear4bitWeightsC(ctypes.Structure):
     _fields_ = [("packed", c_void_p), ("scales", c_void_p), ("zeros", c_void_p), ("code", c_void_p),
                 ("bias", c_void_p), ("bias_dtype", c_int32), ("out_features", c_int32), ("in_features", c_int32),
                 ("group_size", c_int32)]
+
+
+class BeamStateC(ctypes.Structure):
+    _fields_ = [("data", c_void_p), ("row_stride", c_int64), ("outer0", c_int64), ("outer0_stride", c_int64),
+                ("outer1", c_int64), ("outer1_stride", c_int64), ("run_bytes", c_int64), ("position_bytes", c_int64),
+                ("positions", c_int64)]
 
 
 _SIGS = {
@@ -164,6 +172,13 @@ _SIGS = {
     "nsm_linear4bit_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32]),
     "nsm_linear4bit": (c_int, [c_void_p, c_int32, c_int32, c_int64, POINTER(Linear4bitWeightsC), c_void_p, c_int32,
                                c_int64, c_void_p, c_size_t, c_void_p]),
+    "nsm_beam_select_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32]),
+    "nsm_beam_select": (c_int, [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_int32, c_int32,
+                                c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "nsm_beam_states_bytes": (c_size_t, [c_int32]),
+    "nsm_beam_states_set": (c_int, [POINTER(BeamStateC), c_int32, c_void_p, c_size_t, c_void_p]),
+    "nsm_beam_reorder": (c_int, [POINTER(BeamStateC), c_void_p, c_int32, c_int32, c_int32, c_void_p, c_int64,
+                                 c_void_p]),
 }
 
 _lock = threading.Lock()

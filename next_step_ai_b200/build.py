@@ -16,7 +16,8 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libnsm.so"
 SOURCES = ["nsm_abi.cu", "nsm_router.cu", "nsm_decode.cu", "nsm_aux.cu", "nsm_static.cu", "nsm_union.cu", "nsm_exchange.cu",
-           "nsm_lmhead.cu", "nsm_token.cu", "nsm_linear4bit.cu"]
+           "nsm_lmhead.cu", "nsm_token.cu", "nsm_linear4bit.cu",
+           "nsm_beam.cu"]
 GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -1,0 +1,115 @@
+"""Host side of beam selection and reordering (no GPU): the description of a
+state's runs, size queries and refusals."""
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+from next_step_ai_b200 import _lib, beam  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not _lib.LIB_PATH.exists():
+        from next_step_ai_b200.build import build
+
+        build()
+    return _lib.load()
+
+
+def _elements(c, rows, es, length=None):
+    """The element offsets of row 1 that a move of `length` positions touches."""
+    run = c.run_bytes if length is None or c.position_bytes == 0 else min(length, c.positions) * c.position_bytes
+    return sorted(c.row_stride + a * c.outer0_stride + b * c.outer1_stride + i
+                  for a in range(c.outer0) for b in range(c.outer1) for i in range(0, run, es))
+
+
+def _expect(t, dim, length):
+    v = t[1] if dim is None or length is None else t[1].narrow(dim - 1, 0, length)
+    base, es, out = t.data_ptr(), t.element_size(), []
+    off = (v.data_ptr() - base) // es
+    idx = torch.cartesian_prod(*(torch.arange(n) for n in v.shape)).reshape(-1, v.dim()) if v.dim() else torch.zeros((1, 0))
+    for i in idx.tolist():
+        out.append((off + sum(int(a) * s for a, s in zip(i, v.stride()))) * es)
+    return sorted(out)
+
+
+@pytest.mark.parametrize("make,dim", [
+    (lambda: torch.zeros((4, 6)), None),
+    (lambda: torch.zeros(4, dtype=torch.int64), None),
+    (lambda: torch.zeros((4, 6), dtype=torch.uint8), 1),
+    (lambda: torch.zeros((4, 2, 5, 3)), 2),
+    (lambda: torch.zeros((4, 2, 3, 5)), 3),
+    (lambda: torch.zeros((4, 5, 2, 3)), 1),
+    (lambda: torch.zeros((4, 3, 8, 6))[:, :, 1:6, 2:5], None),
+    (lambda: torch.zeros((5, 4, 3)).transpose(0, 1), None),
+    (lambda: torch.zeros((4, 2, 5, 3))[:, 1:], 2),
+    (lambda: torch.zeros((4, 2, 5, 3))[:, :, :4], 2),
+])
+def test_runs_cover_the_state(make, dim):
+    t = make()
+    c = beam._describe(t, 4, dim)
+    assert _elements(c, 4, t.element_size()) == _expect(t, None, None)
+    if dim is not None:
+        assert c.positions == t.shape[dim]
+        for n in (0, 1, t.shape[dim] - 1):
+            assert _elements(c, 4, t.element_size(), n) == _expect(t, dim, n)
+
+
+def test_states_that_are_refused():
+    z = torch.zeros
+    with pytest.raises(RuntimeError, match="4 rows"):
+        beam._describe(z((5, 2)), 4, None)
+    with pytest.raises(RuntimeError, match="overlaps itself"):
+        beam._describe(z((1, 8)).expand(4, 8), 4, None)
+    with pytest.raises(RuntimeError, match="overlaps itself"):
+        beam._describe(torch.as_strided(z(64), (4, 8), (4, 1)), 4, None)
+    with pytest.raises(RuntimeError, match="more than two strided"):
+        beam._describe(z((4, 4, 4, 4, 4))[:, :3, :3, :3, :3], 4, None)
+    with pytest.raises(RuntimeError, match="not contiguous"):
+        beam._describe(z((4, 5, 8))[:, :, :6], 4, 1)
+    with pytest.raises(RuntimeError, match="not contiguous"):
+        beam._describe(z((4, 3, 5)).transpose(1, 2), 4, 1)
+    with pytest.raises(RuntimeError, match="length dimension"):
+        beam._describe(z((4, 5)), 4, 0)
+    with pytest.raises(RuntimeError, match="no values"):
+        beam._describe(z((4, 0)), 4, None)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        beam.BeamStates([z((4, 2))], 2, 2)
+    with pytest.raises(RuntimeError, match="at least one"):
+        beam.BeamStates([], 2, 2)
+    with pytest.raises(RuntimeError, match="beams"):
+        beam.BeamStates([z((66, 2))], 2, 33)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        beam.beam_select(z((1, 2, 8)), z((1, 2)))
+
+
+def test_bad_arguments_are_errors_before_any_device_call(lib):
+    one = 256                                              # an address that is never read
+    sel = lib.nsm_beam_select
+
+    def call(logits=one, dt=0, bs=8, ws_=4, scores=one, B=1, W=2, V=8, k=4, pad=0, ws=one):
+        return sel(logits, dt, bs, ws_, scores, None, B, W, V, k, pad, one, one, one, ws, 1 << 20, None)
+
+    bad, big = _lib.NSM_ERR_INVALID_ARG, _lib.NSM_ERR_UNSUPPORTED
+    assert call(dt=3) == bad and call(logits=None) == bad and call(scores=None) == bad and call(ws=None) == bad
+    assert call(B=-1) == bad and call(pad=8) == bad and call(pad=-1) == bad and call(bs=-8) == bad
+    assert call(logits=one + 2) == bad
+    assert call(W=33) == big and call(k=65) == big and call(V=0) == big and call(k=0) == big
+    assert call(B=0) == _lib.NSM_OK
+    assert lib.nsm_beam_select_workspace_bytes(1, 33, 8, 4) == 0
+    assert lib.nsm_beam_states_bytes(3) == 3 * 72 and lib.nsm_beam_states_bytes(0) == 0
+    st = (_lib.BeamStateC * 1)(_lib.BeamStateC(one, 8, 1, 0, 1, 0, 8, 0, 0))
+    assert lib.nsm_beam_states_set(st, 1, one, 8, None) == _lib.NSM_ERR_WORKSPACE
+    assert lib.nsm_beam_states_set(st, 0, one, 72, None) == bad
+    for field, value in (("data", None), ("outer0", 0), ("run_bytes", 0), ("row_stride", -1), ("position_bytes", 3)):
+        keep = getattr(st[0], field)
+        setattr(st[0], field, value)
+        assert lib.nsm_beam_states_set(st, 1, one, 72, None) == bad
+        setattr(st[0], field, keep)
+    re = lib.nsm_beam_reorder
+    assert re(st, one, 1, -1, 2, one, -1, None) == bad
+    assert re(st, None, 1, 1, 2, one, -1, None) == bad
+    assert re(st, one, 1, 1, 2, None, -1, None) == bad
+    assert re(st, one, 1, 1, 33, one, -1, None) == big
+    assert re(st, one, 1, 0, 2, one, -1, None) == _lib.NSM_OK
