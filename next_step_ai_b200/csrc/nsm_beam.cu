@@ -11,9 +11,9 @@
 // a running maximum and sum of exponentials per thread (fp32), and collects its
 // piece's k best as 64-bit keys (value in ordered bits, then the complement of
 // the index: every key differs, so "the k best" is one set whatever the order
-// in which threads find them).  A value enters the list only above a threshold:
-// after the first tile the smallest of 16 to 64 group maxima (at least k values
-// are that large), later the k-th best key whenever the list was cut down.
+// in which threads find them).  A value enters the list only at or above a
+// threshold, the smallest of 16 to 64 group maxima so far (at least k values are that
+// large); what the last threshold leaves is ranked by counting.
 // beam_merge_kernel, one CTA per batch item, joins the pieces: the sums in 64
 // bits, the scores of at most W * pieces * k + W candidates in 64 bits, and the
 // k best of them.
@@ -84,28 +84,11 @@ struct ScanParams {
   u64* piece_keys;                    // [rows][pieces][k]
 };
 
-template <typename T>
-__device__ __forceinline__ void unpack16(const uint4& a, const uint4& b, float* v);
-template <>
-__device__ __forceinline__ void unpack16<__half>(const uint4& a, const uint4& b, float* v) {
-  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
-}
-template <>
-__device__ __forceinline__ void unpack16<__nv_bfloat16>(const uint4& a, const uint4& b, float* v) {
-  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-}
-
+// The 16 values of a thread as they are loaded: 16-byte pieces, or one value each.
+template <typename T, bool kVec>
+struct RawTile {
+  uint32_t r[kVec ? 4 * (int)sizeof(T) : kBsPer];
+};
 // Position in the tile of value i of a thread.  kVec: runs of 16 bytes, so that
 // 16-byte loads of neighbouring lanes touch neighbouring memory; otherwise one value
 // per lane.  The mapping is the same for every row of a call: equal rows give
@@ -117,40 +100,67 @@ __device__ __forceinline__ int tile_pos(int i) {
   return (i / n) * (kBsThreads * n) + threadIdx.x * n + i % n;
 }
 
+template <typename T>
+__device__ __forceinline__ uint32_t raw_bits(T v);
+template <>
+__device__ __forceinline__ uint32_t raw_bits<float>(float v) { return __float_as_uint(v); }
+template <>
+__device__ __forceinline__ uint32_t raw_bits<__half>(__half v) { return __half_as_ushort(v); }
+template <>
+__device__ __forceinline__ uint32_t raw_bits<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
+
+template <typename T>
+constexpr uint32_t kMinusInf = sizeof(T) == 4 ? 0xff800000u : 0xff80u;  // fp32, bf16
+template <>
+constexpr uint32_t kMinusInf<__half> = 0xfc00u;
+
 template <typename T, bool kVec>
-__device__ __forceinline__ void load_tile(const T* row, int64_t at, int left, float* v) {
-  if (kVec && left >= kBsTile) {
-    constexpr int n = 16 / sizeof(T);
-    const uint4* src = reinterpret_cast<const uint4*>(row + at) + threadIdx.x;
-    if constexpr (sizeof(T) == 4) {
+__device__ __forceinline__ void load_tile(const T* row, int64_t at, int left, RawTile<T, kVec>& q) {
+  if constexpr (kVec) {
+    if (left >= kBsTile) {
+      const uint4* src = reinterpret_cast<const uint4*>(row + at) + threadIdx.x;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint4 q = ldg_stream_u4(src + i * kBsThreads);
-        v[4 * i] = __uint_as_float(q.x);
-        v[4 * i + 1] = __uint_as_float(q.y);
-        v[4 * i + 2] = __uint_as_float(q.z);
-        v[4 * i + 3] = __uint_as_float(q.w);
+      for (int i = 0; i < (int)sizeof(T); ++i) {
+        const uint4 u = ldg_stream_u4(src + i * kBsThreads);
+        q.r[4 * i] = u.x;
+        q.r[4 * i + 1] = u.y;
+        q.r[4 * i + 2] = u.z;
+        q.r[4 * i + 3] = u.w;
       }
-    } else {
-      const uint4 a = ldg_stream_u4(src), b = ldg_stream_u4(src + kBsThreads);
-      unpack16<T>(a, b, v);
+      return;
     }
-    (void)n;
-  } else {
+  }
 #pragma unroll
-    for (int i = 0; i < kBsPer; ++i) {
-      const int pos = tile_pos<T, kVec>(i);
-      v[i] = pos < left ? to_f32<T>(row[at + pos]) : -INFINITY;
+  for (int i = 0; i < kBsPer; ++i) {
+    const int pos = tile_pos<T, kVec>(i);
+    const uint32_t b = pos < left ? raw_bits<T>(row[at + pos]) : kMinusInf<T>;
+    if constexpr (kVec && sizeof(T) == 2) {
+      q.r[i / 2] = i % 2 ? q.r[i / 2] | b << 16 : b;
+    } else {
+      q.r[i] = b;
+    }
+  }
+}
+
+template <typename T, bool kVec>
+__device__ __forceinline__ void unpack_tile(const RawTile<T, kVec>& q, float* v) {
+#pragma unroll
+  for (int i = 0; i < kBsPer; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      v[i] = __uint_as_float(q.r[i]);
+    } else {
+      const uint32_t h = kVec ? (i % 2 ? q.r[i / 2] >> 16 : q.r[i / 2] & 0xffffu) : q.r[i];
+      v[i] = to_f32<T>(*reinterpret_cast<const T*>(&h));
     }
   }
 }
 
 struct ScanShared {
   u64 list[kBsCap];
-  u64 group[64];
+  uint32_t group[2][64];  // maxima of the groups, written for one tile while the other is read
   float wmax[kBsWarps], wsum[kBsWarps];
   int wcnt[kBsWarps];
-  int count;
+  int count, kept;
 };
 
 __device__ __forceinline__ int block_sum(int v, ScanShared& sh) {
@@ -164,32 +174,54 @@ __device__ __forceinline__ int block_sum(int v, ScanShared& sh) {
   return s;
 }
 
-// Cuts the list (n keys, and with kRegs the tile's values too) down to the k best
-// keys; returns the smallest of them (0 when there are at most k).  A search of the
-// k-th largest key bit by bit: 64 counts at most, and only when the list
-// filled up.
-template <typename T, bool kVec, bool kRegs>
-__device__ u64 cut_list(ScanShared& sh, int n, int k, const float* v, int64_t at, int left) {
-  u64 mine[kBsCap / kBsThreads];
+// 16, 32 or 64 groups of threads, at least k of them.  If every group has a value >= x,
+// at least k values are >= x: the smallest of the groups' maxima is a threshold.
+__device__ __forceinline__ int group_count(int k) { return k <= 16 ? 16 : k <= 32 ? 32 : 64; }
+__device__ __forceinline__ void put_group_max(uint32_t v, int groups, uint32_t* group) {
+  if (groups == 16) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if ((threadIdx.x & 31) == 0) group[threadIdx.x >> 5] = v;
+  } else {
+    const int span = kBsThreads / groups;
+    for (int o = span / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (threadIdx.x % span == 0) group[threadIdx.x / span] = v;
+  }
+}
+__device__ __forceinline__ uint32_t min_group_max(int groups, const uint32_t* group) {
+  const int lane = threadIdx.x & 31;
+  uint32_t v = group[lane & (groups - 1)];
+  if (groups == 64) v = min(v, group[lane + 32]);
+  return __reduce_min_sync(0xffffffffu, v);
+}
+
+// Cuts the list and the tile that starts at `at` (whose keys may be in the list
+// or not) down to the k best keys: a search of the k-th largest key bit by bit,
+// only when the list ran over, which takes very many equal values.  The tile is
+// read again, so that the scan keeps no registers for this.  Returns the smallest
+// key that stays, 0 when there are no more than k.
+template <typename T>
+__device__ __noinline__ u64 cut_list(ScanShared& sh, int k, const T* row, int64_t at, int left) {
+  const int n = min(sh.count, kBsCap);
+  u64 mine[kBsCap / kBsThreads], tile[kBsPer];
 #pragma unroll
   for (int i = 0; i < kBsCap / kBsThreads; ++i) {
     const int e = i * kBsThreads + threadIdx.x;
     mine[i] = e < n ? sh.list[e] : 0ull;
+    if (0xffffffffu - (uint32_t)mine[i] >= (uint32_t)at) mine[i] = 0;  // from this tile
   }
-  auto reg_key = [&](int i) {
-    const int pos = tile_pos<T, kVec>(i);
-    return pos < left ? make_key(clean(v[i]), (uint32_t)(at + pos)) : 0ull;
-  };
+#pragma unroll
+  for (int i = 0; i < kBsPer; ++i) {
+    const int pos = i * kBsThreads + threadIdx.x;
+    tile[i] = pos < left ? make_key(clean(to_f32<T>(row[at + pos])), (uint32_t)(at + pos)) : 0ull;
+  }
   u64 cut = 0;
   for (int bit = 63; bit >= 0; --bit) {
     const u64 tr = cut | (1ull << bit);
     int c = 0;
 #pragma unroll
     for (int i = 0; i < kBsCap / kBsThreads; ++i) c += mine[i] >= tr;
-    if constexpr (kRegs) {
 #pragma unroll
-      for (int i = 0; i < kBsPer; ++i) c += reg_key(i) >= tr;
-    }
+    for (int i = 0; i < kBsPer; ++i) c += tile[i] >= tr;
     c = block_sum(c, sh);
     if (c >= k) cut = tr;
     if (c == k) break;
@@ -202,10 +234,8 @@ __device__ u64 cut_list(ScanShared& sh, int n, int k, const float* v, int64_t at
   };
 #pragma unroll
   for (int i = 0; i < kBsCap / kBsThreads; ++i) keep(mine[i]);
-  if constexpr (kRegs) {
 #pragma unroll
-    for (int i = 0; i < kBsPer; ++i) keep(reg_key(i));
-  }
+  for (int i = 0; i < kBsPer; ++i) keep(tile[i]);
   __syncthreads();
   return cut;
 }
@@ -229,26 +259,38 @@ __global__ void __launch_bounds__(kBsThreads, 2) beam_scan_kernel(ScanParams p) 
   const T* src = reinterpret_cast<const T*>(p.logits) + b * p.batch_stride + w * p.beam_stride;
   const int64_t begin = (int64_t)pc * p.piece, end = min((int64_t)p.V, begin + p.piece);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x == 0) sh.count = 0;
+  const int groups = group_count(p.k);
+  if (threadIdx.x == 0) sh.count = sh.kept = 0;
 
   float m = -INFINITY, s = 0.f;
-  u64 cut = 0;  // only keys above it can be among the k best
-  for (int64_t at = begin; at < end; at += kBsTile) {
+  // Values below `cut` (in ordered bits; 0 stands for -infinity) are not among the
+  // k best; `enter` is above it where an equal value would come too late.
+  uint32_t cut = 1, enter = 1;
+  RawTile<T, kVec> next;
+  load_tile<T, kVec>(src, begin, (int)min((int64_t)kBsTile, end - begin), next);
+  int parity = 0;
+  for (int64_t at = begin; at < end; at += kBsTile, parity ^= 1) {
     const int left = (int)min((int64_t)kBsTile, end - at);
     float v[kBsPer];
-    load_tile<T, kVec>(src, at, left, v);
+    unpack_tile<T, kVec>(next, v);
+    if (at + kBsTile < end)
+      load_tile<T, kVec>(src, at + kBsTile, (int)min((int64_t)kBsTile, end - at - kBsTile), next);
     // fmaxf passes over NaN, so a tile with NaN or +infinity shows in its sum (NaN)
     // or its maximum; such a tile is cleaned and summed again
-    float tm, e;
+    float tm;
     for (int again = 0;; ++again) {
       tm = v[0];
 #pragma unroll
       for (int i = 1; i < kBsPer; ++i) tm = fmaxf(tm, v[i]);
       if (!(tm > -INFINITY)) break;  // nothing but -infinity (and NaN)
       const float nm = fmaxf(m, tm);
-      e = 0.f;
+      float e0 = 0.f, e1 = 0.f;
 #pragma unroll
-      for (int i = 0; i < kBsPer; ++i) e += exp2_fast((v[i] - nm) * kLog2e);
+      for (int i = 0; i < kBsPer; i += 2) {
+        e0 += exp2_fast((v[i] - nm) * kLog2e);
+        e1 += exp2_fast((v[i + 1] - nm) * kLog2e);
+      }
+      const float e = e0 + e1;
       if (again || (tm <= kFltMax && e == e)) {
         s = s * exp2_fast((m - nm) * kLog2e) + e;  // m = -infinity: s is 0
         m = nm;
@@ -257,64 +299,57 @@ __global__ void __launch_bounds__(kBsThreads, 2) beam_scan_kernel(ScanParams p) 
 #pragma unroll
       for (int i = 0; i < kBsPer; ++i) v[i] = clean(v[i]);
     }
-    const bool any = tm > -INFINITY;
-    if (at == begin) {
-      // at least k values are as large as the smallest of >= k group maxima
-      u64 best = 0;
-      if (any) {
-#pragma unroll
-        for (int i = 0; i < kBsPer; ++i) {
-          const u64 key = make_key(v[i], (uint32_t)(at + tile_pos<T, kVec>(i)));
-          best = key > best ? key : best;
-        }
-      }
-      const int groups = p.k <= 16 ? 16 : p.k <= 32 ? 32 : 64;
-      const int span = kBsThreads / groups;  // 32, 16 or 8 lanes
-      for (int o = span / 2; o > 0; o >>= 1) {
-        const u64 other = __shfl_xor_sync(0xffffffffu, best, o);
-        best = other > best ? other : best;
-      }
-      if (threadIdx.x % span == 0) sh.group[threadIdx.x / span] = best;
-      __syncthreads();
-      u64 lo = sh.group[lane & (groups - 1)];
-      if (groups == 64) lo = min(lo, sh.group[lane + 32]);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      cut = lo == 0 ? 0 : lo - 1;  // keys >= lo stay
-    }
-    const int before = at == begin ? 0 : sh.count;  // uniform: nothing was added since the last barrier
-    if (at != begin) __syncthreads();               // everybody has read it
-    if (any && order_f32(tm + 0.f) >= (uint32_t)(cut >> 32)) {
+    const uint32_t om = tm > -INFINITY ? order_f32(tm + 0.f) : 0u;
+    // the threshold of the running maxima: it rises from tile to tile
+    put_group_max(m > -INFINITY ? order_f32(m + 0.f) : 0u, groups, sh.group[parity]);
+    __syncthreads();
+    cut = max(cut, min_group_max(groups, sh.group[parity]));
+    enter = max(enter, cut);
+    bool over = false;
+    if (om >= enter) {
 #pragma unroll
       for (int i = 0; i < kBsPer; ++i) {
         const u64 key = make_key(v[i], (uint32_t)(at + tile_pos<T, kVec>(i)));
-        if (key > cut) {
+        if ((uint32_t)(key >> 32) >= enter) {
           const int e = atomicAdd(&sh.count, 1);
-          if (e < kBsCap) sh.list[e] = key;
+          if (e < kBsCap)
+            sh.list[e] = key;
+          else
+            over = true;
         }
       }
     }
-    __syncthreads();
-    const int n = sh.count;
-    if (n > kBsCap) {
-      cut = cut_list<T, kVec, true>(sh, before, p.k, v, at, left);
-    } else if (n > kBsCap / 2) {
-      cut = cut_list<T, kVec, false>(sh, n, p.k, v, at, left);
+    // a list that ran over is cut down at once (nobody goes on before all know)
+    if (__syncthreads_or(over)) {
+      const uint32_t c = (uint32_t)(cut_list<T>(sh, p.k, src, at, left) >> 32);
+      if (c) {
+        cut = max(cut, c);
+        enter = max(enter, c + 1);  // k keys are listed, and later indices lose against equal values
+      }
     }
   }
-  __syncthreads();
 
-  // the piece's maximum and sum
+  // the piece's maximum and sum; of the list, what the last threshold leaves
   const float wm = warp_max(m);
   if (lane == 0) sh.wmax[warp] = wm;
+  u64 mine[kBsCap / kBsThreads];
+  const int listed = sh.count;
+#pragma unroll
+  for (int i = 0; i < kBsCap / kBsThreads; ++i) {
+    const int e = i * kBsThreads + threadIdx.x;
+    mine[i] = e < listed ? sh.list[e] : 0ull;
+  }
   __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kBsCap / kBsThreads; ++i)
+    if ((uint32_t)(mine[i] >> 32) >= cut) sh.list[atomicAdd(&sh.kept, 1)] = mine[i];
   float pm = sh.wmax[0];
 #pragma unroll
   for (int i = 1; i < kBsWarps; ++i) pm = fmaxf(pm, sh.wmax[i]);
   const float ws = warp_sum(m > -INFINITY ? s * exp2_fast((m - pm) * kLog2e) : 0.f);
   if (lane == 0) sh.wsum[warp] = ws;
   __syncthreads();
-  const int n = sh.count;
+  const int n = sh.kept;
   if (threadIdx.x == 0) {
     float t = 0.f;
 #pragma unroll
@@ -326,6 +361,7 @@ __global__ void __launch_bounds__(kBsThreads, 2) beam_scan_kernel(ScanParams p) 
   for (int i = threadIdx.x; i < n; i += kBsThreads) {
     const u64 key = sh.list[i];
     int rank = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) rank += sh.list[j] > key;
     if (rank < p.k) p.piece_keys[slot * p.k + rank] = key;
   }
@@ -377,10 +413,11 @@ __global__ void __launch_bounds__(kBsThreads) beam_merge_kernel(MergeParams p) {
     u64 q = 0;
     uint32_t t = 0;
     if (i < p.W * per) {
-      const int w = i / per, r = i - w * per, pc = r / p.k, e = r - pc * p.k;
-      const int64_t slot = (int64_t)(b * p.W + w) * p.pieces + pc;
-      if (e < __ldcg(p.piece_count + slot)) {
-        const u64 x = __ldcg(p.piece_keys + slot * p.k + e);
+      const int list = i / p.k, e = i - list * p.k, w = list / p.pieces;
+      const int64_t slot = (int64_t)b * p.W * p.pieces + list;
+      const int have = __ldcg(p.piece_count + slot);
+      const u64 x = __ldcg(p.piece_keys + slot * p.k + e);  // (stale beyond the count)
+      if (e < have) {
         t = 0xffffffffu - (uint32_t)x;
         const double sc = (double)p.scores[b * p.W + w] + ((double)unorder_f32((uint32_t)(x >> 32)) - lse[w]);
         q = sc > -INFINITY ? order_f64(sc) : 0ull;
@@ -401,20 +438,14 @@ __global__ void __launch_bounds__(kBsThreads) beam_merge_kernel(MergeParams p) {
     const int w = i < p.W * per ? i / per : i - p.W * per;
     return (u64)w * (u64)p.V + tok[i];
   };
-  // a threshold as in the scan
-  const int groups = p.k <= 16 ? 16 : p.k <= 32 ? 32 : 64, span = kBsThreads / groups;
-  for (int o = span / 2; o > 0; o >>= 1) {
-    const u64 other = __shfl_xor_sync(0xffffffffu, best, o);
-    best = other > best ? other : best;
-  }
-  if (threadIdx.x % span == 0) sh.group[threadIdx.x / span] = best;
+  // a threshold as in the scan, on the upper half of the scores
+  const int groups = group_count(p.k);
+  put_group_max((uint32_t)(best >> 32), groups, sh.group[0]);
   __syncthreads();
-  u64 lo = sh.group[lane & (groups - 1)];
-  if (groups == 64) lo = min(lo, sh.group[lane + 32]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+  const uint32_t cut = min_group_max(groups, sh.group[0]);
   for (int i = threadIdx.x; i < M; i += kBsThreads) {
-    if (key[i] != 0 && key[i] >= lo) {
+    const u64 q = key[i];
+    if (q != 0 && (uint32_t)(q >> 32) >= cut) {
       const int e = atomicAdd(&sh.count, 1);
       if (e < kBsCap) sh.list[e] = (u64)i;
     }
@@ -457,9 +488,12 @@ __global__ void __launch_bounds__(kBsThreads) beam_merge_kernel(MergeParams p) {
     const int i = (int)sh.list[a];
     const u64 ki = key[i], fi = flat(i);
     int rank = 0;
+#pragma unroll 4
     for (int c = 0; c < n; ++c) {
       const int j = (int)sh.list[c];
-      rank += key[j] > ki || (key[j] == ki && flat(j) < fi);
+      const u64 kj = key[j];
+      rank += kj > ki;
+      if (kj == ki && j != i) rank += flat(j) < fi;
     }
     if (rank < p.k) found[rank] = (u64)i;
   }
