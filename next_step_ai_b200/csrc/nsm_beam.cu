@@ -89,15 +89,15 @@ template <typename T, bool kVec>
 struct RawTile {
   uint32_t r[kVec ? 4 * (int)sizeof(T) : kBsPer];
 };
-// Position in the tile of value i of a thread.  kVec: runs of 16 bytes, so that
-// 16-byte loads of neighbouring lanes touch neighbouring memory; otherwise one value
-// per lane.  The mapping is the same for every row of a call: equal rows give
-// equal sums, bit for bit.
+// Position in the tile of value i of a thread.  A full tile with kVec: runs of 16
+// bytes, so that 16-byte loads of neighbouring lanes touch neighbouring memory; otherwise
+// one value per lane, so that a short tile reaches all threads.  The mapping is the same
+// for every row of a call: equal rows give equal sums, bit for bit.
 template <typename T, bool kVec>
-__device__ __forceinline__ int tile_pos(int i) {
-  if constexpr (!kVec) return i * kBsThreads + threadIdx.x;
+__device__ __forceinline__ int tile_pos(int i, bool full) {
   constexpr int n = 16 / sizeof(T);
-  return (i / n) * (kBsThreads * n) + threadIdx.x * n + i % n;
+  if (kVec && full) return (i / n) * (kBsThreads * n) + threadIdx.x * n + i % n;
+  return i * kBsThreads + threadIdx.x;
 }
 
 template <typename T>
@@ -132,7 +132,7 @@ __device__ __forceinline__ void load_tile(const T* row, int64_t at, int left, Ra
   }
 #pragma unroll
   for (int i = 0; i < kBsPer; ++i) {
-    const int pos = tile_pos<T, kVec>(i);
+    const int pos = tile_pos<T, kVec>(i, false);
     const uint32_t b = pos < left ? raw_bits<T>(row[at + pos]) : kMinusInf<T>;
     if constexpr (kVec && sizeof(T) == 2) {
       q.r[i / 2] = i % 2 ? q.r[i / 2] | b << 16 : b;
@@ -157,7 +157,7 @@ __device__ __forceinline__ void unpack_tile(const RawTile<T, kVec>& q, float* v)
 
 struct ScanShared {
   u64 list[kBsCap];
-  uint32_t group[2][64];  // maxima of the groups, written for one tile while the other is read
+  uint32_t group[64];     // running maxima of the groups, in ordered bits
   float wmax[kBsWarps], wsum[kBsWarps];
   int wcnt[kBsWarps];
   int count, kept;
@@ -177,67 +177,88 @@ __device__ __forceinline__ int block_sum(int v, ScanShared& sh) {
 // 16, 32 or 64 groups of threads, at least k of them.  If every group has a value >= x,
 // at least k values are >= x: the smallest of the groups' maxima is a threshold.
 __device__ __forceinline__ int group_count(int k) { return k <= 16 ? 16 : k <= 32 ? 32 : 64; }
+__device__ __forceinline__ void st_relaxed(uint32_t* p, uint32_t v) {
+  asm volatile("st.relaxed.cta.shared.u32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_relaxed(const uint32_t* p) {
+  uint32_t v;
+  asm volatile("ld.relaxed.cta.shared.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory");
+  return v;
+}
 __device__ __forceinline__ void put_group_max(uint32_t v, int groups, uint32_t* group) {
   if (groups == 16) {
     v = __reduce_max_sync(0xffffffffu, v);
-    if ((threadIdx.x & 31) == 0) group[threadIdx.x >> 5] = v;
+    if ((threadIdx.x & 31) == 0) st_relaxed(group + (threadIdx.x >> 5), v);
   } else {
     const int span = kBsThreads / groups;
     for (int o = span / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if (threadIdx.x % span == 0) group[threadIdx.x / span] = v;
+    if (threadIdx.x % span == 0) st_relaxed(group + threadIdx.x / span, v);
   }
 }
 __device__ __forceinline__ uint32_t min_group_max(int groups, const uint32_t* group) {
   const int lane = threadIdx.x & 31;
-  uint32_t v = group[lane & (groups - 1)];
-  if (groups == 64) v = min(v, group[lane + 32]);
+  uint32_t v = ld_relaxed(group + (lane & (groups - 1)));
+  if (groups == 64) v = min(v, ld_relaxed(group + lane + 32));
   return __reduce_min_sync(0xffffffffu, v);
 }
 
-// Cuts the list and the tile that starts at `at` (whose keys may be in the list
-// or not) down to the k best keys: a search of the k-th largest key bit by bit,
-// only when the list ran over, which takes very many equal values.  The tile is
-// read again, so that the scan keeps no registers for this.  Returns the smallest
-// key that stays, 0 when there are no more than k.
+// The k best keys of a piece whose list ran over (it takes very many equal
+// values): tile by tile, a search of the k-th largest key bit by bit over the list so far and
+// the tile.  The values are read again, so that the scan keeps no registers for
+// this.  Leaves the keys in sh.list and their number in sh.kept.
 template <typename T>
-__device__ __noinline__ u64 cut_list(ScanShared& sh, int k, const T* row, int64_t at, int left) {
-  const int n = min(sh.count, kBsCap);
-  u64 mine[kBsCap / kBsThreads], tile[kBsPer];
-#pragma unroll
-  for (int i = 0; i < kBsCap / kBsThreads; ++i) {
-    const int e = i * kBsThreads + threadIdx.x;
-    mine[i] = e < n ? sh.list[e] : 0ull;
-    if (0xffffffffu - (uint32_t)mine[i] >= (uint32_t)at) mine[i] = 0;  // from this tile
-  }
-#pragma unroll
-  for (int i = 0; i < kBsPer; ++i) {
-    const int pos = i * kBsThreads + threadIdx.x;
-    tile[i] = pos < left ? make_key(clean(to_f32<T>(row[at + pos])), (uint32_t)(at + pos)) : 0ull;
-  }
-  u64 cut = 0;
-  for (int bit = 63; bit >= 0; --bit) {
-    const u64 tr = cut | (1ull << bit);
-    int c = 0;
-#pragma unroll
-    for (int i = 0; i < kBsCap / kBsThreads; ++i) c += mine[i] >= tr;
-#pragma unroll
-    for (int i = 0; i < kBsPer; ++i) c += tile[i] >= tr;
-    c = block_sum(c, sh);
-    if (c >= k) cut = tr;
-    if (c == k) break;
-  }
-  // the keys are unique, so exactly k are >= cut, or all are (cut stays 0)
-  if (threadIdx.x == 0) sh.count = 0;
+__device__ __noinline__ void list_again(ScanShared& sh, int k, const T* row, int64_t begin, int64_t end) {
   __syncthreads();
-  auto keep = [&](u64 key) {
-    if (key != 0 && key >= cut) sh.list[atomicAdd(&sh.count, 1)] = key;
-  };
-#pragma unroll
-  for (int i = 0; i < kBsCap / kBsThreads; ++i) keep(mine[i]);
-#pragma unroll
-  for (int i = 0; i < kBsPer; ++i) keep(tile[i]);
+  if (threadIdx.x == 0) sh.kept = 0;
   __syncthreads();
-  return cut;
+  uint32_t enter = 1;  // once k keys are listed, an equal value at a later index loses
+  for (int64_t at = begin; at < end; at += kBsTile) {
+    const int n = sh.kept;  // at most k
+    const u64 mine = (int)threadIdx.x < n ? sh.list[threadIdx.x] : 0ull;
+    u64 tile[kBsPer];
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < kBsPer; ++i) {
+      const int64_t pos = at + i * kBsThreads + threadIdx.x;
+      tile[i] = pos < end ? make_key(clean(to_f32<T>(row[pos])), (uint32_t)pos) : 0ull;
+      if ((uint32_t)(tile[i] >> 32) < enter) tile[i] = 0;
+      any |= tile[i] != 0;
+    }
+    if (!__syncthreads_or(any)) continue;
+    u64 cut = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      const u64 tr = cut | (1ull << bit);
+      int c = mine >= tr;
+#pragma unroll
+      for (int i = 0; i < kBsPer; ++i) c += tile[i] >= tr;
+      c = block_sum(c, sh);
+      if (c >= k) cut = tr;
+      if (c == k) break;
+    }
+    // the keys are unique, so exactly k are >= cut, or all are (cut stays 0)
+    if (threadIdx.x == 0) sh.kept = 0;
+    __syncthreads();
+    auto keep = [&](u64 key) {
+      if (key != 0 && key >= cut) sh.list[atomicAdd(&sh.kept, 1)] = key;
+    };
+    keep(mine);
+#pragma unroll
+    for (int i = 0; i < kBsPer; ++i) keep(tile[i]);
+    __syncthreads();
+    if (cut) enter = (uint32_t)(cut >> 32) + 1;
+  }
+  __syncthreads();
+}
+
+// Rank of each of the n keys among all: eight threads count for one key.
+__device__ __forceinline__ int count_above(const u64* list, int n, u64 key, int part) {
+  int rank = 0;
+#pragma unroll 4
+  for (int j = part; j < n; j += 8) rank += list[j] > key;
+  rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+  rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+  rank += __shfl_xor_sync(0xffffffffu, rank, 4);
+  return rank;
 }
 
 template <typename T, bool kVec>
@@ -263,14 +284,10 @@ __global__ void __launch_bounds__(kBsThreads, 2) beam_scan_kernel(ScanParams p) 
   if (threadIdx.x == 0) sh.count = sh.kept = 0;
 
   float m = -INFINITY, s = 0.f;
-  // Values below `cut` (in ordered bits; 0 stands for -infinity) are not among the
-  // k best; `enter` is above it where an equal value would come too late.
-  uint32_t cut = 1, enter = 1;
+  bool over = false;
   RawTile<T, kVec> next;
   load_tile<T, kVec>(src, begin, (int)min((int64_t)kBsTile, end - begin), next);
-  int parity = 0;
-  for (int64_t at = begin; at < end; at += kBsTile, parity ^= 1) {
-    const int left = (int)min((int64_t)kBsTile, end - at);
+  for (int64_t at = begin; at < end; at += kBsTile) {
     float v[kBsPer];
     unpack_tile<T, kVec>(next, v);
     if (at + kBsTile < end)
@@ -299,32 +316,23 @@ __global__ void __launch_bounds__(kBsThreads, 2) beam_scan_kernel(ScanParams p) 
 #pragma unroll
       for (int i = 0; i < kBsPer; ++i) v[i] = clean(v[i]);
     }
-    const uint32_t om = tm > -INFINITY ? order_f32(tm + 0.f) : 0u;
-    // the threshold of the running maxima: it rises from tile to tile
-    put_group_max(m > -INFINITY ? order_f32(m + 0.f) : 0u, groups, sh.group[parity]);
-    __syncthreads();
-    cut = max(cut, min_group_max(groups, sh.group[parity]));
-    enter = max(enter, cut);
-    bool over = false;
-    if (om >= enter) {
+    // The threshold of the running maxima.  All groups have to be in it once; after
+    // that a maximum that is not up to date is only a lower threshold.
+    put_group_max(m > -INFINITY ? order_f32(m + 0.f) : 0u, groups, sh.group);
+    if (at == begin) __syncthreads();
+    const uint32_t cut = min_group_max(groups, sh.group);
+    const float thr = cut ? unorder_f32(cut) : -kFltMax;
+    if (tm >= thr) {
+      const bool full = end - at >= kBsTile;
 #pragma unroll
       for (int i = 0; i < kBsPer; ++i) {
-        const u64 key = make_key(v[i], (uint32_t)(at + tile_pos<T, kVec>(i)));
-        if ((uint32_t)(key >> 32) >= enter) {
+        if (v[i] >= thr) {
           const int e = atomicAdd(&sh.count, 1);
           if (e < kBsCap)
-            sh.list[e] = key;
+            sh.list[e] = make_key(v[i], (uint32_t)(at + tile_pos<T, kVec>(i, full)));
           else
             over = true;
         }
-      }
-    }
-    // a list that ran over is cut down at once (nobody goes on before all know)
-    if (__syncthreads_or(over)) {
-      const uint32_t c = (uint32_t)(cut_list<T>(sh, p.k, src, at, left) >> 32);
-      if (c) {
-        cut = max(cut, c);
-        enter = max(enter, c + 1);  // k keys are listed, and later indices lose against equal values
       }
     }
   }
@@ -332,23 +340,30 @@ __global__ void __launch_bounds__(kBsThreads, 2) beam_scan_kernel(ScanParams p) 
   // the piece's maximum and sum; of the list, what the last threshold leaves
   const float wm = warp_max(m);
   if (lane == 0) sh.wmax[warp] = wm;
-  u64 mine[kBsCap / kBsThreads];
-  const int listed = sh.count;
-#pragma unroll
-  for (int i = 0; i < kBsCap / kBsThreads; ++i) {
-    const int e = i * kBsThreads + threadIdx.x;
-    mine[i] = e < listed ? sh.list[e] : 0ull;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kBsCap / kBsThreads; ++i)
-    if ((uint32_t)(mine[i] >> 32) >= cut) sh.list[atomicAdd(&sh.kept, 1)] = mine[i];
+  over = __syncthreads_or(over);
   float pm = sh.wmax[0];
 #pragma unroll
   for (int i = 1; i < kBsWarps; ++i) pm = fmaxf(pm, sh.wmax[i]);
   const float ws = warp_sum(m > -INFINITY ? s * exp2_fast((m - pm) * kLog2e) : 0.f);
   if (lane == 0) sh.wsum[warp] = ws;
-  __syncthreads();
+  if (over) {
+    list_again<T>(sh, p.k, src, begin, end);
+  } else {
+    u64 mine[kBsCap / kBsThreads];
+    const int listed = sh.count;
+    const uint32_t cut = min_group_max(groups, sh.group);
+#pragma unroll
+    for (int i = 0; i < kBsCap / kBsThreads; ++i) {
+      const int e = i * kBsThreads + threadIdx.x;
+      mine[i] = e < listed ? sh.list[e] : 0ull;
+      if ((uint32_t)(mine[i] >> 32) < cut) mine[i] = 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kBsCap / kBsThreads; ++i)
+      if (mine[i]) sh.list[atomicAdd(&sh.kept, 1)] = mine[i];
+    __syncthreads();
+  }
   const int n = sh.kept;
   if (threadIdx.x == 0) {
     float t = 0.f;
@@ -358,12 +373,11 @@ __global__ void __launch_bounds__(kBsThreads, 2) beam_scan_kernel(ScanParams p) 
     p.piece_sum[slot] = t;
     p.piece_count[slot] = min(n, p.k);
   }
-  for (int i = threadIdx.x; i < n; i += kBsThreads) {
-    const u64 key = sh.list[i];
-    int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) rank += sh.list[j] > key;
-    if (rank < p.k) p.piece_keys[slot * p.k + rank] = key;
+  for (int i0 = 0; i0 < n; i0 += kBsThreads / 8) {  // uniform: the shuffles need whole warps
+    const int i = i0 + (threadIdx.x >> 3);
+    const u64 key = i < n ? sh.list[i] : 0ull;
+    const int rank = count_above(sh.list, n, key, threadIdx.x & 7);
+    if (i < n && rank < p.k && (threadIdx.x & 7) == 0) p.piece_keys[slot * p.k + rank] = key;
   }
 }
 
@@ -383,46 +397,52 @@ struct MergeParams {
 __global__ void __launch_bounds__(kBsThreads) beam_merge_kernel(MergeParams p) {
   extern __shared__ __align__(16) unsigned char bm_smem[];
   __shared__ ScanShared sh;
+  __shared__ u64 at_flat[kBsCap];  // the flat indices of sh.list's candidates
   __shared__ double lse[kBsMaxBeams];
-  __shared__ u64 found[kBsMaxK];
-  const int M = p.W * p.pieces * p.k + p.W;
-  u64* key = reinterpret_cast<u64*>(bm_smem);                 // [M] score, 0 = none
-  uint32_t* tok = reinterpret_cast<uint32_t*>(key + M);       // [M]
+  const int per = p.pieces * p.k, M = p.W * per + p.W;
+  u64* key = reinterpret_cast<u64*>(bm_smem);            // [M] scores in ordered bits, 0 = none
+  uint32_t* tok = reinterpret_cast<uint32_t*>(key + M);  // [M]
   const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) sh.count = 0;
   pdl_wait();
+  const int64_t lists = (int64_t)b * p.W * p.pieces;
+  // a candidate's key and token, as the scan left them; the first ones are on their way while
+  // the sums are joined
+  auto fetch = [&](int i) -> u64 {
+    if (i >= p.W * per) return 0ull;
+    const int list = i / p.k, e = i - list * p.k;
+    const int have = __ldcg(p.piece_count + lists + list);
+    const u64 x = __ldcg(p.piece_keys + (lists + list) * p.k + e);  // (stale beyond the count)
+    return e < have ? x : 0ull;
+  };
+  u64 first = fetch(threadIdx.x);
   for (int w = warp; w < p.W; w += kBsWarps) {
-    const int64_t base = (int64_t)(b * p.W + w) * p.pieces;
-    float m = -INFINITY;
+    const int64_t base = lists + (int64_t)w * p.pieces;
+    float m = -INFINITY, q = -INFINITY, u = 0.f;  // the warp's pieces one by one per lane
     for (int i = lane; i < p.pieces; i += 32) m = fmaxf(m, __ldcg(p.piece_max + base + i));
     m = warp_max(m);
     double s = 0.0;
     for (int i = lane; i < p.pieces; i += 32) {
-      const float pm = __ldcg(p.piece_max + base + i);
-      if (pm > -INFINITY) s += (double)__ldcg(p.piece_sum + base + i) * exp((double)pm - (double)m);
+      q = __ldcg(p.piece_max + base + i);
+      u = __ldcg(p.piece_sum + base + i);
+      if (q > -INFINITY) s += (double)u * exp((double)q - (double)m);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane == 0) lse[w] = m > -INFINITY ? (double)m + log(s) : 0.0;
   }
-  if (threadIdx.x == 0) sh.count = 0;
-  if (threadIdx.x < kBsMaxK) found[threadIdx.x] = ~0ull;
   __syncthreads();
-  const int per = p.pieces * p.k;
   u64 best = 0;
   for (int i = threadIdx.x; i < M; i += kBsThreads) {
+    const u64 x = i == (int)threadIdx.x ? first : fetch(i);
     u64 q = 0;
     uint32_t t = 0;
-    if (i < p.W * per) {
-      const int list = i / p.k, e = i - list * p.k, w = list / p.pieces;
-      const int64_t slot = (int64_t)b * p.W * p.pieces + list;
-      const int have = __ldcg(p.piece_count + slot);
-      const u64 x = __ldcg(p.piece_keys + slot * p.k + e);  // (stale beyond the count)
-      if (e < have) {
-        t = 0xffffffffu - (uint32_t)x;
-        const double sc = (double)p.scores[b * p.W + w] + ((double)unorder_f32((uint32_t)(x >> 32)) - lse[w]);
-        q = sc > -INFINITY ? order_f64(sc) : 0ull;
-      }
-    } else {
+    if (x) {
+      const int w = i / per;
+      t = 0xffffffffu - (uint32_t)x;
+      const double sc = (double)p.scores[b * p.W + w] + ((double)unorder_f32((uint32_t)(x >> 32)) - lse[w]);
+      q = sc > -INFINITY ? order_f64(sc) : 0ull;
+    } else if (i >= p.W * per) {
       const int w = i - p.W * per;  // a finished beam goes on as it is
       const float sc = p.scores[b * p.W + w];
       if (p.finished && p.finished[b * p.W + w] && sc > -INFINITY) {
@@ -434,20 +454,21 @@ __global__ void __launch_bounds__(kBsThreads) beam_merge_kernel(MergeParams p) {
     tok[i] = t;
     best = q > best ? q : best;
   }
-  auto flat = [&](int i) {
-    const int w = i < p.W * per ? i / per : i - p.W * per;
-    return (u64)w * (u64)p.V + tok[i];
-  };
+  auto beam_of = [&](int i) { return i < p.W * per ? i / per : i - p.W * per; };
+  auto flat = [&](int i) { return (u64)beam_of(i) * (u64)p.V + tok[i]; };
   // a threshold as in the scan, on the upper half of the scores
   const int groups = group_count(p.k);
-  put_group_max((uint32_t)(best >> 32), groups, sh.group[0]);
+  put_group_max((uint32_t)(best >> 32), groups, sh.group);
   __syncthreads();
-  const uint32_t cut = min_group_max(groups, sh.group[0]);
+  const uint32_t cut = min_group_max(groups, sh.group);
   for (int i = threadIdx.x; i < M; i += kBsThreads) {
     const u64 q = key[i];
     if (q != 0 && (uint32_t)(q >> 32) >= cut) {
       const int e = atomicAdd(&sh.count, 1);
-      if (e < kBsCap) sh.list[e] = (u64)i;
+      if (e < kBsCap) {
+        sh.list[e] = q;
+        at_flat[e] = flat(i);
+      }
     }
   }
   __syncthreads();
@@ -478,38 +499,39 @@ __global__ void __launch_bounds__(kBsThreads) beam_merge_kernel(MergeParams p) {
     for (int i = threadIdx.x; i < M; i += kBsThreads) {
       if (key[i] != 0 && (key[i] > ck || (key[i] == ck && ~flat(i) >= cf))) {
         const int e = atomicAdd(&sh.count, 1);
-        if (e < kBsCap) sh.list[e] = (u64)i;
+        if (e < kBsCap) {
+          sh.list[e] = key[i];
+          at_flat[e] = flat(i);
+        }
       }
     }
     __syncthreads();
     n = min(sh.count, kBsCap);
   }
-  for (int a = threadIdx.x; a < n; a += kBsThreads) {
-    const int i = (int)sh.list[a];
-    const u64 ki = key[i], fi = flat(i);
+  const int64_t out = (int64_t)b * p.k;
+  for (int i0 = 0; i0 < n; i0 += kBsThreads / 8) {  // eight threads count for one candidate
+    const int i = i0 + (threadIdx.x >> 3);
+    const u64 ki = i < n ? sh.list[i] : ~0ull, fi = i < n ? at_flat[i] : 0ull;
     int rank = 0;
 #pragma unroll 4
-    for (int c = 0; c < n; ++c) {
-      const int j = (int)sh.list[c];
-      const u64 kj = key[j];
-      rank += kj > ki;
-      if (kj == ki && j != i) rank += flat(j) < fi;
+    for (int j = threadIdx.x & 7; j < n; j += 8) {
+      const u64 kj = sh.list[j], fj = at_flat[j];
+      rank += kj > ki || (kj == ki && fj < fi);
     }
-    if (rank < p.k) found[rank] = (u64)i;
+    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+    rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+    rank += __shfl_xor_sync(0xffffffffu, rank, 4);
+    if (i < n && rank < p.k && (threadIdx.x & 7) == 0) {
+      const u64 w = fi / (u64)p.V;
+      p.out_scores[out + rank] = (float)unorder_f64(ki);
+      p.out_tokens[out + rank] = (int64_t)(fi - w * (u64)p.V);
+      p.out_parents[out + rank] = (int64_t)w;
+    }
   }
-  __syncthreads();
-  if (threadIdx.x < p.k) {
-    const int64_t o = (int64_t)b * p.k + threadIdx.x;
-    const u64 i = found[threadIdx.x];
-    if (i == ~0ull) {
-      p.out_scores[o] = -INFINITY;
-      p.out_tokens[o] = -1;
-      p.out_parents[o] = 0;
-    } else {
-      p.out_scores[o] = (float)unorder_f64(key[i]);
-      p.out_tokens[o] = (int64_t)tok[i];
-      p.out_parents[o] = (int64_t)((int)i < p.W * per ? (int)i / per : (int)i - p.W * per);
-    }
+  for (int r = n + threadIdx.x; r < p.k; r += kBsThreads) {  // too few candidates
+    p.out_scores[out + r] = -INFINITY;
+    p.out_tokens[out + r] = -1;
+    p.out_parents[out + r] = 0;
   }
 }
 
