@@ -6,17 +6,18 @@
 //   score[w] + logit[w][v] - logsumexp(logit[w][:])
 //
 // and the k best are wanted, equal scores in the order of w, then v.  Inside one
-// beam the order of the scores is the order of the logits, so the logits are
-// read once (beam_scan_kernel): a CTA takes a contiguous piece of a row, keeps
-// a running maximum and sum of exponentials per thread (fp32), and collects its
-// piece's k best as 64-bit keys (value in ordered bits, then the complement of
-// the index: every key differs, so "the k best" is one set whatever the order
-// in which threads find them).  A value enters the list only at or above a
-// threshold, the smallest of 16 to 64 group maxima so far (at least k values are that
-// large); what the last threshold leaves is ranked by counting.
-// beam_merge_kernel, one CTA per batch item, joins the pieces: the sums in 64
-// bits, the scores of at most W * pieces * k + W candidates in 64 bits, and the
-// k best of them.
+// beam the order of the scores is the order of the logits.  beam_scan_kernel reads
+// the logits once and selects nothing: a warp takes a contiguous piece of a row,
+// 1024 values at a time in registers, keeps a running maximum and sum of exponentials per
+// lane (fp32), and notes the largest value of each block of 1024.
+// beam_merge_kernel, one CTA per batch item, joins the sums (in 64 bits) and picks
+// the k best blocks by (largest score, position).  The k best candidates are in
+// them: any candidate of another block is beaten by the largest of each of these k,
+// equal scores included, since blocks are contiguous and in the order of the
+// candidates.  Their values are read again (from L2), scored in 64 bits, and those
+// that reach the k-th block's largest, hardly more than k, are ranked by counting.
+// What bounds the scan is the issue of its instructions for 16-bit logits (about 6 per value)
+// and HBM for fp32.
 //
 // Reordering.  beam_reorder_kernel moves the states in place: a thread owns
 // one 1- to 16-byte column of all beams of a batch item, loads the beams that
@@ -33,14 +34,16 @@ namespace {
 
 using u64 = unsigned long long;
 
-constexpr int kBsThreads = 512;
+constexpr int kBsThreads = 256;
 constexpr int kBsWarps = kBsThreads / 32;
-constexpr int kBsPer = 16;                       // values per thread and tile
-constexpr int kBsTile = kBsThreads * kBsPer;
-constexpr int kBsCap = 1024;                     // keys of the candidate list
+constexpr int kBsPer = 32;                       // values per lane
+constexpr int kBsBlock = 32 * kBsPer;            // values of a block: one warp's registers
+constexpr int kBsMaxEntries = 384;               // noted maxima of a row
+constexpr int kBmThreads = 512;                  // of the merge
+constexpr int kBmWarps = kBmThreads / 32;
+constexpr int kBmCap = 2048;                     // candidates ranked by counting
 constexpr int kBsMaxK = 64;
 constexpr int kBsMaxBeams = 32;
-constexpr int kBsMaxMerge = 12288;               // candidates of one merge (12 bytes each in shared memory)
 constexpr float kFltMax = 3.4028234663852886e38f;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -68,8 +71,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // +infinity then share the whole probability.
 __device__ __forceinline__ float clean(float v) { return fminf(fmaxf(v, -INFINITY), kFltMax); }
 // 0 = no candidate (-infinity); -0 counts as 0
-__device__ __forceinline__ u64 make_key(float v, uint32_t idx) {
-  return v == -INFINITY ? 0ull : ((u64)order_f32(v + 0.f) << 32) | (0xffffffffu - idx);
+__device__ __forceinline__ uint32_t order_clean(float v) {
+  v = clean(v);
+  return v == -INFINITY ? 0u : order_f32(v + 0.f);
 }
 
 struct ScanParams {
@@ -77,27 +81,104 @@ struct ScanParams {
   int64_t batch_stride, beam_stride;  // elements
   const float* scores;                // [B][W]
   const uint8_t* finished;            // [B][W] or NULL
-  int W, V, k, pieces, piece;         // piece = elements per CTA, a multiple of the tile
-  float* piece_max;                   // [rows][pieces]
-  float* piece_sum;
-  int* piece_count;
-  u64* piece_keys;                    // [rows][pieces][k]
+  int rows, W, V;
+  int segs, seg_blocks;               // warps per row, blocks of 1024 per warp (a multiple of run)
+  int entries, run;                   // noted maxima per row, blocks of each
+  float2* seg;                        // [rows][segs] maximum, sum of exp(value - maximum)
+  uint32_t* top;                      // [rows][entries] largest value in ordered bits
 };
 
-// The 16 values of a thread as they are loaded: 16-byte pieces, or one value each.
-template <typename T, bool kVec>
+// The values of a thread as they are loaded; 16-bit types two to a word.
+template <typename T>
 struct RawTile {
-  uint32_t r[kVec ? 4 * (int)sizeof(T) : kBsPer];
+  uint32_t r[kBsPer * (int)sizeof(T) / 4];
 };
-// Position in the tile of value i of a thread.  A full tile with kVec: runs of 16
+template <typename T>
+__device__ __forceinline__ float raw_value(uint32_t word, int i) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(word);
+  } else if constexpr (sizeof(T) == 2 && __is_same(T, __nv_bfloat16)) {
+    return __uint_as_float(i % 2 ? word & 0xffff0000u : word << 16);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&word));
+    return i % 2 ? f.y : f.x;
+  }
+}
+template <typename T>
+__device__ __forceinline__ float raw_value(const RawTile<T>& q, int i) {
+  return raw_value<T>(q.r[i * (int)sizeof(T) / 4], i);
+}
+// The largest value (NaN is passed over); 16-bit types two at a time.
+template <typename T>
+__device__ __forceinline__ float raw_max(const RawTile<T>& q) {
+  if constexpr (sizeof(T) == 4) {
+    float m = __uint_as_float(q.r[0]);
+#pragma unroll
+    for (int i = 1; i < kBsPer; ++i) m = fmaxf(m, __uint_as_float(q.r[i]));
+    return m;
+  } else if constexpr (__is_same(T, __nv_bfloat16)) {
+    __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162*>(&q.r[0]);
+#pragma unroll
+    for (int i = 1; i < kBsPer / 2; ++i) m = __hmax2(m, *reinterpret_cast<const __nv_bfloat162*>(&q.r[i]));
+    return fmaxf(__low2float(m), __high2float(m));
+  } else {
+    __half2 m = *reinterpret_cast<const __half2*>(&q.r[0]);
+#pragma unroll
+    for (int i = 1; i < kBsPer / 2; ++i) m = __hmax2(m, *reinterpret_cast<const __half2*>(&q.r[i]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+}
+
+// Two fp32 values in one register pair: one instruction works on both.
+__device__ __forceinline__ u64 pair2(float a, float b) {
+  u64 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair2(u64 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+  u64 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
+  u64 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// sum of exp(value - top) over the thread's values
+template <typename T, bool kClean>
+__device__ __forceinline__ float raw_exp_sum(const RawTile<T>& q, float top) {
+  const u64 off = pair2(-top, -top), l2e = pair2(kLog2e, kLog2e);
+  u64 sum[2] = {0, 0};  // two chains of two sums
+#pragma unroll
+  for (int i = 0; i < kBsPer; i += 2) {
+    float a = raw_value<T>(q, i), b = raw_value<T>(q, i + 1);
+    if (kClean) {
+      a = clean(a);
+      b = clean(b);
+    }
+    const float2 x = unpair2(mul2(add2(pair2(a, b), off), l2e));
+    sum[(i / 2) % 2] = add2(sum[(i / 2) % 2], pair2(exp2_fast(x.x), exp2_fast(x.y)));
+  }
+  const float2 t = unpair2(add2(sum[0], sum[1]));
+  return t.x + t.y;
+}
+
+// Position in the block of value i of a lane.  A full block with kVec: runs of 16
 // bytes, so that 16-byte loads of neighbouring lanes touch neighbouring memory; otherwise
-// one value per lane, so that a short tile reaches all threads.  The mapping is the same
-// for every row of a call: equal rows give equal sums, bit for bit.
+// one value per lane.  The mapping is the same for every row of a call: equal rows give
+// equal sums, bit for bit.
 template <typename T, bool kVec>
-__device__ __forceinline__ int tile_pos(int i, bool full) {
+__device__ __forceinline__ int block_pos(int i, bool full) {
   constexpr int n = 16 / sizeof(T);
-  if (kVec && full) return (i / n) * (kBsThreads * n) + threadIdx.x * n + i % n;
-  return i * kBsThreads + threadIdx.x;
+  const int lane = threadIdx.x & 31;
+  if (kVec && full) return (i / n) * (32 * n) + lane * n + i % n;
+  return i * 32 + lane;
 }
 
 template <typename T>
@@ -114,14 +195,15 @@ constexpr uint32_t kMinusInf = sizeof(T) == 4 ? 0xff800000u : 0xff80u;  // fp32,
 template <>
 constexpr uint32_t kMinusInf<__half> = 0xfc00u;
 
+// Block values [at, at + left) of a row (left > 0); beyond it -infinity.
 template <typename T, bool kVec>
-__device__ __forceinline__ void load_tile(const T* row, int64_t at, int left, RawTile<T, kVec>& q) {
+__device__ __forceinline__ void load_block(const T* row, int64_t at, int left, RawTile<T>& q) {
   if constexpr (kVec) {
-    if (left >= kBsTile) {
-      const uint4* src = reinterpret_cast<const uint4*>(row + at) + threadIdx.x;
+    if (left >= kBsBlock) {
+      const uint4* src = reinterpret_cast<const uint4*>(row + at) + (threadIdx.x & 31);
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T); ++i) {
-        const uint4 u = ldg_stream_u4(src + i * kBsThreads);
+      for (int i = 0; i < kBsPer * (int)sizeof(T) / 16; ++i) {
+        const uint4 u = ldg_stream_u4(src + i * 32);
         q.r[4 * i] = u.x;
         q.r[4 * i + 1] = u.y;
         q.r[4 * i + 2] = u.z;
@@ -132,9 +214,9 @@ __device__ __forceinline__ void load_tile(const T* row, int64_t at, int left, Ra
   }
 #pragma unroll
   for (int i = 0; i < kBsPer; ++i) {
-    const int pos = tile_pos<T, kVec>(i, false);
+    const int pos = block_pos<T, kVec>(i, false);
     const uint32_t b = pos < left ? raw_bits<T>(row[at + pos]) : kMinusInf<T>;
-    if constexpr (kVec && sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 2) {
       q.r[i / 2] = i % 2 ? q.r[i / 2] | b << 16 : b;
     } else {
       q.r[i] = b;
@@ -143,428 +225,309 @@ __device__ __forceinline__ void load_tile(const T* row, int64_t at, int left, Ra
 }
 
 template <typename T, bool kVec>
-__device__ __forceinline__ void unpack_tile(const RawTile<T, kVec>& q, float* v) {
-#pragma unroll
-  for (int i = 0; i < kBsPer; ++i) {
-    if constexpr (sizeof(T) == 4) {
-      v[i] = __uint_as_float(q.r[i]);
-    } else {
-      const uint32_t h = kVec ? (i % 2 ? q.r[i / 2] >> 16 : q.r[i / 2] & 0xffffu) : q.r[i];
-      v[i] = to_f32<T>(*reinterpret_cast<const T*>(&h));
-    }
-  }
-}
-
-struct ScanShared {
-  u64 list[kBsCap];
-  uint32_t group[64];     // running maxima of the groups, in ordered bits
-  float wmax[kBsWarps], wsum[kBsWarps];
-  int wcnt[kBsWarps];
-  int count, kept;
-};
-
-__device__ __forceinline__ int block_sum(int v, ScanShared& sh) {
-  v = __reduce_add_sync(0xffffffffu, v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh.wcnt[threadIdx.x >> 5] = v;
-  __syncthreads();
-  int s = 0;
-#pragma unroll
-  for (int w = 0; w < kBsWarps; ++w) s += sh.wcnt[w];
-  return s;
-}
-
-// 16, 32 or 64 groups of threads, at least k of them.  If every group has a value >= x,
-// at least k values are >= x: the smallest of the groups' maxima is a threshold.
-__device__ __forceinline__ int group_count(int k) { return k <= 16 ? 16 : k <= 32 ? 32 : 64; }
-__device__ __forceinline__ void st_relaxed(uint32_t* p, uint32_t v) {
-  asm volatile("st.relaxed.cta.shared.u32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
-}
-__device__ __forceinline__ uint32_t ld_relaxed(const uint32_t* p) {
-  uint32_t v;
-  asm volatile("ld.relaxed.cta.shared.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory");
-  return v;
-}
-__device__ __forceinline__ void put_group_max(uint32_t v, int groups, uint32_t* group) {
-  if (groups == 16) {
-    v = __reduce_max_sync(0xffffffffu, v);
-    if ((threadIdx.x & 31) == 0) st_relaxed(group + (threadIdx.x >> 5), v);
-  } else {
-    const int span = kBsThreads / groups;
-    for (int o = span / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if (threadIdx.x % span == 0) st_relaxed(group + threadIdx.x / span, v);
-  }
-}
-__device__ __forceinline__ uint32_t min_group_max(int groups, const uint32_t* group) {
-  const int lane = threadIdx.x & 31;
-  uint32_t v = ld_relaxed(group + (lane & (groups - 1)));
-  if (groups == 64) v = min(v, ld_relaxed(group + lane + 32));
-  return __reduce_min_sync(0xffffffffu, v);
-}
-
-// The k best keys of a piece whose list ran over (it takes very many equal
-// values): tile by tile, a search of the k-th largest key bit by bit over the list so far and
-// the tile.  The values are read again, so that the scan keeps no registers for
-// this.  Leaves the keys in sh.list and their number in sh.kept.
-template <typename T>
-__device__ __noinline__ void list_again(ScanShared& sh, int k, const T* row, int64_t begin, int64_t end) {
-  __syncthreads();
-  if (threadIdx.x == 0) sh.kept = 0;
-  __syncthreads();
-  uint32_t enter = 1;  // once k keys are listed, an equal value at a later index loses
-  for (int64_t at = begin; at < end; at += kBsTile) {
-    const int n = sh.kept;  // at most k
-    const u64 mine = (int)threadIdx.x < n ? sh.list[threadIdx.x] : 0ull;
-    u64 tile[kBsPer];
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < kBsPer; ++i) {
-      const int64_t pos = at + i * kBsThreads + threadIdx.x;
-      tile[i] = pos < end ? make_key(clean(to_f32<T>(row[pos])), (uint32_t)pos) : 0ull;
-      if ((uint32_t)(tile[i] >> 32) < enter) tile[i] = 0;
-      any |= tile[i] != 0;
-    }
-    if (!__syncthreads_or(any)) continue;
-    u64 cut = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-      const u64 tr = cut | (1ull << bit);
-      int c = mine >= tr;
-#pragma unroll
-      for (int i = 0; i < kBsPer; ++i) c += tile[i] >= tr;
-      c = block_sum(c, sh);
-      if (c >= k) cut = tr;
-      if (c == k) break;
-    }
-    // the keys are unique, so exactly k are >= cut, or all are (cut stays 0)
-    if (threadIdx.x == 0) sh.kept = 0;
-    __syncthreads();
-    auto keep = [&](u64 key) {
-      if (key != 0 && key >= cut) sh.list[atomicAdd(&sh.kept, 1)] = key;
-    };
-    keep(mine);
-#pragma unroll
-    for (int i = 0; i < kBsPer; ++i) keep(tile[i]);
-    __syncthreads();
-    if (cut) enter = (uint32_t)(cut >> 32) + 1;
-  }
-  __syncthreads();
-}
-
-// Rank of each of the n keys among all: eight threads count for one key.
-__device__ __forceinline__ int count_above(const u64* list, int n, u64 key, int part) {
-  int rank = 0;
-#pragma unroll 4
-  for (int j = part; j < n; j += 8) rank += list[j] > key;
-  rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-  rank += __shfl_xor_sync(0xffffffffu, rank, 2);
-  rank += __shfl_xor_sync(0xffffffffu, rank, 4);
-  return rank;
-}
-
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(kBsThreads, 2) beam_scan_kernel(ScanParams p) {
-  __shared__ ScanShared sh;
+__global__ void __launch_bounds__(kBsThreads, 4) beam_scan_kernel(ScanParams p) {
   pdl_trigger();
-  const int row = blockIdx.x / p.pieces, pc = blockIdx.x - row * p.pieces;
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = (int64_t)blockIdx.x * kBsWarps + (threadIdx.x >> 5);
+  const int row = (int)(unit / p.segs), sg = (int)(unit - (int64_t)row * p.segs);
+  // a beam that is out (no score above -infinity) or finished is not read, here or later
+  if (row >= p.rows || !(p.scores[row] > -INFINITY) || (p.finished && p.finished[row])) return;
   const int b = row / p.W, w = row - b * p.W;
-  const int64_t slot = (int64_t)row * p.pieces + pc;
-  // a beam that is out (no score above -infinity) or finished is not read
-  if (!(p.scores[row] > -INFINITY) || (p.finished && p.finished[row])) {
-    if (threadIdx.x == 0) {
-      p.piece_max[slot] = -INFINITY;
-      p.piece_sum[slot] = 0.f;
-      p.piece_count[slot] = 0;
-    }
-    return;
-  }
   const T* src = reinterpret_cast<const T*>(p.logits) + b * p.batch_stride + w * p.beam_stride;
-  const int64_t begin = (int64_t)pc * p.piece, end = min((int64_t)p.V, begin + p.piece);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int groups = group_count(p.k);
-  if (threadIdx.x == 0) sh.count = sh.kept = 0;
-
-  float m = -INFINITY, s = 0.f;
-  bool over = false;
-  RawTile<T, kVec> next;
-  load_tile<T, kVec>(src, begin, (int)min((int64_t)kBsTile, end - begin), next);
-  for (int64_t at = begin; at < end; at += kBsTile) {
-    float v[kBsPer];
-    unpack_tile<T, kVec>(next, v);
-    if (at + kBsTile < end)
-      load_tile<T, kVec>(src, at + kBsTile, (int)min((int64_t)kBsTile, end - at - kBsTile), next);
-    // fmaxf passes over NaN, so a tile with NaN or +infinity shows in its sum (NaN)
-    // or its maximum; such a tile is cleaned and summed again
-    float tm;
-    for (int again = 0;; ++again) {
-      tm = v[0];
-#pragma unroll
-      for (int i = 1; i < kBsPer; ++i) tm = fmaxf(tm, v[i]);
-      if (!(tm > -INFINITY)) break;  // nothing but -infinity (and NaN)
-      const float nm = fmaxf(m, tm);
-      float e0 = 0.f, e1 = 0.f;
-#pragma unroll
-      for (int i = 0; i < kBsPer; i += 2) {
-        e0 += exp2_fast((v[i] - nm) * kLog2e);
-        e1 += exp2_fast((v[i + 1] - nm) * kLog2e);
-      }
-      const float e = e0 + e1;
-      if (again || (tm <= kFltMax && e == e)) {
-        s = s * exp2_fast((m - nm) * kLog2e) + e;  // m = -infinity: s is 0
-        m = nm;
-        break;
-      }
-#pragma unroll
-      for (int i = 0; i < kBsPer; ++i) v[i] = clean(v[i]);
+  const int64_t begin = (int64_t)sg * p.seg_blocks * kBsBlock;
+  const int64_t end = min((int64_t)p.V, begin + (int64_t)p.seg_blocks * kBsBlock);
+  float m = -INFINITY, s = 0.f, run_top = -INFINITY;
+  int in_run = 0;
+  uint32_t* top = p.top + (int64_t)row * p.entries + sg * (p.seg_blocks / p.run);
+  for (int64_t at = begin; at < end; at += kBsBlock) {  // the SM's other warps cover the wait for a block
+    RawTile<T> q;
+    load_block<T, kVec>(src, at, (int)min((int64_t)kBsBlock, end - at), q);
+    const float rm = raw_max<T>(q);
+    if (rm > -INFINITY) {  // else nothing but -infinity and NaN
+      const float tm = fminf(rm, kFltMax), nm = fmaxf(m, tm);
+      float e = raw_exp_sum<T, false>(q, nm);
+      // the maximum passes over NaN and infinities make NaN: such a block is summed again
+      if (!(e <= kFltMax)) e = raw_exp_sum<T, true>(q, nm);
+      s = s * exp2_fast((m - nm) * kLog2e) + e;  // m = -infinity: s is 0
+      m = nm;
+      run_top = fmaxf(run_top, tm);
     }
-    // The threshold of the running maxima.  All groups have to be in it once; after
-    // that a maximum that is not up to date is only a lower threshold.
-    put_group_max(m > -INFINITY ? order_f32(m + 0.f) : 0u, groups, sh.group);
-    if (at == begin) __syncthreads();
-    const uint32_t cut = min_group_max(groups, sh.group);
-    const float thr = cut ? unorder_f32(cut) : -kFltMax;
-    if (tm >= thr) {
-      const bool full = end - at >= kBsTile;
-#pragma unroll
-      for (int i = 0; i < kBsPer; ++i) {
-        if (v[i] >= thr) {
-          const int e = atomicAdd(&sh.count, 1);
-          if (e < kBsCap)
-            sh.list[e] = make_key(v[i], (uint32_t)(at + tile_pos<T, kVec>(i, full)));
-          else
-            over = true;
-        }
-      }
+    if (++in_run == p.run || at + kBsBlock >= end) {
+      const uint32_t o = __reduce_max_sync(0xffffffffu, order_clean(run_top));
+      if (lane == 0) *top = o;
+      ++top;
+      run_top = -INFINITY;
+      in_run = 0;
     }
   }
-
-  // the piece's maximum and sum; of the list, what the last threshold leaves
   const float wm = warp_max(m);
-  if (lane == 0) sh.wmax[warp] = wm;
-  over = __syncthreads_or(over);
-  float pm = sh.wmax[0];
-#pragma unroll
-  for (int i = 1; i < kBsWarps; ++i) pm = fmaxf(pm, sh.wmax[i]);
-  const float ws = warp_sum(m > -INFINITY ? s * exp2_fast((m - pm) * kLog2e) : 0.f);
-  if (lane == 0) sh.wsum[warp] = ws;
-  if (over) {
-    list_again<T>(sh, p.k, src, begin, end);
-  } else {
-    u64 mine[kBsCap / kBsThreads];
-    const int listed = sh.count;
-    const uint32_t cut = min_group_max(groups, sh.group);
-#pragma unroll
-    for (int i = 0; i < kBsCap / kBsThreads; ++i) {
-      const int e = i * kBsThreads + threadIdx.x;
-      mine[i] = e < listed ? sh.list[e] : 0ull;
-      if ((uint32_t)(mine[i] >> 32) < cut) mine[i] = 0;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kBsCap / kBsThreads; ++i)
-      if (mine[i]) sh.list[atomicAdd(&sh.kept, 1)] = mine[i];
-    __syncthreads();
-  }
-  const int n = sh.kept;
-  if (threadIdx.x == 0) {
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < kBsWarps; ++i) t += sh.wsum[i];
-    p.piece_max[slot] = pm;
-    p.piece_sum[slot] = t;
-    p.piece_count[slot] = min(n, p.k);
-  }
-  for (int i0 = 0; i0 < n; i0 += kBsThreads / 8) {  // uniform: the shuffles need whole warps
-    const int i = i0 + (threadIdx.x >> 3);
-    const u64 key = i < n ? sh.list[i] : 0ull;
-    const int rank = count_above(sh.list, n, key, threadIdx.x & 7);
-    if (i < n && rank < p.k && (threadIdx.x & 7) == 0) p.piece_keys[slot * p.k + rank] = key;
-  }
+  const float ws = warp_sum(m > -INFINITY ? s * exp2_fast((m - wm) * kLog2e) : 0.f);
+  if (lane == 0) p.seg[(int64_t)row * p.segs + sg] = make_float2(wm, ws);
 }
 
 struct MergeParams {
-  const float* scores;
-  const uint8_t* finished;
-  int W, V, k, pieces, pad;
-  const float* piece_max;
-  const float* piece_sum;
-  const int* piece_count;
-  const u64* piece_keys;
+  ScanParams scan;
+  int k, pad;
   float* out_scores;  // [B][k]
   int64_t* out_tokens;
   int64_t* out_parents;
 };
 
-__global__ void __launch_bounds__(kBsThreads) beam_merge_kernel(MergeParams p) {
-  extern __shared__ __align__(16) unsigned char bm_smem[];
-  __shared__ ScanShared sh;
-  __shared__ u64 at_flat[kBsCap];  // the flat indices of sh.list's candidates
-  __shared__ double lse[kBsMaxBeams];
-  const int per = p.pieces * p.k, M = p.W * per + p.W;
-  u64* key = reinterpret_cast<u64*>(bm_smem);            // [M] scores in ordered bits, 0 = none
-  uint32_t* tok = reinterpret_cast<uint32_t*>(key + M);  // [M]
-  const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x == 0) sh.count = 0;
-  pdl_wait();
-  const int64_t lists = (int64_t)b * p.W * p.pieces;
-  // a candidate's key and token, as the scan left them; the first ones are on their way while
-  // the sums are joined
-  auto fetch = [&](int i) -> u64 {
-    if (i >= p.W * per) return 0ull;
-    const int list = i / p.k, e = i - list * p.k;
-    const int have = __ldcg(p.piece_count + lists + list);
-    const u64 x = __ldcg(p.piece_keys + (lists + list) * p.k + e);  // (stale beyond the count)
-    return e < have ? x : 0ull;
-  };
-  u64 first = fetch(threadIdx.x);
-  for (int w = warp; w < p.W; w += kBsWarps) {
-    const int64_t base = lists + (int64_t)w * p.pieces;
-    float m = -INFINITY, q = -INFINITY, u = 0.f;  // the warp's pieces one by one per lane
-    for (int i = lane; i < p.pieces; i += 32) m = fmaxf(m, __ldcg(p.piece_max + base + i));
-    m = warp_max(m);
-    double s = 0.0;
-    for (int i = lane; i < p.pieces; i += 32) {
-      q = __ldcg(p.piece_max + base + i);
-      u = __ldcg(p.piece_sum + base + i);
-      if (q > -INFINITY) s += (double)u * exp((double)q - (double)m);
-    }
+struct MergeShared {
+  u64 key[kBmCap];    // scores in ordered bits, larger is better
+  u64 flat[kBmCap];   // beam * V + token: smaller is better among equal scores
+  double lse[kBsMaxBeams], score[kBsMaxBeams];
+  int alive[kBsMaxBeams];
+  uint32_t group[64];
+  u64 best_key[kBsMaxK], best_flat[kBsMaxK];  // the k best blocks
+  int sum[kBmWarps];
+  int count;
+};
+
+__device__ __forceinline__ int block_sum(int v, MergeShared& sh) {
+  v = __reduce_add_sync(0xffffffffu, v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh.sum[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int s = 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) lse[w] = m > -INFINITY ? (double)m + log(s) : 0.0;
+  for (int w = 0; w < kBmWarps; ++w) s += sh.sum[w];
+  return s;
+}
+
+// The k-th best (key, flat) of what `each` runs over (it calls its argument with
+// every key and flat index), bit by bit: exactly k are at least that good if there are k.
+template <typename Each>
+__device__ __forceinline__ void kth_best(MergeShared& sh, int k, Each each, u64& ck, u64& cf) {
+  ck = 0;
+  cf = ~0ull;
+  bool done = false;
+  for (int bit = 63; bit >= 0 && !done; --bit) {
+    const u64 tr = ck | (1ull << bit);
+    int c = 0;
+    each([&](u64 key, u64) { c += key >= tr; });
+    c = block_sum(c, sh);
+    if (c >= k) ck = tr;
+    done = c == k;
   }
-  __syncthreads();
-  u64 best = 0;
-  for (int i = threadIdx.x; i < M; i += kBsThreads) {
-    const u64 x = i == (int)threadIdx.x ? first : fetch(i);
-    u64 q = 0;
-    uint32_t t = 0;
-    if (x) {
-      const int w = i / per;
-      t = 0xffffffffu - (uint32_t)x;
-      const double sc = (double)p.scores[b * p.W + w] + ((double)unorder_f32((uint32_t)(x >> 32)) - lse[w]);
-      q = sc > -INFINITY ? order_f64(sc) : 0ull;
-    } else if (i >= p.W * per) {
-      const int w = i - p.W * per;  // a finished beam goes on as it is
-      const float sc = p.scores[b * p.W + w];
-      if (p.finished && p.finished[b * p.W + w] && sc > -INFINITY) {
-        q = order_f64((double)sc);
-        t = (uint32_t)p.pad;
-      }
-    }
-    key[i] = q;
-    tok[i] = t;
-    best = q > best ? q : best;
+  if (done) return;
+  u64 low = 0;  // of ~flat
+  for (int bit = 63; bit >= 0 && !done; --bit) {
+    const u64 tr = low | (1ull << bit);
+    int c = 0;
+    each([&](u64 key, u64 flat) { c += key > ck || (key == ck && ~flat >= tr); });
+    c = block_sum(c, sh);
+    if (c >= k) low = tr;
+    done = c == k;
   }
-  auto beam_of = [&](int i) { return i < p.W * per ? i / per : i - p.W * per; };
-  auto flat = [&](int i) { return (u64)beam_of(i) * (u64)p.V + tok[i]; };
-  // a threshold as in the scan, on the upper half of the scores
-  const int groups = group_count(p.k);
-  put_group_max((uint32_t)(best >> 32), groups, sh.group);
-  __syncthreads();
-  const uint32_t cut = min_group_max(groups, sh.group);
-  for (int i = threadIdx.x; i < M; i += kBsThreads) {
-    const u64 q = key[i];
-    if (q != 0 && (uint32_t)(q >> 32) >= cut) {
-      const int e = atomicAdd(&sh.count, 1);
-      if (e < kBsCap) {
-        sh.list[e] = q;
-        at_flat[e] = flat(i);
-      }
-    }
-  }
-  __syncthreads();
-  int n = sh.count;
-  if (n > kBsCap) {
-    // many equal scores: the k-th best (score, flat index) bit by bit
-    u64 ck = 0, cf = 0;  // candidates with (key, ~flat) >= (ck, cf) stay
-    bool done = false;
-    for (int bit = 63; bit >= 0 && !done; --bit) {
-      const u64 tr = ck | (1ull << bit);
-      int c = 0;
-      for (int i = threadIdx.x; i < M; i += kBsThreads) c += key[i] >= tr;
-      c = block_sum(c, sh);
-      if (c >= p.k) ck = tr;
-      done = c == p.k;
-    }
-    for (int bit = 63; bit >= 0 && !done; --bit) {
-      const u64 tr = cf | (1ull << bit);
-      int c = 0;
-      for (int i = threadIdx.x; i < M; i += kBsThreads) c += key[i] > ck || (key[i] == ck && ~flat(i) >= tr);
-      c = block_sum(c, sh);
-      if (c >= p.k) cf = tr;
-      done = c == p.k;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) sh.count = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < M; i += kBsThreads) {
-      if (key[i] != 0 && (key[i] > ck || (key[i] == ck && ~flat(i) >= cf))) {
-        const int e = atomicAdd(&sh.count, 1);
-        if (e < kBsCap) {
-          sh.list[e] = key[i];
-          at_flat[e] = flat(i);
-        }
-      }
-    }
-    __syncthreads();
-    n = min(sh.count, kBsCap);
-  }
-  const int64_t out = (int64_t)b * p.k;
-  for (int i0 = 0; i0 < n; i0 += kBsThreads / 8) {  // eight threads count for one candidate
+  cf = ~low;
+}
+
+// Calls found(rank, key, flat) for the k best of the n in sh.key / sh.flat; eight
+// threads count for one.
+template <typename Found>
+__device__ __forceinline__ void rank_list(const MergeShared& sh, int n, int k, Found found) {
+  for (int i0 = 0; i0 < n; i0 += kBmThreads / 8) {
     const int i = i0 + (threadIdx.x >> 3);
-    const u64 ki = i < n ? sh.list[i] : ~0ull, fi = i < n ? at_flat[i] : 0ull;
+    const u64 ki = i < n ? sh.key[i] : ~0ull, fi = i < n ? sh.flat[i] : 0ull;
     int rank = 0;
 #pragma unroll 4
     for (int j = threadIdx.x & 7; j < n; j += 8) {
-      const u64 kj = sh.list[j], fj = at_flat[j];
+      const u64 kj = sh.key[j], fj = sh.flat[j];
       rank += kj > ki || (kj == ki && fj < fi);
     }
     rank += __shfl_xor_sync(0xffffffffu, rank, 1);
     rank += __shfl_xor_sync(0xffffffffu, rank, 2);
     rank += __shfl_xor_sync(0xffffffffu, rank, 4);
-    if (i < n && rank < p.k && (threadIdx.x & 7) == 0) {
-      const u64 w = fi / (u64)p.V;
-      p.out_scores[out + rank] = (float)unorder_f64(ki);
-      p.out_tokens[out + rank] = (int64_t)(fi - w * (u64)p.V);
-      p.out_parents[out + rank] = (int64_t)w;
-    }
+    if (i < n && rank < k && (threadIdx.x & 7) == 0) found(rank, ki, fi);
   }
-  for (int r = n + threadIdx.x; r < p.k; r += kBsThreads) {  // too few candidates
-    p.out_scores[out + r] = -INFINITY;
-    p.out_tokens[out + r] = -1;
-    p.out_parents[out + r] = 0;
+}
+
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(MergeParams mp) {
+  extern __shared__ __align__(16) unsigned char bm_smem[];
+  const ScanParams& p = mp.scan;
+  MergeShared& sh = *reinterpret_cast<MergeShared*>(bm_smem);
+  u64* entry = reinterpret_cast<u64*>(bm_smem + sizeof(MergeShared));  // [W][entries] largest scores
+  const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = p.W;
+  const int E = W * p.entries;
+  if (threadIdx.x == 0) sh.count = 0;
+  if (threadIdx.x < 64) sh.group[threadIdx.x] = 0;
+  for (int w = threadIdx.x; w < W; w += kBmThreads) {
+    const float sc = p.scores[b * W + w];
+    sh.score[w] = (double)sc;
+    sh.alive[w] = !(sc > -INFINITY) ? 0 : p.finished && p.finished[b * W + w] ? 2 : 1;  // 2: finished
+  }
+  __syncthreads();
+  pdl_wait();
+  // the first noted maximum of each thread is on its way while the sums are joined
+  auto fetch = [&](int i) { return sh.alive[i / p.entries] == 1 ? __ldcg(p.top + (int64_t)b * E + i) : 0u; };
+  const uint32_t first = (int)threadIdx.x < E ? fetch(threadIdx.x) : 0u;
+  for (int w = warp; w < W; w += kBmWarps) {
+    if (sh.alive[w] != 1) continue;
+    const float2* seg = p.seg + (int64_t)(b * W + w) * p.segs;
+    float m = -INFINITY;
+    for (int i = lane; i < p.segs; i += 32) m = fmaxf(m, __ldcg(seg + i).x);
+    m = warp_max(m);
+    double s = 0.0;
+    for (int i = lane; i < p.segs; i += 32) {
+      const float2 q = __ldcg(seg + i);
+      if (q.x > -INFINITY) s += (double)q.y * exp((double)q.x - (double)m);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) sh.lse[w] = m > -INFINITY ? (double)m + log(s) : 0.0;
+  }
+  __syncthreads();
+  auto score_key = [&](int w, float v) { return order_f64(sh.score[w] + ((double)v - sh.lse[w])); };
+
+  // 1. the k best blocks; a finished beam is a block of one candidate
+  const int groups = mp.k <= 16 ? 16 : mp.k <= 32 ? 32 : 64, shift = groups == 16 ? 28 : groups == 32 ? 27 : 26;
+  for (int i = threadIdx.x; i < E + W; i += kBmThreads) {
+    u64 q = 0;
+    if (i < E) {
+      const uint32_t o = i == (int)threadIdx.x ? first : fetch(i);
+      q = o ? score_key(i / p.entries, unorder_f32(o)) : 0ull;
+    } else if (sh.alive[i - E] == 2) {
+      q = order_f64(sh.score[i - E]);
+    }
+    entry[i] = q;
+    // if each of >= k groups of blocks has one above a score, so have >= k blocks: the
+    // smallest of the groups' maxima leaves few to rank.  A hash spreads each beam's blocks.
+    if (q) atomicMax(&sh.group[((uint32_t)i * 2654435769u) >> shift], (uint32_t)(q >> 32));
+  }
+  auto entry_flat = [&](int i) {
+    return i < E ? (u64)(i / p.entries) * (u64)p.V + (u64)(i % p.entries) * (u64)(p.run * kBsBlock)
+                 : (u64)(i - E) * (u64)p.V + (u64)mp.pad;
+  };
+  __syncthreads();
+  uint32_t cut = sh.group[lane & (groups - 1)];
+  if (groups == 64) cut = min(cut, sh.group[lane + 32]);
+  cut = __reduce_min_sync(0xffffffffu, cut);
+  auto append = [&](u64 key, u64 flat) {
+    const int e = atomicAdd(&sh.count, 1);
+    if (e < kBmCap) {
+      sh.key[e] = key;
+      sh.flat[e] = flat;
+    }
+  };
+  for (int i = threadIdx.x; i < E + W; i += kBmThreads) {
+    const u64 q = entry[i];
+    if (q && (uint32_t)(q >> 32) >= cut) append(q, entry_flat(i));
+  }
+  __syncthreads();
+  int n = sh.count;
+  if (n > kBmCap) {  // very many equal maxima
+    u64 ck, cf;
+    kth_best(sh, mp.k, [&](auto use) {
+      for (int i = threadIdx.x; i < E + W; i += kBmThreads)
+        if (entry[i]) use(entry[i], entry_flat(i));
+    }, ck, cf);
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < E + W; i += kBmThreads) {
+      const u64 q = entry[i], f = entry_flat(i);
+      if (q && (q > ck || (q == ck && f <= cf))) append(q, f);
+    }
+    __syncthreads();
+    n = sh.count;
+  }
+  rank_list(sh, n, mp.k, [&](int rank, u64 key, u64 flat) {
+    sh.best_key[rank] = key;
+    sh.best_flat[rank] = flat;
+  });
+  __syncthreads();
+  const int blocks = min(n, mp.k);
+  const u64 least = blocks == mp.k ? sh.best_key[blocks - 1] : 1ull;
+  if (threadIdx.x == 0) sh.count = 0;
+  __syncthreads();
+
+  // 2. their candidates that reach the k-th block's largest score
+  auto each_value = [&](auto use) {
+    for (int i = warp; i < blocks * p.run; i += kBmWarps) {
+      const u64 at_flat = sh.best_flat[i / p.run];
+      const int w = (int)(at_flat / (u64)p.V);
+      if (sh.alive[w] == 2) {
+        if (lane == 0 && i % p.run == 0) use(sh.best_key[i / p.run], at_flat);
+        continue;
+      }
+      const int64_t at = (int64_t)(at_flat - (u64)w * (u64)p.V) + (int64_t)(i % p.run) * kBsBlock;
+      if (at >= p.V) continue;
+      const T* row = reinterpret_cast<const T*>(p.logits) + b * p.batch_stride + w * p.beam_stride;
+      const int left = (int)min((int64_t)kBsBlock, p.V - at);
+      // the lowest logit of this beam that can reach `least`, with room for rounding
+      const double lo = unorder_f64(least) - sh.score[w] + sh.lse[w];
+      const float thr = least > 1ull && isfinite(lo)
+                            ? (float)(lo - 1e-6 * (fabs(lo) + fabs(sh.score[w]) + fabs(sh.lse[w]) + 1.0))
+                            : -kFltMax;
+      RawTile<T> q;
+      load_block<T, kVec>(row, at, left, q);
+#pragma unroll
+      for (int e = 0; e < kBsPer; ++e) {
+        const float v = clean(raw_value<T>(q, e));
+        if (v >= thr) {
+          const u64 key = score_key(w, v);
+          if (key >= least) use(key, (u64)w * (u64)p.V + (u64)at + (u64)block_pos<T, kVec>(e, left >= kBsBlock));
+        }
+      }
+    }
+  };
+  each_value(append);
+  __syncthreads();
+  n = sh.count;
+  if (n > kBmCap) {  // very many equal scores
+    u64 ck, cf;
+    kth_best(sh, mp.k, each_value, ck, cf);
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    each_value([&](u64 key, u64 flat) {
+      if (key > ck || (key == ck && flat <= cf)) append(key, flat);
+    });
+    __syncthreads();
+    n = sh.count;
+  }
+  const int64_t out = (int64_t)b * mp.k;
+  rank_list(sh, n, mp.k, [&](int rank, u64 key, u64 flat) {
+    const u64 w = flat / (u64)p.V;
+    mp.out_scores[out + rank] = (float)unorder_f64(key);
+    mp.out_tokens[out + rank] = (int64_t)(flat - w * (u64)p.V);
+    mp.out_parents[out + rank] = (int64_t)w;
+  });
+  for (int r = n + threadIdx.x; r < mp.k; r += kBmThreads) {  // too few candidates
+    mp.out_scores[out + r] = -INFINITY;
+    mp.out_tokens[out + r] = -1;
+    mp.out_parents[out + r] = 0;
   }
 }
 
 struct BeamPlan {
-  int pieces = 1, piece = kBsTile;
-  size_t max_off = 0, sum_off = 0, count_off = 0, key_off = 0, bytes = 0, merge_smem = 0;
+  int segs = 1, seg_blocks = 1, entries = 1, run = 1;
+  size_t top_off = 0, bytes = 0, merge_smem = 0;
 };
 
-// Pieces per row: the split that takes the fewest rounds of tiles when two CTAs fit
-// an SM; a piece costs about 1.5 tiles beside its tiles (threshold, final ranks).
-BeamPlan beam_plan(int rows, int W, int V, int k, int sm_count) {
+constexpr int kMergeMaxSmem = (int)sizeof(MergeShared) + (kBsMaxBeams * kBsMaxEntries + kBsMaxBeams) * 8;
+
+// Blocks per warp: the split that takes the fewest rounds of blocks when 32 warps fit
+// an SM; a warp costs about half a block beside its blocks.
+BeamPlan beam_plan(int rows, int W, int V, int sm_count) {
   BeamPlan pl;
-  const int tiles = (int)(((int64_t)V + kBsTile - 1) / kBsTile);
-  const int most = std::max(1, std::min({tiles, (kBsMaxMerge - W) / (W * k), 1024, INT_MAX / rows}));
+  const int blocks = (int)(((int64_t)V + kBsBlock - 1) / kBsBlock);
+  pl.run = (blocks + kBsMaxEntries - 1) / kBsMaxEntries;
+  pl.entries = (blocks + pl.run - 1) / pl.run;
   double best = 1e30;
-  for (int s = 1; s <= most; ++s) {
-    const int t = (tiles + s - 1) / s;
-    if ((t - 1) * s >= tiles && s > 1) continue;
-    const int64_t rounds = ((int64_t)rows * s + 2 * sm_count - 1) / (2 * sm_count);
-    const double cost = (double)rounds * (t + 1.5);
+  for (int e = 1; e <= pl.entries; ++e) {  // entries per warp
+    const int segs = (pl.entries + e - 1) / e;
+    const int64_t rounds = ((int64_t)rows * segs + 32 * sm_count - 1) / (32 * sm_count);
+    const double cost = (double)rounds * (e * pl.run + 0.5);
     if (cost < best) {
       best = cost;
-      pl.piece = t * kBsTile;
-      pl.pieces = (tiles + t - 1) / t;
+      pl.seg_blocks = e * pl.run;
+      pl.segs = segs;
     }
   }
-  const size_t n = (size_t)rows * pl.pieces;
-  pl.max_off = 0;
-  pl.sum_off = align_up(n * 4, 256);
-  pl.count_off = pl.sum_off + align_up(n * 4, 256);
-  pl.key_off = pl.count_off + align_up(n * 4, 256);
-  pl.bytes = pl.key_off + n * k * 8;
-  pl.merge_smem = ((size_t)W * pl.pieces * k + W) * 12;
+  pl.top_off = align_up((size_t)rows * pl.segs * sizeof(float2), 256);
+  pl.bytes = pl.top_off + (size_t)rows * pl.entries * 4;
+  pl.merge_smem = sizeof(MergeShared) + ((size_t)W * pl.entries + W) * 8;
   return pl;
 }
 
@@ -574,6 +537,13 @@ bool beam_size_ok(int batch, int beams, int vocab, int k) {
 }
 
 using ScanFn = void (*)(ScanParams);
+using MergeFn = void (*)(MergeParams);
+
+template <typename T>
+void beam_pick(bool vec, ScanFn* scan, MergeFn* merge) {
+  *scan = vec ? beam_scan_kernel<T, true> : beam_scan_kernel<T, false>;
+  *merge = vec ? beam_merge_kernel<T, true> : beam_merge_kernel<T, false>;
+}
 
 // ---- reordering -------------------------------------------------------------------
 constexpr int kBrThreads = 256;
@@ -678,7 +648,7 @@ size_t nsm_beam_select_workspace_bytes(int32_t batch, int32_t beams, int32_t voc
   if (!beam_size_ok(batch, beams, vocab, candidates)) return 0;
   DeviceInfo di;
   if (current_device(&di) != NSM_OK) return 0;
-  return beam_plan(batch * beams, beams, vocab, candidates, di.sm_count).bytes;
+  return beam_plan(batch * beams, beams, vocab, di.sm_count).bytes;
 }
 
 int nsm_beam_select(const void* logits, int32_t logits_dtype, int64_t batch_stride, int64_t beam_stride,
@@ -701,51 +671,48 @@ int nsm_beam_select(const void* logits, int32_t logits_dtype, int64_t batch_stri
   const int rc = current_device(&di);
   if (rc != NSM_OK) return rc;
   const int rows = batch * beams;
-  const BeamPlan pl = beam_plan(rows, beams, vocab, candidates, di.sm_count);
+  const BeamPlan pl = beam_plan(rows, beams, vocab, di.sm_count);
   NSM_REQUIRE(((uintptr_t)workspace & 255) == 0 && workspace_bytes >= pl.bytes, NSM_ERR_WORKSPACE,
               "nsm_beam_select: workspace misaligned or too small (nsm_beam_select_workspace_bytes)");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   auto* ws = static_cast<unsigned char*>(workspace);
-  ScanParams sp;
+  MergeParams mp;
+  ScanParams& sp = mp.scan;
   sp.logits = logits;
   sp.batch_stride = batch_stride;
   sp.beam_stride = beam_stride;
   sp.scores = scores;
   sp.finished = finished;
+  sp.rows = rows;
   sp.W = beams;
   sp.V = vocab;
-  sp.k = candidates;
-  sp.pieces = pl.pieces;
-  sp.piece = pl.piece;
-  sp.piece_max = reinterpret_cast<float*>(ws + pl.max_off);
-  sp.piece_sum = reinterpret_cast<float*>(ws + pl.sum_off);
-  sp.piece_count = reinterpret_cast<int*>(ws + pl.count_off);
-  sp.piece_keys = reinterpret_cast<u64*>(ws + pl.key_off);
-  // 16-byte loads when every row starts on 16 bytes, else one value per lane
-  const bool vec = (((uintptr_t)logits | (uintptr_t)(batch_stride * es) | (uintptr_t)(beam_stride * es)) & 15) == 0;
-  const ScanFn fn = logits_dtype == NSM_F32   ? (vec ? beam_scan_kernel<float, true> : beam_scan_kernel<float, false>)
-                    : logits_dtype == NSM_F16 ? (vec ? beam_scan_kernel<__half, true> : beam_scan_kernel<__half, false>)
-                                              : (vec ? beam_scan_kernel<__nv_bfloat16, true>
-                                                     : beam_scan_kernel<__nv_bfloat16, false>);
-  fn<<<(unsigned)(rows * pl.pieces), kBsThreads, 0, s>>>(sp);
-  NSM_CHECK_CUDA(cudaGetLastError());
-  MergeParams mp;
-  mp.scores = scores;
-  mp.finished = finished;
-  mp.W = beams;
-  mp.V = vocab;
+  sp.segs = pl.segs;
+  sp.seg_blocks = pl.seg_blocks;
+  sp.entries = pl.entries;
+  sp.run = pl.run;
+  sp.seg = reinterpret_cast<float2*>(ws);
+  sp.top = reinterpret_cast<uint32_t*>(ws + pl.top_off);
   mp.k = candidates;
-  mp.pieces = pl.pieces;
   mp.pad = pad_token;
-  mp.piece_max = sp.piece_max;
-  mp.piece_sum = sp.piece_sum;
-  mp.piece_count = sp.piece_count;
-  mp.piece_keys = sp.piece_keys;
   mp.out_scores = out_scores;
   mp.out_tokens = out_tokens;
   mp.out_parents = out_parents;
-  NSM_CHECK_CUDA(cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBsMaxMerge * 12));
-  NSM_CHECK_CUDA(launch_pdl(beam_merge_kernel, dim3(batch), dim3(kBsThreads), pl.merge_smem, s, mp));
+  // 16-byte loads when every row starts on 16 bytes, else one value per lane
+  const bool vec = (((uintptr_t)logits | (uintptr_t)(batch_stride * es) | (uintptr_t)(beam_stride * es)) & 15) == 0;
+  ScanFn scan;
+  MergeFn merge;
+  if (logits_dtype == NSM_F32)
+    beam_pick<float>(vec, &scan, &merge);
+  else if (logits_dtype == NSM_F16)
+    beam_pick<__half>(vec, &scan, &merge);
+  else
+    beam_pick<__nv_bfloat16>(vec, &scan, &merge);
+  const int64_t warps = (int64_t)rows * pl.segs;
+  scan<<<(unsigned)((warps + kBsWarps - 1) / kBsWarps), kBsThreads, 0, s>>>(sp);
+  NSM_CHECK_CUDA(cudaGetLastError());
+  static SmemOnce once[6];
+  NSM_CHECK_CUDA(once[logits_dtype * 2 + vec].set(merge, kMergeMaxSmem, di.device));
+  NSM_CHECK_CUDA(launch_pdl(merge, dim3(batch), dim3(kBmThreads), pl.merge_smem, s, mp));
   return NSM_OK;
 }
 

@@ -7,6 +7,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 #include <utility>
 
@@ -116,6 +117,20 @@ struct LaunchShape {
   int warps_per_cta = 8;
 };
 int launch_shape(LaunchShape* s);
+
+// Raises a kernel's dynamic shared memory limit the first time it is used on a
+// device; one object per kernel, always with the same size, so host threads may call at once.
+struct SmemOnce {
+  std::atomic<unsigned long long> done{0};  // a bit per device
+  template <typename Kernel>
+  cudaError_t set(Kernel kern, int bytes, int device) {
+    const unsigned long long bit = 1ull << (device & 63);
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+  }
+};
 
 // Launch with programmatic stream serialization (PDL): the kernel may begin
 // before its predecessor finishes and must call griddepcontrol.wait before it

@@ -566,7 +566,9 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
               : mode == kInt       ? lin4_pick_npg<kInt>(sh.npg, pl.cols)
                                    : lin4_pick_npg<kIntZeros>(sh.npg, pl.cols);
   const size_t smem = w->code ? (size_t)kLutBytes : 0;
-  if (smem > 0) NSM_CHECK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static SmemOnce once[2][3][3];
+  if (smem > 0)
+    NSM_CHECK_CUDA(once[mode][sh.npg / 2][pl.cols <= 8 ? 0 : pl.cols <= 16 ? 1 : 2].set(fn, (int)smem, di.device));
   lin4_prep_kernel<<<rows, 1024, 0, s>>>(x, x_dtype, x_row_stride, sh.K, sh.kp, rows, x_dtype == NSM_F32, w->code, xh,
                                          scale);
   NSM_CHECK_CUDA(cudaGetLastError());
