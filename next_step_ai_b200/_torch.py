@@ -40,7 +40,13 @@ def row_ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr()
 
 
+# the current stream's handle without a Stream object around it, where torch has it
+_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_handle(device: torch.device | None = None) -> int:
+    if _RAW_STREAM is not None and device is not None and device.index is not None:
+        return _RAW_STREAM(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

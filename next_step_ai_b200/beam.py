@@ -64,18 +64,29 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, num_candidates: i
     return _select(logits, code, scores, fin, B, W, V, k, pad_token, dev)
 
 
+_WS_BYTES: dict[tuple[int, int, int, int, int], int] = {}  # by device and sizes
+
+
 def _select(logits, code, scores, fin, B, W, V, k, pad_token, dev):
     lib = _lib.load()
-    out_s = torch.empty((B, k), dtype=torch.float32, device=dev)
-    out_i = torch.empty((2, B, k), dtype=torch.int64, device=dev)
+    out_s = torch.empty(B, k, dtype=torch.float32, device=dev)
+    out_t = torch.empty(B, k, dtype=torch.int64, device=dev)
+    out_p = torch.empty_like(out_t)
     if B:
-        need = int(lib.nsm_beam_select_workspace_bytes(B, W, V, k))
+        key = (dev.index, B, W, V, k)
+        need = _WS_BYTES.get(key)
+        if need is None:
+            if len(_WS_BYTES) > 4096:
+                _WS_BYTES.clear()
+            need = _WS_BYTES[key] = int(lib.nsm_beam_select_workspace_bytes(B, W, V, k))
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        at = out_i.data_ptr()
-        _lib.check(lib.nsm_beam_select(logits.data_ptr(), code, logits.stride(0), logits.stride(1), scores.data_ptr(),
-                                       fin, B, W, V, k, pad_token, out_s.data_ptr(), at, at + 8 * B * k, ws.data_ptr(),
-                                       need, stream_handle(dev)), "nsm_beam_select")
-    return out_s, out_i[0], out_i[1]
+        stride = logits.stride()
+        status = lib.nsm_beam_select(logits.data_ptr(), code, stride[0], stride[1], scores.data_ptr(), fin, B, W, V, k,
+                                     pad_token, out_s.data_ptr(), out_t.data_ptr(), out_p.data_ptr(), ws.data_ptr(),
+                                     need, stream_handle(dev))
+        if status:
+            _lib.check(status, "nsm_beam_select")
+    return out_s, out_t, out_p
 
 
 def _describe(t: torch.Tensor, rows: int, length_dim: int | None) -> _lib.BeamStateC:

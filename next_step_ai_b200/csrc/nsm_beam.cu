@@ -39,7 +39,8 @@ constexpr int kBsWarps = kBsThreads / 32;
 constexpr int kBsPer = 32;                       // values per lane
 constexpr int kBsBlock = 32 * kBsPer;            // values of a block: one warp's registers
 constexpr int kBsMaxEntries = 384;               // noted maxima of a row
-constexpr int kBmThreads = 512;                  // of the merge
+constexpr int kBmThreads = 1024;                 // of the merge: a warp per beam, 8 threads per ranked candidate
+constexpr int kBmGroups = 128;                   // groups of blocks for the first threshold
 constexpr int kBmWarps = kBmThreads / 32;
 constexpr int kBmCap = 2048;                     // candidates ranked by counting
 constexpr int kBsMaxK = 64;
@@ -273,15 +274,18 @@ struct MergeParams {
   int64_t* out_parents;
 };
 
+// A candidate is (beam << 32 | token), a block (its index among [W][entries + 1]): smaller
+// comes first among equal scores.  A finished beam has one block, of one candidate.
 struct MergeShared {
-  u64 key[kBmCap];    // scores in ordered bits, larger is better
-  u64 flat[kBmCap];   // beam * V + token: smaller is better among equal scores
+  u64 key[kBmCap];  // scores in ordered bits, larger is better
+  u64 id[kBmCap];
   double lse[kBsMaxBeams], score[kBsMaxBeams];
-  int alive[kBsMaxBeams];
-  uint32_t group[64];
-  u64 best_key[kBsMaxK], best_flat[kBsMaxK];  // the k best blocks
+  int alive[kBsMaxBeams];  // 0: out, 1: read, 2: finished
+  uint32_t group[kBmGroups], cut;
+  u64 best_key[kBsMaxK];   // the k best blocks
+  int best_id[kBsMaxK];
   int sum[kBmWarps];
-  int count;
+  int entries_listed, values_listed;
 };
 
 __device__ __forceinline__ int block_sum(int v, MergeShared& sh) {
@@ -295,8 +299,8 @@ __device__ __forceinline__ int block_sum(int v, MergeShared& sh) {
   return s;
 }
 
-// The k-th best (key, flat) of what `each` runs over (it calls its argument with
-// every key and flat index), bit by bit: exactly k are at least that good if there are k.
+// The k-th best (key, id) of what `each` runs over (it calls its argument with
+// every key and id), bit by bit: exactly k are at least that good if there are k.
 template <typename Each>
 __device__ __forceinline__ void kth_best(MergeShared& sh, int k, Each each, u64& ck, u64& cf) {
   ck = 0;
@@ -311,11 +315,11 @@ __device__ __forceinline__ void kth_best(MergeShared& sh, int k, Each each, u64&
     done = c == k;
   }
   if (done) return;
-  u64 low = 0;  // of ~flat
+  u64 low = 0;  // of ~id
   for (int bit = 63; bit >= 0 && !done; --bit) {
     const u64 tr = low | (1ull << bit);
     int c = 0;
-    each([&](u64 key, u64 flat) { c += key > ck || (key == ck && ~flat >= tr); });
+    each([&](u64 key, u64 id) { c += key > ck || (key == ck && ~id >= tr); });
     c = block_sum(c, sh);
     if (c >= k) low = tr;
     done = c == k;
@@ -323,175 +327,273 @@ __device__ __forceinline__ void kth_best(MergeShared& sh, int k, Each each, u64&
   cf = ~low;
 }
 
-// Calls found(rank, key, flat) for the k best of the n in sh.key / sh.flat; eight
+// Calls found(rank, key, id) for the k best of the n in sh.key / sh.id; eight
 // threads count for one.
 template <typename Found>
 __device__ __forceinline__ void rank_list(const MergeShared& sh, int n, int k, Found found) {
   for (int i0 = 0; i0 < n; i0 += kBmThreads / 8) {
     const int i = i0 + (threadIdx.x >> 3);
-    const u64 ki = i < n ? sh.key[i] : ~0ull, fi = i < n ? sh.flat[i] : 0ull;
+    const u64 ki = i < n ? sh.key[i] : ~0ull, di = i < n ? sh.id[i] : 0ull;
     int rank = 0;
 #pragma unroll 4
     for (int j = threadIdx.x & 7; j < n; j += 8) {
-      const u64 kj = sh.key[j], fj = sh.flat[j];
-      rank += kj > ki || (kj == ki && fj < fi);
+      const u64 kj = sh.key[j], dj = sh.id[j];
+      rank += kj > ki || (kj == ki && dj < di);
     }
     rank += __shfl_xor_sync(0xffffffffu, rank, 1);
     rank += __shfl_xor_sync(0xffffffffu, rank, 2);
     rank += __shfl_xor_sync(0xffffffffu, rank, 4);
-    if (i < n && rank < k && (threadIdx.x & 7) == 0) found(rank, ki, fi);
+    if (i < n && rank < k && (threadIdx.x & 7) == 0) found(rank, ki, di);
   }
 }
 
+// Group maxima: a hash spreads what is put in over the groups.  The k-th largest of the
+// maxima is a threshold that k of them reach, and hardly more than k / (1 - k / 256) of all
+// (0 when fewer than k groups have any).
+__device__ __forceinline__ void put_group(MergeShared& sh, int i, u64 key) {
+  static_assert(kBmGroups == 128, "the upper 7 bits of the hash");
+  if (key) atomicMax(&sh.group[((uint32_t)i * 2654435769u) >> 25], (uint32_t)(key >> 32));
+}
+__device__ __forceinline__ uint32_t group_threshold(MergeShared& sh, int k) {
+  static_assert(kBmGroups * 8 == kBmThreads && kBmGroups >= kBsMaxK, "eight threads per group");
+  const int g = threadIdx.x >> 3;
+  const uint32_t mine = sh.group[g];
+  int rank = 0;
+#pragma unroll 4
+  for (int o = threadIdx.x & 7; o < kBmGroups; o += 8) {
+    const uint32_t other = sh.group[o];
+    rank += other > mine || (other == mine && o < g);
+  }
+  rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+  rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+  rank += __shfl_xor_sync(0xffffffffu, rank, 4);
+  if (rank == k - 1 && (threadIdx.x & 7) == 0) sh.cut = mine;
+  __syncthreads();
+  return sh.cut;
+}
+
+// What the steps of the merge share.
+struct MergeView {
+  const MergeParams& mp;
+  MergeShared& sh;
+  u64* entry;  // [W][entries + 1] the blocks' largest scores, 0 = none
+  int b;
+
+  __device__ __forceinline__ u64 score_key(int w, float v) const {
+    return order_f64(sh.score[w] + ((double)v - sh.lse[w]));
+  }
+  __device__ __forceinline__ void append(int* count, u64 key, u64 id) const {
+    const int e = atomicAdd(count, 1);
+    if (e < kBmCap) {
+      sh.key[e] = key;
+      sh.id[e] = id;
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ const T* row(int w) const {
+    return reinterpret_cast<const T*>(mp.scan.logits) + b * mp.scan.batch_stride + w * mp.scan.beam_stride;
+  }
+};
+
+// The k best blocks when very many have equal maxima.
+__device__ __noinline__ void entries_again(const MergeView& v) {
+  const int n = v.mp.scan.W * (v.mp.scan.entries + 1);
+  u64 ck, cf;
+  kth_best(v.sh, v.mp.k, [&](auto use) {
+    for (int i = threadIdx.x; i < n; i += kBmThreads)
+      if (v.entry[i]) use(v.entry[i], (u64)i);
+  }, ck, cf);
+  if (threadIdx.x == 0) v.sh.entries_listed = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kBmThreads) {
+    const u64 q = v.entry[i];
+    if (q && (q > ck || (q == ck && (u64)i <= cf))) v.append(&v.sh.entries_listed, q, i);
+  }
+  __syncthreads();
+}
+
+// The k best of the blocks' values when very many scores are equal.
+template <typename T>
+__device__ __noinline__ void values_again(const MergeView& v, int blocks, u64 least) {
+  const ScanParams& p = v.mp.scan;
+  auto each = [&](auto use) {
+    const int64_t per = (int64_t)p.run * kBsBlock;
+    for (int64_t i = threadIdx.x; i < blocks * per; i += kBmThreads) {
+      const int j = (int)(i / per), id = v.sh.best_id[j], w = id / (p.entries + 1);
+      if (v.sh.alive[w] == 2) {
+        if (i == j * per) use(v.sh.best_key[j], (u64)w << 32 | (u64)v.mp.pad);
+        continue;
+      }
+      const int64_t pos = (id - w * (p.entries + 1)) * per + (i - j * per);
+      if (pos >= p.V) continue;
+      const float x = clean(to_f32<T>(v.row<T>(w)[pos]));
+      if (x == -INFINITY) continue;
+      const u64 key = v.score_key(w, x);
+      if (key >= least) use(key, (u64)w << 32 | (u64)pos);
+    }
+  };
+  u64 ck, cf;
+  kth_best(v.sh, v.mp.k, each, ck, cf);
+  if (threadIdx.x == 0) v.sh.values_listed = 0;
+  __syncthreads();
+  each([&](u64 key, u64 id) {
+    if (key > ck || (key == ck && id <= cf)) v.append(&v.sh.values_listed, key, id);
+  });
+  __syncthreads();
+}
+
 template <typename T, bool kVec>
-__global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(MergeParams mp) {
+__global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(const __grid_constant__ MergeParams mp) {
   extern __shared__ __align__(16) unsigned char bm_smem[];
   const ScanParams& p = mp.scan;
   MergeShared& sh = *reinterpret_cast<MergeShared*>(bm_smem);
-  u64* entry = reinterpret_cast<u64*>(bm_smem + sizeof(MergeShared));  // [W][entries] largest scores
+  const MergeView view{mp, sh, reinterpret_cast<u64*>(bm_smem + sizeof(MergeShared)), (int)blockIdx.x};
   const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = p.W;
-  const int E = W * p.entries;
-  if (threadIdx.x == 0) sh.count = 0;
-  if (threadIdx.x < 64) sh.group[threadIdx.x] = 0;
-  for (int w = threadIdx.x; w < W; w += kBmThreads) {
-    const float sc = p.scores[b * W + w];
-    sh.score[w] = (double)sc;
-    sh.alive[w] = !(sc > -INFINITY) ? 0 : p.finished && p.finished[b * W + w] ? 2 : 1;  // 2: finished
-  }
+  const int per_beam = p.entries + 1;
+  if (threadIdx.x == 0) sh.entries_listed = sh.values_listed = 0;
+  if (threadIdx.x < kBmGroups) sh.group[threadIdx.x] = 0;
   __syncthreads();
-  pdl_wait();
-  // the first noted maximum of each thread is on its way while the sums are joined
-  auto fetch = [&](int i) { return sh.alive[i / p.entries] == 1 ? __ldcg(p.top + (int64_t)b * E + i) : 0u; };
-  const uint32_t first = (int)threadIdx.x < E ? fetch(threadIdx.x) : 0u;
+
+  // 1. a warp per beam: the sums joined, the scores of its blocks' maxima
+  bool waited = false;
   for (int w = warp; w < W; w += kBmWarps) {
-    if (sh.alive[w] != 1) continue;
-    const float2* seg = p.seg + (int64_t)(b * W + w) * p.segs;
-    float m = -INFINITY;
-    for (int i = lane; i < p.segs; i += 32) m = fmaxf(m, __ldcg(seg + i).x);
-    m = warp_max(m);
-    double s = 0.0;
-    for (int i = lane; i < p.segs; i += 32) {
-      const float2 q = __ldcg(seg + i);
-      if (q.x > -INFINITY) s += (double)q.y * exp((double)q.x - (double)m);
-    }
+    const float sc = p.scores[b * W + w];
+    const int alive = !(sc > -INFINITY) ? 0 : p.finished && p.finished[b * W + w] ? 2 : 1;
+    if (!waited) pdl_wait();
+    waited = true;
+    u64* entry = view.entry + w * per_beam;
+    double lse = 0.0;
+    if (alive == 1) {
+      const float2* seg = p.seg + (int64_t)(b * W + w) * p.segs;
+      const uint32_t* top = p.top + (int64_t)(b * W + w) * p.entries;
+      const float2 none = make_float2(-INFINITY, 0.f);
+      const float2 q0 = lane < p.segs ? __ldcg(seg + lane) : none;
+      uint32_t o[4];  // on their way while the sums are joined
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) sh.lse[w] = m > -INFINITY ? (double)m + log(s) : 0.0;
-  }
-  __syncthreads();
-  auto score_key = [&](int w, float v) { return order_f64(sh.score[w] + ((double)v - sh.lse[w])); };
-
-  // 1. the k best blocks; a finished beam is a block of one candidate
-  const int groups = mp.k <= 16 ? 16 : mp.k <= 32 ? 32 : 64, shift = groups == 16 ? 28 : groups == 32 ? 27 : 26;
-  for (int i = threadIdx.x; i < E + W; i += kBmThreads) {
-    u64 q = 0;
-    if (i < E) {
-      const uint32_t o = i == (int)threadIdx.x ? first : fetch(i);
-      q = o ? score_key(i / p.entries, unorder_f32(o)) : 0ull;
-    } else if (sh.alive[i - E] == 2) {
-      q = order_f64(sh.score[i - E]);
-    }
-    entry[i] = q;
-    // if each of >= k groups of blocks has one above a score, so have >= k blocks: the
-    // smallest of the groups' maxima leaves few to rank.  A hash spreads each beam's blocks.
-    if (q) atomicMax(&sh.group[((uint32_t)i * 2654435769u) >> shift], (uint32_t)(q >> 32));
-  }
-  auto entry_flat = [&](int i) {
-    return i < E ? (u64)(i / p.entries) * (u64)p.V + (u64)(i % p.entries) * (u64)(p.run * kBsBlock)
-                 : (u64)(i - E) * (u64)p.V + (u64)mp.pad;
-  };
-  __syncthreads();
-  uint32_t cut = sh.group[lane & (groups - 1)];
-  if (groups == 64) cut = min(cut, sh.group[lane + 32]);
-  cut = __reduce_min_sync(0xffffffffu, cut);
-  auto append = [&](u64 key, u64 flat) {
-    const int e = atomicAdd(&sh.count, 1);
-    if (e < kBmCap) {
-      sh.key[e] = key;
-      sh.flat[e] = flat;
-    }
-  };
-  for (int i = threadIdx.x; i < E + W; i += kBmThreads) {
-    const u64 q = entry[i];
-    if (q && (uint32_t)(q >> 32) >= cut) append(q, entry_flat(i));
-  }
-  __syncthreads();
-  int n = sh.count;
-  if (n > kBmCap) {  // very many equal maxima
-    u64 ck, cf;
-    kth_best(sh, mp.k, [&](auto use) {
-      for (int i = threadIdx.x; i < E + W; i += kBmThreads)
-        if (entry[i]) use(entry[i], entry_flat(i));
-    }, ck, cf);
-    if (threadIdx.x == 0) sh.count = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < E + W; i += kBmThreads) {
-      const u64 q = entry[i], f = entry_flat(i);
-      if (q && (q > ck || (q == ck && f <= cf))) append(q, f);
-    }
-    __syncthreads();
-    n = sh.count;
-  }
-  rank_list(sh, n, mp.k, [&](int rank, u64 key, u64 flat) {
-    sh.best_key[rank] = key;
-    sh.best_flat[rank] = flat;
-  });
-  __syncthreads();
-  const int blocks = min(n, mp.k);
-  const u64 least = blocks == mp.k ? sh.best_key[blocks - 1] : 1ull;
-  if (threadIdx.x == 0) sh.count = 0;
-  __syncthreads();
-
-  // 2. their candidates that reach the k-th block's largest score
-  auto each_value = [&](auto use) {
-    for (int i = warp; i < blocks * p.run; i += kBmWarps) {
-      const u64 at_flat = sh.best_flat[i / p.run];
-      const int w = (int)(at_flat / (u64)p.V);
-      if (sh.alive[w] == 2) {
-        if (lane == 0 && i % p.run == 0) use(sh.best_key[i / p.run], at_flat);
-        continue;
+      for (int i = 0; i < 4; ++i) o[i] = lane + 32 * i < p.entries ? __ldcg(top + lane + 32 * i) : 0u;
+      float m = q0.x;
+      for (int i = lane + 32; i < p.segs; i += 32) m = fmaxf(m, __ldcg(seg + i).x);
+      m = warp_max(m);
+      if (m > -INFINITY) {
+        float s = q0.y * exp2_fast((q0.x - m) * kLog2e);
+        for (int i = lane + 32; i < p.segs; i += 32) {
+          const float2 q = __ldcg(seg + i);
+          s += q.y * exp2_fast((q.x - m) * kLog2e);
+        }
+        s = warp_sum(s);
+        lse = (double)m + log((double)s);
       }
-      const int64_t at = (int64_t)(at_flat - (u64)w * (u64)p.V) + (int64_t)(i % p.run) * kBsBlock;
-      if (at >= p.V) continue;
-      const T* row = reinterpret_cast<const T*>(p.logits) + b * p.batch_stride + w * p.beam_stride;
-      const int left = (int)min((int64_t)kBsBlock, p.V - at);
-      // the lowest logit of this beam that can reach `least`, with room for rounding
-      const double lo = unorder_f64(least) - sh.score[w] + sh.lse[w];
-      const float thr = least > 1ull && isfinite(lo)
-                            ? (float)(lo - 1e-6 * (fabs(lo) + fabs(sh.score[w]) + fabs(sh.lse[w]) + 1.0))
-                            : -kFltMax;
-      RawTile<T> q;
-      load_block<T, kVec>(row, at, left, q);
+      for (int e0 = 0; e0 < p.entries; e0 += 128) {
 #pragma unroll
-      for (int e = 0; e < kBsPer; ++e) {
-        const float v = clean(raw_value<T>(q, e));
-        if (v >= thr) {
-          const u64 key = score_key(w, v);
-          if (key >= least) use(key, (u64)w * (u64)p.V + (u64)at + (u64)block_pos<T, kVec>(e, left >= kBsBlock));
+        for (int i = 0; i < 4; ++i) {
+          const int e = e0 + lane + 32 * i;
+          if (e < p.entries) {
+            const u64 q = o[i] ? order_f64((double)sc + ((double)unorder_f32(o[i]) - lse)) : 0ull;
+            entry[e] = q;
+            put_group(sh, w * per_beam + e, q);
+          }
+          if (e + 128 < p.entries) o[i] = __ldcg(top + e + 128);
         }
       }
+    } else {
+      for (int e = lane; e < p.entries; e += 32) entry[e] = 0;
     }
-  };
-  each_value(append);
-  __syncthreads();
-  n = sh.count;
-  if (n > kBmCap) {  // very many equal scores
-    u64 ck, cf;
-    kth_best(sh, mp.k, each_value, ck, cf);
-    if (threadIdx.x == 0) sh.count = 0;
-    __syncthreads();
-    each_value([&](u64 key, u64 flat) {
-      if (key > ck || (key == ck && flat <= cf)) append(key, flat);
-    });
-    __syncthreads();
-    n = sh.count;
+    if (lane == 0) {
+      sh.score[w] = (double)sc;
+      sh.alive[w] = alive;
+      sh.lse[w] = lse;
+      const u64 q = alive == 2 ? order_f64((double)sc) : 0ull;
+      entry[p.entries] = q;
+      put_group(sh, w * per_beam + p.entries, q);
+    }
   }
+  if (!waited) pdl_wait();
+  __syncthreads();
+
+  // 2. the k best blocks
+  const uint32_t cut = group_threshold(sh, mp.k);
+  for (int i = threadIdx.x; i < W * per_beam; i += kBmThreads) {
+    const u64 q = view.entry[i];
+    if (q && (uint32_t)(q >> 32) >= cut) view.append(&sh.entries_listed, q, i);
+  }
+  __syncthreads();
+  if (sh.entries_listed > kBmCap) entries_again(view);
+  const int listed = sh.entries_listed, blocks = min(listed, mp.k);
+  rank_list(sh, listed, mp.k, [&](int rank, u64 key, u64 id) {
+    sh.best_key[rank] = key;
+    sh.best_id[rank] = (int)id;
+  });
+  __syncthreads();
+
+  // 3. their values that reach the k-th block's largest score
+  u64 least = blocks == mp.k ? sh.best_key[blocks - 1] : 1ull;
+  auto load_chosen = [&](int i, RawTile<T>& q, int& w, int64_t& at) {  // false: no values there
+    const int j = p.run == 1 ? i : i / p.run;
+    const int id = sh.best_id[j];
+    w = id / per_beam;
+    at = ((int64_t)(id - w * per_beam) * p.run + (i - j * p.run)) * kBsBlock;
+    if (sh.alive[w] == 2 || at >= p.V) return false;
+    load_block<T, kVec>(view.row<T>(w), at, (int)min((int64_t)kBsBlock, p.V - at), q);
+    return true;
+  };
+  if (blocks < mp.k) {
+    // fewer blocks than candidates (a small vocabulary, a heavy mask): a threshold from the
+    // lanes' maxima
+    if (threadIdx.x < kBmGroups) sh.group[threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = warp; i < blocks * p.run; i += kBmWarps) {
+      RawTile<T> q;
+      int w;
+      int64_t at;
+      if (!load_chosen(i, q, w, at)) {
+        if (sh.alive[w] == 2 && lane == 0 && i % p.run == 0) put_group(sh, i * 32, sh.best_key[i / p.run]);
+        continue;
+      }
+      const uint32_t o = order_clean(raw_max<T>(q));
+      put_group(sh, i * 32 + lane, o ? view.score_key(w, unorder_f32(o)) : 0ull);
+    }
+    __syncthreads();
+    least = max(1ull, (u64)group_threshold(sh, mp.k) << 32);
+  }
+  for (int i = warp; i < blocks * p.run; i += kBmWarps) {
+    RawTile<T> q;
+    int w;
+    int64_t at;
+    if (!load_chosen(i, q, w, at)) {
+      if (sh.alive[w] == 2 && lane == 0 && i % p.run == 0)
+        view.append(&sh.values_listed, sh.best_key[i / p.run], (u64)w << 32 | (u64)mp.pad);
+      continue;
+    }
+    const int left = (int)min((int64_t)kBsBlock, p.V - at);
+    // the lowest logit of this beam that can reach `least`, with room for rounding
+    const double lo = unorder_f64(least) - sh.score[w] + sh.lse[w];
+    const float thr = least > 1ull && isfinite(lo)
+                          ? (float)(lo - 1e-6 * (fabs(lo) + fabs(sh.score[w]) + fabs(sh.lse[w]) + 1.0))
+                          : -kFltMax;
+    uint32_t hits = 0;
+#pragma unroll
+    for (int e = 0; e < kBsPer; ++e)
+      if (clean(raw_value<T>(q, e)) >= thr) hits |= 1u << e;
+    while (hits) {  // few
+      const int at_e = __ffs(hits) - 1;
+      hits &= hits - 1;
+      uint32_t word = q.r[0];
+#pragma unroll
+      for (int e = 1; e < kBsPer * (int)sizeof(T) / 4; ++e)
+        if (e == at_e * (int)sizeof(T) / 4) word = q.r[e];
+      const u64 key = view.score_key(w, clean(raw_value<T>(word, at_e)));
+      if (key >= least)
+        view.append(&sh.values_listed, key, (u64)w << 32 | (u64)(at + block_pos<T, kVec>(at_e, left >= kBsBlock)));
+    }
+  }
+  __syncthreads();
+  if (sh.values_listed > kBmCap) values_again<T>(view, blocks, least);
+  const int n = sh.values_listed;
   const int64_t out = (int64_t)b * mp.k;
-  rank_list(sh, n, mp.k, [&](int rank, u64 key, u64 flat) {
-    const u64 w = flat / (u64)p.V;
+  rank_list(sh, n, mp.k, [&](int rank, u64 key, u64 id) {
     mp.out_scores[out + rank] = (float)unorder_f64(key);
-    mp.out_tokens[out + rank] = (int64_t)(flat - w * (u64)p.V);
-    mp.out_parents[out + rank] = (int64_t)w;
+    mp.out_tokens[out + rank] = (int64_t)(id & 0xffffffffu);
+    mp.out_parents[out + rank] = (int64_t)(id >> 32);
   });
   for (int r = n + threadIdx.x; r < mp.k; r += kBmThreads) {  // too few candidates
     mp.out_scores[out + r] = -INFINITY;
@@ -510,6 +612,7 @@ constexpr int kMergeMaxSmem = (int)sizeof(MergeShared) + (kBsMaxBeams * kBsMaxEn
 // Blocks per warp: the split that takes the fewest rounds of blocks when 32 warps fit
 // an SM; a warp costs about half a block beside its blocks.
 BeamPlan beam_plan(int rows, int W, int V, int sm_count) {
+  const int64_t warps = 32LL * sm_count;
   BeamPlan pl;
   const int blocks = (int)(((int64_t)V + kBsBlock - 1) / kBsBlock);
   pl.run = (blocks + kBsMaxEntries - 1) / kBsMaxEntries;
@@ -517,7 +620,7 @@ BeamPlan beam_plan(int rows, int W, int V, int sm_count) {
   double best = 1e30;
   for (int e = 1; e <= pl.entries; ++e) {  // entries per warp
     const int segs = (pl.entries + e - 1) / e;
-    const int64_t rounds = ((int64_t)rows * segs + 32 * sm_count - 1) / (32 * sm_count);
+    const int64_t rounds = ((int64_t)rows * segs + warps - 1) / warps;
     const double cost = (double)rounds * (e * pl.run + 0.5);
     if (cost < best) {
       best = cost;

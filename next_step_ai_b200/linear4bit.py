@@ -146,37 +146,48 @@ class Linear4bit:
         """``x [..., K]`` -> ``y [..., N]`` (``out_dtype``, default x's); rows are
         processed in groups of ``max_rows_per_call``, each group streaming the
         weight once."""
-        dev, K, N = self.device, self.in_features, self.out_features
+        dev, K = self.device, self.in_features
         if x.device != dev:
             require_cuda(x, "x")
             raise RuntimeError(f"x is on {x.device} but the weight is on {dev}")
-        if x.dim() == 0 or x.shape[-1] != K:
-            raise RuntimeError(f"x has shape {tuple(x.shape)} but the layer expects {K} features")
-        xc, oc = dtype_code(x.dtype), dtype_code(out_dtype or x.dtype)
-        out = torch.empty((*x.shape[:-1], N), dtype=out_dtype or x.dtype, device=dev)
-        if out.numel() == 0:
+        shape = x.shape
+        if not shape or shape[-1] != K:
+            raise RuntimeError(f"x has shape {tuple(shape)} but the layer expects {K} features")
+        if out_dtype is None:
+            out_dtype = x.dtype
+        xc, oc = dtype_code(x.dtype), dtype_code(out_dtype)
+        out = torch.empty(*shape[:-1], self.out_features, dtype=out_dtype, device=dev)
+        if len(shape) != 2:
+            x = x.reshape(-1, K)
+        rows, (stride, inner) = x.shape[0], x.stride()
+        if rows == 0:
             return out
-        x = x if x.dim() == 2 else x.reshape(-1, K)
-        if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < K):
+        if inner != 1 or (rows > 1 and stride < K):
             x = x.contiguous()
+            stride = K
         if torch.cuda.current_device() != dev.index:
             with torch.cuda.device(dev):
-                self._run(x, xc, out, oc)
+                self._run(x, xc, stride, rows, out, oc)
         else:
-            self._run(x, xc, out, oc)
+            self._run(x, xc, stride, rows, out, oc)
         return out
 
-    def _run(self, x: torch.Tensor, xc: int, out: torch.Tensor, oc: int) -> None:
-        lib, rows, N = self._lib, x.shape[0], self.out_features
+    def _run(self, x: torch.Tensor, xc: int, stride: int, rows: int, out: torch.Tensor, oc: int) -> None:
+        lib, N, dev = self._lib, self.out_features, self.device
         per = 16 if xc == _lib.NSM_F32 else 32
-        stream, xs = stream_handle(self.device), x.stride(0)
         xp, op = x.data_ptr(), out.data_ptr()
-        for r0 in range(0, rows, per):
-            n = min(per, rows - r0)
+        stream = stream_handle(dev)
+        while True:
+            n = rows if rows < per else per
             need = self._ws_bytes.get((n, xc))
             if need is None:
                 need = self._ws_bytes[(n, xc)] = int(lib.nsm_linear4bit_workspace_bytes(n, xc, N, self.in_features))
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-            _lib.check(lib.nsm_linear4bit(xp + r0 * xs * x.element_size(), xc, n, xs, self._ref,
-                                          op + r0 * N * out.element_size(), oc, N, ws.data_ptr(), need, stream),
-                       "nsm_linear4bit")
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            status = lib.nsm_linear4bit(xp, xc, n, stride, self._ref, op, oc, N, ws.data_ptr(), need, stream)
+            if status:
+                _lib.check(status, "nsm_linear4bit")
+            rows -= n
+            if rows == 0:
+                return
+            xp += n * stride * x.element_size()
+            op += n * N * out.element_size()
