@@ -6,26 +6,28 @@
 // T is a 16-entry codebook (z = 0: NF4 and the like) or the identity (integer
 // weights, z = 8 or a zero point per group).
 //
-// Layout (written once by nsm_linear4bit_pack): tiles of 16 rows x 128 columns,
-// 1 KB each, row tile by row tile, so a warp streams contiguous memory with two
-// 16-byte loads per lane and tile.  Lane (g = lane / 4, t = lane % 4) holds, of
-// row g (first load) and row g + 8 (second), one 32-bit word for each of the
-// tile's four 32-column blocks: columns 32j + 8t .. + 8.  A block's two
-// mma.sync m16n8k16 therefore stay inside one scale group of 32 or more, and
-// their B fragments are 16 contiguous bytes of x in natural order.
+// Layout (written once by nsm_linear4bit_pack): tiles of 128 rows x 128 columns, 8 KB
+// each, row tile by row tile, as [4 column chunks][128 rows][16 bytes]: a thread owns a
+// row, and a warp's 16-byte loads are 512 contiguous bytes.  Scales and zero points lie
+// as [row tile][tile][128 rows][granules], a granule being the group or 128 columns.
 //
 // Three launches, linked by programmatic dependent launch:
 //  1. lin4_prep_kernel: per row of x a power-of-two scale that brings the
 //     largest finite |x| to [2^14, 2^15) and x as fp16 (exact for fp16, and for bf16
 //     down to 2^-38 of the row's largest); an fp32 x becomes two fp16 columns
-//     (value and remainder, 22 bits);
-//  2. lin4_kernel: one CTA of 16 warps per SM.  A unit is 256 rows (one tile per
-//     warp) x 128 columns; the units, row block by row block, are cut into equal
-//     contiguous runs, one per CTA, so no CTA finishes late, and the 16 warps
-//     read the same piece of x at the same time (it stays in L1).  fp16 weights x
-//     fp16 x on the tensor pipe with fp32 accumulation -- every product is exact
-//     -- and the group's scale is applied in fp32.  Each CTA leaves one
-//     fp32 partial per row block that it touched;
+//     (value and remainder, 22 bits).  x is written as the 8 x 16-byte core matrices of a
+//     K-major tensor-core operand;
+//  2. lin4_kernel: two CTAs per SM.  A unit is 256 rows x 128 columns; the units, row block
+//     by row block, are cut into equal contiguous runs, one per CTA, so no CTA
+//     finishes late.  Each of two warpgroups turns the 4-bit weights of its 128 rows into fp16
+//     (a byte -> half2 table for codebooks, mask and subtract for integers: both
+//     exact but for the codebook's rounding) and stores them to tensor memory, 32 or 64
+//     columns at a time, in two slots; a ninth warp multiplies them with x from shared
+//     memory (tcgen05.mma, M = 128 rows, N = the columns of x, fp32 accumulation),
+//     and the warpgroup adds scale * product to its fp32 sums in registers one slot later.
+//     With weights as the M operand in tensor memory x never passes through registers, so one
+//     row of x or 32 cost the threads the same but for the sums.  Each CTA leaves one fp32
+//     partial per row block that it touched;
 //  3. lin4_finalize_kernel: the partials of a row block in CTA order (the same
 //     bits every time), times the scale of x, + bias, in the output's type.
 #include <algorithm>
@@ -37,15 +39,16 @@
 namespace nsm {
 namespace {
 
-constexpr int kL4Warps = 16;
-constexpr int kL4Threads = 32 * kL4Warps;
-constexpr int kL4TileRows = 16;
+constexpr int kL4Groups = 2;                          // warpgroups of a CTA
+constexpr int kL4Threads = kL4Groups * 128 + 32;      // + the warp that issues copies and MMAs
+constexpr int kL4TileRows = 128;
 constexpr int kL4TileCols = 128;
 constexpr int kL4TileBytes = kL4TileRows * kL4TileCols / 2;
-constexpr int kL4BlockRows = kL4TileRows * kL4Warps;  // rows of a unit
+constexpr int kL4BlockRows = kL4TileRows * kL4Groups;  // rows of a unit
 constexpr int kL4MaxCols = 32;                        // fp16 columns of x in one call
 constexpr int kL4MaxSegs = 32;                        // CTAs that share one row block
-constexpr int kL4Depth = 3;                           // tiles in flight per warp
+constexpr int kL4Stages = 4;                          // x tiles in flight
+constexpr int kL4TmemCols = 256;                      // of 512: two CTAs per SM
 
 // Kinds of weights: codebook rounded to fp16; codebook as fp16 value +
 // remainder (22 bits, two table reads and two MMAs: outputs in fp32); integers
@@ -67,7 +70,7 @@ Lin4Shape lin4_shape(int N, int K, int group) {
   s.group = group;
   s.row_tiles = (N + kL4TileRows - 1) / kL4TileRows;
   s.steps = (K + kL4TileCols - 1) / kL4TileCols;
-  s.row_blocks = (s.row_tiles + kL4Warps - 1) / kL4Warps;
+  s.row_blocks = (s.row_tiles + kL4Groups - 1) / kL4Groups;
   s.kp = s.steps * kL4TileCols;
   s.npg = group % 128 == 0 ? 1 : (group % 64 == 0 ? 2 : 4);
   s.div = s.npg == 1 ? group / 128 : 1;
@@ -76,20 +79,21 @@ Lin4Shape lin4_shape(int N, int K, int group) {
 }
 
 // ---- packing ------------------------------------------------------------------
-// One thread per 32-bit word of the tiled weight.  Codebook words keep the byte
-// order (byte i = columns 2i, 2i+1: an index into the byte table).  Integer
-// words put columns c and c + 1 of a pair 16 bits apart, so one mask leaves a
-// half2: nibbles 0..7 = columns 0, 2, 4, 6, 1, 3, 5, 7.
+// One thread per 32-bit word of the tiled weight: columns 8w .. of a row.  Codebook
+// words keep the byte order (byte i = columns 2i, 2i+1: an index into the byte
+// table).  Integer words put columns c and c + 1 of a pair 16 bits apart, so one mask
+// leaves a half2: nibbles 0..7 = columns 0, 2, 4, 6, 1, 3, 5, 7.
 __global__ void lin4_pack_kernel(const uint8_t* __restrict__ src, int64_t row_bytes, Lin4Shape sh, int is_code,
                                  uint32_t* __restrict__ dst) {
-  const int64_t words = (int64_t)sh.row_tiles * sh.steps * (kL4TileBytes / 4);
+  constexpr int kWords = kL4TileBytes / 4;
+  const int64_t words = (int64_t)sh.row_tiles * sh.steps * kWords;
   const int kb = sh.K / 2;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < words; i += (int64_t)gridDim.x * blockDim.x) {
-    const int in_tile = (int)(i & 255);  // [2 halves][32 lanes][4 words]
-    const int64_t tile = i >> 8;
-    const int j = in_tile & 3, lane = (in_tile >> 2) & 31, h = in_tile >> 7;
-    const int64_t row = tile / sh.steps * kL4TileRows + (lane >> 2) + 8 * h;
-    const int col_byte = (int)(tile % sh.steps) * (kL4TileCols / 2) + 16 * j + 4 * (lane & 3);
+    const int in_tile = (int)(i % kWords);  // [4 chunks][128 rows][4 words]
+    const int64_t tile = i / kWords;
+    const int j = in_tile & 3, chunk = in_tile / (4 * kL4TileRows);
+    const int64_t row = tile / sh.steps * kL4TileRows + (in_tile / 4) % kL4TileRows;
+    const int col_byte = (int)(tile % sh.steps) * (kL4TileCols / 2) + 16 * chunk + 4 * j;
     uint32_t v = 0;
     if (row < sh.N) {
       const uint8_t* r = src + row * row_bytes;
@@ -106,17 +110,17 @@ __global__ void lin4_pack_kernel(const uint8_t* __restrict__ src, int64_t row_by
   }
 }
 
-// Scales (and zero points) as [row tile][scale step][8 g][npg][2 rows g, g + 8];
-// rows and columns past the end get scale 0 and zero point 0.
+// Scales (and zero points) as [row tile][scale step][128 rows][npg]; rows and columns
+// past the end get scale 0 and zero point 0.
 __global__ void lin4_pack_scales_kernel(const void* __restrict__ scales, int dt, const uint8_t* __restrict__ zeros,
                                         Lin4Shape sh, int groups, float* __restrict__ ds, uint8_t* __restrict__ dz) {
-  const int per = 16 * sh.npg;
+  const int per = kL4TileRows * sh.npg;
   const int64_t n = (int64_t)sh.row_tiles * sh.scale_steps * per;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
     const int e = (int)(i % per);
     const int64_t ts = i / per;
-    const int h = e & 1, pg = (e >> 1) % sh.npg, g = (e >> 1) / sh.npg;
-    const int64_t row = ts / sh.scale_steps * kL4TileRows + g + 8 * h;
+    const int pg = e % sh.npg;
+    const int64_t row = ts / sh.scale_steps * kL4TileRows + e / sh.npg;
     const int64_t col = (ts % sh.scale_steps) * sh.div * kL4TileCols + pg * (kL4TileCols / sh.npg);
     const int64_t grp = col / sh.group;
     const bool in = row < sh.N && grp < groups && col < sh.K;
@@ -139,38 +143,67 @@ __device__ __forceinline__ float code_scale(const float* code) {
   return ldexpf(1.f, max(-120, min(120, 6 - ilogbf(m))));
 }
 
-__global__ void __launch_bounds__(1024) lin4_prep_kernel(const void* x, int dt, int64_t stride, int K, int kp, int rows,
-                                                         int split, const float* code, __half* xh, float* scale) {
+// Halves of column c of x, column k of the weight: [tile][k / 8][c / 8][c % 8][k % 8].
+__device__ __forceinline__ int64_t x_index(int c, int k, int groups) {
+  const int step = k / kL4TileCols, kk = k % kL4TileCols;
+  return (((int64_t)step * (kL4TileCols / 8) + kk / 8) * groups + c / 8) * 64 + (c % 8) * 8 + kk % 8;
+}
+
+// CTA (slice, row): the row's largest value (each slice reads the whole row, from
+// L2, rather than wait for the others), then its slice as fp16.  kp / 8 runs of eight columns.
+__global__ void __launch_bounds__(256) lin4_prep_kernel(const void* x, int dt, int64_t stride, int K, int kp, int rows,
+                                                        int groups, const float* code, __half* xh, float* scale) {
   pdl_trigger();
-  __shared__ float wmax[32];
-  const int r = blockIdx.x;
+  __shared__ float wmax[8];
+  const int r = blockIdx.y;
   const int64_t base = (int64_t)r * stride;
+  const int es = dt == NSM_F32 ? 4 : 2;
+  const char* row = static_cast<const char*>(x) + base * es;
+  const bool vec = ((uintptr_t)row & 15) == 0;
   float s = 1.f;
+  auto finite = [](float v) {  // infinities and NaN stay what they are
+    const float a = fabsf(v);
+    return a <= 3.4028234e38f ? a : 0.f;
+  };
   if (dt != NSM_F16) {
     float m = 0.f;
-    for (int k = threadIdx.x; k < K; k += blockDim.x) {
-      const float a = fabsf(load_as_f32(x, dt, base + k));
-      if (a <= 3.4028234e38f) m = fmaxf(m, a);  // infinities and NaN stay what they are
+    const int per = 16 / es, nv = vec ? K / per : 0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nv; i += 256) {
+      const uint4 q = ldg_u4(row + 16 * (int64_t)i);
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (dt == NSM_F32) {
+          m = fmaxf(m, finite(__uint_as_float(w[j])));
+        } else {
+          m = fmaxf(m, fmaxf(finite(__uint_as_float(w[j] << 16)), finite(__uint_as_float(w[j] & 0xffff0000u))));
+        }
+      }
     }
+    for (int k = nv * per + threadIdx.x; k < K; k += 256) m = fmaxf(m, finite(load_as_f32(x, dt, base + k)));
     m = warp_max(m);
     if ((threadIdx.x & 31) == 0) wmax[threadIdx.x >> 5] = m;
     __syncthreads();
-    m = warp_max(wmax[threadIdx.x & 31]);
+    m = warp_max(wmax[threadIdx.x & 7]);
     if (m > 0.f) s = ldexpf(1.f, max(-120, min(120, ilogbf(m) - 14)));
   }
   const float inv = 1.f / s;  // a power of two: exact
-  __half* hi = xh + (int64_t)r * kp;
-  __half* lo = xh + (int64_t)(rows + r) * kp;
-  for (int k = threadIdx.x; k < kp; k += blockDim.x) {
-    const float v = k < K ? load_as_f32(x, dt, base + k) * inv : 0.f;
-    const __half h = __float2half_rn(v);
-    hi[k] = h;
-    if (split) {
-      const float rem = v - __half2float(h);
-      lo[k] = __float2half_rn(fabsf(rem) <= 3.4028234e38f ? rem : 0.f);
+  const int runs = kp / 8;
+  for (int q = blockIdx.x * 256 + threadIdx.x; q < runs; q += gridDim.x * 256) {
+    __half hi[8], lo[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int k = 8 * q + j;
+      const float v = k < K ? load_as_f32(x, dt, base + k) * inv : 0.f;
+      hi[j] = __float2half_rn(v);
+      const float rem = v - __half2float(hi[j]);
+      lo[j] = __float2half_rn(fabsf(rem) <= 3.4028234e38f ? rem : 0.f);
     }
+    *reinterpret_cast<uint4*>(xh + x_index(r, 8 * q, groups)) = *reinterpret_cast<const uint4*>(hi);
+    if (dt == NSM_F32) *reinterpret_cast<uint4*>(xh + x_index(rows + r, 8 * q, groups)) = *reinterpret_cast<const uint4*>(lo);
   }
-  if (threadIdx.x == 0) scale[r] = code ? s / code_scale(code) : s;
+  if (blockIdx.x == 0 && threadIdx.x == 0) scale[r] = code ? s / code_scale(code) : s;
 }
 
 // ---- products -------------------------------------------------------------------
@@ -181,16 +214,10 @@ struct Lin4Params {
   const float* code;
   const __half* xh;
   float* part;  // [row block][segment][column of x][256]
-  int row_tiles, steps, scale_steps, div, kp, cols;
-  int units, ctas, max_segs;
+  int row_tiles, steps, scale_steps, div, cols;
+  int units, ctas, max_segs, wait_limit;
 };
 
-// x written by the kernel before: volatile, so it is never moved over the wait
-__device__ __forceinline__ uint4 ld_x(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  return r;
-}
 __device__ __forceinline__ uint32_t hsub2_u32(uint32_t a, uint32_t b) {
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
@@ -210,67 +237,136 @@ __device__ __forceinline__ uint32_t int_pair(uint32_t w, uint32_t za, uint32_t z
   return hfma2_u32((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, zb);
 }
 
-template <int NPG>
-struct Lin4Stage {
-  uint4 a, b;
-  float s[2 * NPG];
-  uint32_t z[(NPG + 1) / 2];  // zero points, two bytes per granule
+// ---- tensor memory and the 5th-generation tensor core ----
+__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// 16 columns of the warp's 32 lanes
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t* r) {
+  if constexpr (N == 1) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r[0]) : "r"(addr) : "memory");
+  } else if constexpr (N == 2) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+  } else if constexpr (N == 4) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+  } else {
+    static_assert(N == 8, "columns at a time");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr)
+                 : "memory");
+  }
+}
+// D[128 lanes][N] (+)= A (tensor memory, fp16 pairs along K) x B (shared memory, K-major)
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b_desc), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+// The barrier is arrived at when the MMAs issued so far by this thread are done.
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+struct Lin4Bars {
+  unsigned long long full[kL4Groups][2];  // a slot of weights is in tensor memory
+  unsigned long long done[kL4Groups][2];  // its MMAs are done
+  unsigned long long x_full[kL4Stages];   // a tile of x is in shared memory
+  unsigned long long x_free[kL4Stages];   // the MMAs that read it are done
+  uint32_t tmem;
 };
 
-template <int MODE, int NPG, int NT>
-__global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(Lin4Params p) {
-  extern __shared__ __align__(1024) uint32_t l4_lut[];
+// NPG: scale granules per tile of 128 columns.  NC: columns of x that the sums hold.
+template <int MODE, int NPG, int NC>
+__global__ void __launch_bounds__(kL4Threads, 2) lin4_kernel(const __grid_constant__ Lin4Params p) {
+  extern __shared__ __align__(1024) uint32_t l4_smem[];
   constexpr bool kIsCode = MODE == kCode || MODE == kCodeExact;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t lanebase = (uint32_t)lane * 4u;
+  constexpr int kSlotCols = (NPG == 4 || MODE == kCodeExact) ? 32 : 64;  // weight columns per slot
+  constexpr int kSlots = kL4TileCols / kSlotCols;                        // per tile
+  constexpr int kSlotsPerScale = kSlots / NPG;
+  constexpr int kXGroups = NC <= 8 ? 1 : NC / 8;                         // groups of eight columns of x
+  constexpr int kXBytes = kXGroups * 8 * kL4TileCols * 2;                // of a tile
+  constexpr int kN = NC <= 16 ? 16 : 32;
+  // fp32 accumulators, fp16 operands, both K-major, N / 8 and M / 16 in bits 17 and 24
+  constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(kN / 8) << 17) | ((128u / 16) << 24);
+
+  unsigned char* smem = reinterpret_cast<unsigned char*>(l4_smem);
+  unsigned char* xs = smem + (kIsCode ? kLutBytes : 0);
+  Lin4Bars& bars = *reinterpret_cast<Lin4Bars*>(xs + kL4Stages * kXBytes + 1024);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int u0 = stream_begin(p.units, p.ctas, blockIdx.x), u1 = stream_begin(p.units, p.ctas, blockIdx.x + 1);
   pdl_trigger();
 
-  Lin4Stage<NPG> st[kL4Depth];
-  auto load = [&](Lin4Stage<NPG>& q, int rb, int step) {
-    const int rt = rb * kL4Warps + warp;
+  // the first tile of this thread's row is on its way while the tables are built
+  const int wg = warp >> 2, row = threadIdx.x & 127;
+  uint4 nw[4];
+  float ns[NPG];
+  uint32_t nz = 0;
+  auto load = [&](int rb, int step) {
+    const int rt = rb * kL4Groups + wg;
     if (rt >= p.row_tiles) return;
-    const uint8_t* w = p.w + ((int64_t)rt * p.steps + step) * kL4TileBytes + lane * 16;
-    q.a = ldg_stream_u4(w);
-    q.b = ldg_stream_u4(w + 512);
+    const uint8_t* w = p.w + ((int64_t)rt * p.steps + step) * kL4TileBytes + row * 16;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) nw[c] = ldg_stream_u4(w + c * kL4TileRows * 16);
     const int ss = (NPG == 1 && p.div > 1) ? step / p.div : step;
-    const int64_t e = (((int64_t)rt * p.scale_steps + ss) * 8 + g) * (2 * NPG);
+    const int64_t e = (((int64_t)rt * p.scale_steps + ss) * kL4TileRows + row) * NPG;
     if constexpr (NPG == 1) {
+      ns[0] = __ldg(p.s + e);
+      if (MODE == kIntZeros) nz = __ldg(p.z + e);
+    } else if constexpr (NPG == 2) {
       const float2 v = __ldg(reinterpret_cast<const float2*>(p.s + e));
-      q.s[0] = v.x;
-      q.s[1] = v.y;
-      if (MODE == kIntZeros) q.z[0] = __ldg(reinterpret_cast<const unsigned short*>(p.z + e));
+      ns[0] = v.x;
+      ns[1] = v.y;
+      if (MODE == kIntZeros) nz = __ldg(reinterpret_cast<const unsigned short*>(p.z + e));
     } else {
-#pragma unroll
-      for (int i = 0; i < NPG / 2; ++i) {
-        const float4 v = ldg_f4(p.s + e + 4 * i);
-        q.s[4 * i] = v.x;
-        q.s[4 * i + 1] = v.y;
-        q.s[4 * i + 2] = v.z;
-        q.s[4 * i + 3] = v.w;
-        if (MODE == kIntZeros) q.z[i] = __ldg(reinterpret_cast<const uint32_t*>(p.z + e + 4 * i));
-      }
+      const float4 v = ldg_f4(p.s + e);
+      ns[0] = v.x;
+      ns[1] = v.y;
+      ns[2] = v.z;
+      ns[3] = v.w;
+      if (MODE == kIntZeros) nz = __ldg(reinterpret_cast<const uint32_t*>(p.z + e));
     }
   };
-  int prb = u0 / p.steps, pstep = u0 - prb * p.steps;  // the next unit to load
-  auto advance = [&](int& rb, int& step) {
-    if (++step == p.steps) {
-      step = 0;
-      ++rb;
-    }
-  };
-  int rb = prb, step = pstep;  // the next unit to multiply
-#pragma unroll
-  for (int d = 0; d < kL4Depth; ++d) {
-    if (u0 + d < u1) {
-      load(st[d], prb, pstep);
-      advance(prb, pstep);
-    }
-  }
+  int rb = u0 / p.steps, step = u0 - rb * p.steps;
+  if (warp < 4 * kL4Groups && u0 < u1) load(rb, step);
 
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem)),
+                 "r"((uint32_t)kL4TmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (threadIdx.x == 32) {
+    for (int i = 0; i < kL4Groups * 2; ++i) {
+      mbar_init(smem_u32(&bars.full[i / 2][i % 2]), 4);  // the group's four warps
+      mbar_init(smem_u32(&bars.done[i / 2][i % 2]), 1);
+    }
+    for (int i = 0; i < kL4Stages; ++i) {
+      mbar_init(smem_u32(&bars.x_full[i]), 1);
+      mbar_init(smem_u32(&bars.x_free[i]), 1);
+    }
+    mbar_init_fence();
+  }
   if constexpr (kIsCode) {  // byte -> half2 table, one copy per lane (conflict-free); the second holds the remainders
     const float cs = code_scale(p.code);
-    uint4* lut4 = reinterpret_cast<uint4*>(l4_lut);
+    uint4* lut4 = reinterpret_cast<uint4*>(smem);
     for (int i = threadIdx.x; i < 256 * 16; i += kL4Threads) {
       const int e = i >> 4;
       if (MODE == kCode && (i & 8)) continue;
@@ -283,124 +379,198 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(Lin4Params p) {
       const uint32_t v = (uint32_t)__half_as_ushort(h0) | ((uint32_t)__half_as_ushort(h1) << 16);
       lut4[i] = make_uint4(v, v, v, v);
     }
-    __syncthreads();
   }
-  pdl_wait();
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = bars.tmem;
+  // per group: two slots of weights (32 columns of fp16 pairs each), two products
+  constexpr uint32_t kA = 32, kD = 32, kPerGroup = 128;
 
-  const __half* xlane = p.xh + (int64_t)g * p.kp + 8 * t;
-  float acc[NT][4];
+  if (warp == 4 * kL4Groups) {
+    // ---- copies of x and MMAs: one thread; every wait is bounded, and one that runs out
+    // ends the issue (the warpgroups' own waits then run out, and leave NaN)
+    if (lane == 0) {
+      pdl_wait();
+      fence_proxy_async_global();
+      const uint64_t keep = l2_evict_last_policy();
+      auto copy = [&](int u) {  // the tile of x of unit u
+        const int st = (u - u0) % kL4Stages;
+        const uint32_t bar = smem_u32(&bars.x_full[st]);
+        mbar_arrive_expect_tx(bar, kXBytes);
+        bulk_g2s(smem_u32(xs + st * kXBytes), reinterpret_cast<const unsigned char*>(p.xh) + (int64_t)(u % p.steps) * kXBytes,
+                 kXBytes, bar, keep);
+      };
+      for (int u = u0; u < min(u1, u0 + kL4Stages); ++u) copy(u);
+      int copied = min(u1, u0 + kL4Stages), landed = u0, issued = u0;
+      bool ok = true;
+      int n[kL4Groups] = {0, 0}, scales[kL4Groups] = {0, 0};  // slots and scale granules issued so far
+      for (int u = u0; u < u1 && ok; ++u) {
+        const int st = (u - u0) % kL4Stages;
+        ok = mbar_wait(smem_u32(&bars.x_full[st]), ((u - u0) / kL4Stages) & 1, p.wait_limit);
+        landed = u + (ok ? 1 : 0);
+        const uint32_t x0 = smem_u32(xs + st * kXBytes);
+        for (int t = 0; t < kSlots && ok; ++t) {
+          for (int g = 0; g < kL4Groups && ok; ++g) {
+            if (rb * kL4Groups + g >= p.row_tiles) continue;
+            const int slot = n[g] & 1;
+            ok = mbar_wait(smem_u32(&bars.full[g][slot]), (n[g] >> 1) & 1, p.wait_limit);
+            if (!ok) break;
+            tmem_fence_after();
+            const uint32_t d = tmem + g * kPerGroup + 2 * kA + (scales[g] & 1) * kD;
+            const uint32_t a = tmem + g * kPerGroup + slot * kA;
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+            for (int half = 0; half < (MODE == kCodeExact ? 2 : 1); ++half) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
-
-  auto flush = [&](int at) {  // this warp's partial of row block `at`
-    if (at * kL4Warps + warp < p.row_tiles) {
-      const int seg = (int)blockIdx.x - stream_owner(p.units, p.ctas, at * p.steps);
-      float* dst = p.part + ((int64_t)(at * p.max_segs + seg) * p.cols) * kL4BlockRows + warp * kL4TileRows + g;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int c = 8 * n + 2 * t + (i & 1);
-          if (c < p.cols) dst[(int64_t)c * kL4BlockRows + (i >> 1) * 8] = acc[n][i];
+              for (int k = 0; k < kSlotCols / 16; ++k) {
+                // K-major without swizzle: 8 columns of the weight are kXGroups x 128 bytes on, 8 columns of
+                // x 128 bytes (with one group the upper eight of N = 16 are never read back)
+                const uint32_t at = x0 + (uint32_t)(t * (kSlotCols / 8) + 2 * k) * (kXGroups * 128u);
+                const uint64_t desc = (uint64_t)((at >> 4) & 0x3fff) | ((uint64_t)(kXGroups * 128 / 16) << 16) |
+                                      ((uint64_t)(128 / 16) << 32) | (1ull << 46);
+                mma_f16_ts(d, a + half * (kSlotCols / 2) + k * 8, desc, kIdesc,
+                           !(t % kSlotsPerScale == 0 && half == 0 && k == 0));
+              }
+            }
+            mma_commit(smem_u32(&bars.done[g][slot]));
+            ++n[g];
+            if (t % kSlotsPerScale == kSlotsPerScale - 1) ++scales[g];
+          }
         }
+        mma_commit(smem_u32(&bars.x_free[st]));
+        issued = u + 1;
+        if (++step == p.steps) {
+          step = 0;
+          ++rb;
+        }
+        // the tile before this one is read: its place takes the next copy
+        if (ok && u > u0 && copied < u1) {
+          const int pt = (u - 1 - u0) % kL4Stages;
+          ok = mbar_wait(smem_u32(&bars.x_free[pt]), ((u - 1 - u0) / kL4Stages) & 1, p.wait_limit);
+          if (ok) copy(copied++);
+        }
+      }
+      // nothing may arrive in shared memory that is gone: the last commits, and after a failure copies
+      for (int u = max(u0, issued - kL4Stages); u < issued; ++u)
+        mbar_wait(smem_u32(&bars.x_free[(u - u0) % kL4Stages]), ((u - u0) / kL4Stages) & 1);
+      for (int u = landed; u < copied; ++u)
+        mbar_wait(smem_u32(&bars.x_full[(u - u0) % kL4Stages]), ((u - u0) / kL4Stages) & 1);
     }
+    __syncwarp();
+  } else {
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of tensor memory
+    const uint32_t a0 = tmem + lanes + wg * kPerGroup, d0 = a0 + 2 * kA;
+    const uint32_t lanebase = (uint32_t)lane * 4u;
+    float acc[NC];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int c = 0; c < NC; ++c) acc[c] = 0.f;
+    bool ok = true;
+    int n = 0, scales = 0;  // slots stored and scale granules finished
+    float last_scale = 0.f;
+    int open = -1;          // row block of the sums, and of the slot that is not added yet
+    auto add_scaled = [&](float s) {  // the products of the granule that is done, scaled
+      const uint32_t d = d0 + (scales & 1) * kD;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
-  };
-
-  auto multiply = [&](const Lin4Stage<NPG>& q, int at, int stp) {
-    if (at * kL4Warps + warp >= p.row_tiles) return;
-    float d[NT][4];
+      for (int c0 = 0; c0 < NC; c0 += 8) {
+        uint32_t r[8];
+        tmem_ld<(NC < 8 ? NC : 8)>(d + c0, r);
+        tmem_wait_ld();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      constexpr int kPer = 4 / NPG;  // 32-column blocks per scale
-      if (j % kPer == 0) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) d[n][i] = 0.f;
+        for (int c = 0; c < (NC < 8 ? NC : 8); ++c) acc[c0 + c] = fmaf(s, __uint_as_float(r[c]), acc[c0 + c]);
       }
-      uint4 xf[NT];
+      ++scales;
+    };
+    auto wait_slot = [&](int i) {  // the MMAs of slot number i are done
+      if (ok) ok = mbar_wait(smem_u32(&bars.done[wg][i & 1]), (i >> 1) & 1, p.wait_limit);
+      __syncwarp();
+      tmem_fence_after();
+    };
+    auto flush = [&]() {
+      const int seg = (int)blockIdx.x - stream_owner(p.units, p.ctas, open * p.steps);
+      float* dst = p.part + ((int64_t)(open * p.max_segs + seg) * p.cols) * kL4BlockRows + wg * kL4TileRows + row;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        xf[n] = make_uint4(0, 0, 0, 0);
-        if (8 * n + g < p.cols) xf[n] = ld_x(xlane + (int64_t)(8 * n) * p.kp + stp * kL4TileCols + 32 * j);
+      for (int c = 0; c < NC; ++c) {
+        if (c < p.cols) dst[(int64_t)c * kL4BlockRows] = ok ? acc[c] : __int_as_float(0x7fc00000);
+        acc[c] = 0.f;
       }
-      const uint32_t wa = j == 0 ? q.a.x : j == 1 ? q.a.y : j == 2 ? q.a.z : q.a.w;
-      const uint32_t wb = j == 0 ? q.b.x : j == 1 ? q.b.y : j == 2 ? q.b.z : q.b.w;
-      uint32_t f[8];  // A fragments of the block's two MMAs
-      if constexpr (kIsCode) {
+    };
+    for (int u = u0; u < u1; ++u) {
+      if (rb * kL4Groups + wg >= p.row_tiles) break;  // only in the last row block
+      uint4 w[4];
+      float s[NPG];
 #pragma unroll
-        for (int tab = 0; tab < (MODE == kCodeExact ? 2 : 1); ++tab) {
+      for (int c = 0; c < 4; ++c) w[c] = nw[c];
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            f[4 * (b >> 1) + 2 * (b & 1)] = lut_lookup_rt(l4_lut, wa, lanebase, b, tab);
-            f[4 * (b >> 1) + 2 * (b & 1) + 1] = lut_lookup_rt(l4_lut, wb, lanebase, b, tab);
-          }
+      for (int c = 0; c < NPG; ++c) s[c] = ns[c];
+      const uint32_t z = nz;
+      int nrb = rb, nstep = step + 1;
+      if (nstep == p.steps) {
+        nstep = 0;
+        ++nrb;
+      }
+      if (u + 1 < u1) load(nrb, nstep);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma_16816(d[n], f[0], f[1], f[2], f[3], xf[n].x, xf[n].y);
-            mma_16816(d[n], f[4], f[5], f[6], f[7], xf[n].z, xf[n].w);
-          }
-        }
-      } else {
-        uint32_t za = 0x64086408u, zb = 0xd480d480u;  // 1032, -72
-        uint32_t za8 = za, zb8 = zb;
+      for (int t = 0; t < kSlots; ++t) {
+        const uint32_t a = a0 + (n & 1) * kA;
+        uint32_t za = 0x64086408u, zb = 0xd480d480u;  // 1024 + 8, -(64 + 8)
         if constexpr (MODE == kIntZeros) {
-          const int gr = j / kPer;
-          const uint32_t zz = q.z[gr / 2] >> (16 * (gr % 2));
-          const uint32_t z0 = zz & 255u, z1 = (zz >> 8) & 255u;
-          za = (0x6400u | z0) * 0x10001u;
-          za8 = (0x6400u | z1) * 0x10001u;
-          zb = hsub2_u32(0x63806380u, za);   // 960 - (1024 + z)
-          zb8 = hsub2_u32(0x63806380u, za8);
+          za = (0x6400u | ((z >> (8 * (t / kSlotsPerScale))) & 255u)) * 0x10001u;
+          zb = hsub2_u32(0x63806380u, za);  // 960 - (1024 + z)
         }
-        f[0] = int_pair<0>(wa, za, zb);
-        f[1] = int_pair<0>(wb, za8, zb8);
-        f[2] = int_pair<1>(wa, za, zb);
-        f[3] = int_pair<1>(wb, za8, zb8);
-        f[4] = int_pair<2>(wa, za, zb);
-        f[5] = int_pair<2>(wb, za8, zb8);
-        f[6] = int_pair<3>(wa, za, zb);
-        f[7] = int_pair<3>(wb, za8, zb8);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          mma_16816(d[n], f[0], f[1], f[2], f[3], xf[n].x, xf[n].y);
-          mma_16816(d[n], f[4], f[5], f[6], f[7], xf[n].z, xf[n].w);
-        }
-      }
-      if (j % kPer == kPer - 1) {
-        const float s0 = q.s[2 * (j / kPer)], s1 = q.s[2 * (j / kPer) + 1];
+        for (int c = 0; c < kSlotCols / 32; ++c) {
+          const uint4 q = w[t * (kSlotCols / 32) + c];
+          const uint32_t word[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          acc[n][0] = fmaf(s0, d[n][0], acc[n][0]);
-          acc[n][1] = fmaf(s0, d[n][1], acc[n][1]);
-          acc[n][2] = fmaf(s1, d[n][2], acc[n][2]);
-          acc[n][3] = fmaf(s1, d[n][3], acc[n][3]);
+          for (int half = 0; half < (MODE == kCodeExact ? 2 : 1); ++half) {
+            uint32_t r[16];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if constexpr (kIsCode) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) r[4 * j + b] = lut_lookup_rt(l4_smem, word[j], lanebase, b, half);
+              } else {
+                r[4 * j] = int_pair<0>(word[j], za, zb);
+                r[4 * j + 1] = int_pair<1>(word[j], za, zb);
+                r[4 * j + 2] = int_pair<2>(word[j], za, zb);
+                r[4 * j + 3] = int_pair<3>(word[j], za, zb);
+              }
+            }
+            tmem_st16(a + half * (kSlotCols / 2) + c * 16, r);
+          }
         }
+        tmem_wait_st();
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bars.full[wg][n & 1]));
+        // the slot before this one: its products are done, or soon
+        if (n > 0) {
+          wait_slot(n - 1);
+          if (t == 0) {
+            add_scaled(last_scale);
+            if (open != rb) flush();
+          } else if (t % kSlotsPerScale == 0) {
+            add_scaled(s[t / kSlotsPerScale - 1]);
+          }
+        }
+        if (t == 0) open = rb;
+        ++n;
       }
+      last_scale = s[NPG - 1];
+      rb = nrb;
+      step = nstep;
     }
-  };
-
-  for (int u = u0; u < u1; u += kL4Depth) {
-#pragma unroll
-    for (int d = 0; d < kL4Depth; ++d) {
-      if (u + d < u1) {
-        multiply(st[d], rb, step);
-        if (u + d + kL4Depth < u1) {
-          load(st[d], prb, pstep);
-          advance(prb, pstep);
-        }
-        const int done = rb;
-        advance(rb, step);
-        if (rb != done || u + d + 1 == u1) flush(done);
-      }
+    if (n > 0) {
+      wait_slot(n - 1);
+      add_scaled(last_scale);
+      flush();
     }
+    tmem_fence_before();
   }
+  __syncthreads();
+  tmem_fence_after();
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kL4TmemCols) : "memory");
 }
 
 __global__ void __launch_bounds__(kL4BlockRows) lin4_finalize_kernel(const float* part, const float* scale, int units,
@@ -427,7 +597,7 @@ __global__ void __launch_bounds__(kL4BlockRows) lin4_finalize_kernel(const float
 }
 
 struct Lin4Plan {
-  int cols = 0, units = 0, ctas = 0, max_segs = 0;
+  int cols = 0, col_groups = 1, units = 0, ctas = 0, max_segs = 0;
   size_t scale_off = 0, part_off = 0, bytes = 0;
 };
 
@@ -435,10 +605,11 @@ Lin4Plan lin4_plan(const Lin4Shape& sh, int rows, int x_dtype, int sm_count) {
   Lin4Plan pl;
   pl.cols = x_dtype == NSM_F32 ? 2 * rows : rows;
   pl.units = sh.row_blocks * sh.steps;
-  pl.ctas = std::max(1, std::min({sm_count, pl.units, sh.row_blocks * (kL4MaxSegs - 2)}));
+  pl.ctas = std::max(1, std::min({2 * sm_count, pl.units, sh.row_blocks * (kL4MaxSegs - 2)}));
   const int least = pl.units / pl.ctas;  // units of the shortest run
   pl.max_segs = (sh.steps - 1 + least - 1) / least + 1;
-  pl.scale_off = align_up((size_t)pl.cols * sh.kp * 2, 256);
+  pl.col_groups = pl.cols <= 8 ? 1 : pl.cols <= 16 ? 2 : 4;
+  pl.scale_off = align_up((size_t)pl.col_groups * 8 * sh.kp * 2, 256);
   pl.part_off = pl.scale_off + align_up((size_t)rows * 4, 256);
   pl.bytes = pl.part_off + (size_t)sh.row_blocks * pl.max_segs * pl.cols * kL4BlockRows * 4;
   return pl;
@@ -453,13 +624,18 @@ int lin4_max_rows(int x_dtype) { return x_dtype == NSM_F32 ? kL4MaxCols / 2 : kL
 
 using Lin4Fn = void (*)(Lin4Params);
 
+// Columns of x that the sums hold: the next of 1, 2, 4, 8, 16, 32.
+int lin4_col_case(int cols) { return cols <= 1 ? 0 : cols <= 2 ? 1 : cols <= 4 ? 2 : cols <= 8 ? 3 : cols <= 16 ? 4 : 5; }
+
 template <int MODE, int NPG>
-Lin4Fn lin4_pick_nt(int cols) {
-  return cols <= 8 ? lin4_kernel<MODE, NPG, 1> : cols <= 16 ? lin4_kernel<MODE, NPG, 2> : lin4_kernel<MODE, NPG, 4>;
+Lin4Fn lin4_pick_cols(int c) {
+  constexpr Lin4Fn fns[6] = {lin4_kernel<MODE, NPG, 1>, lin4_kernel<MODE, NPG, 2>,  lin4_kernel<MODE, NPG, 4>,
+                             lin4_kernel<MODE, NPG, 8>, lin4_kernel<MODE, NPG, 16>, lin4_kernel<MODE, NPG, 32>};
+  return fns[c];
 }
 template <int MODE>
-Lin4Fn lin4_pick_npg(int npg, int cols) {
-  return npg == 1 ? lin4_pick_nt<MODE, 1>(cols) : npg == 2 ? lin4_pick_nt<MODE, 2>(cols) : lin4_pick_nt<MODE, 4>(cols);
+Lin4Fn lin4_pick_npg(int npg, int c) {
+  return npg == 1 ? lin4_pick_cols<MODE, 1>(c) : npg == 2 ? lin4_pick_cols<MODE, 2>(c) : lin4_pick_cols<MODE, 4>(c);
 }
 
 }  // namespace
@@ -478,7 +654,7 @@ size_t nsm_linear4bit_packed_bytes(int32_t out_features, int32_t in_features) {
 size_t nsm_linear4bit_scale_count(int32_t out_features, int32_t in_features, int32_t group_size) {
   if (!lin4_size_ok(out_features, in_features, group_size)) return 0;
   const Lin4Shape sh = lin4_shape(out_features, in_features, group_size);
-  return (size_t)sh.row_tiles * sh.scale_steps * 16 * sh.npg;
+  return (size_t)sh.row_tiles * sh.scale_steps * kL4TileRows * sh.npg;
 }
 
 int nsm_linear4bit_max_rows(int32_t x_dtype) { return lin4_max_rows(x_dtype); }
@@ -505,7 +681,7 @@ int nsm_linear4bit_pack(const uint8_t* packed, int64_t packed_row_bytes, const v
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int groups = (in_features + group_size - 1) / group_size;
   const int64_t words = (int64_t)sh.row_tiles * sh.steps * (kL4TileBytes / 4);
-  const int64_t ns = (int64_t)sh.row_tiles * sh.scale_steps * 16 * sh.npg;
+  const int64_t ns = (int64_t)sh.row_tiles * sh.scale_steps * kL4TileRows * sh.npg;
   lin4_pack_kernel<<<(int)std::min<int64_t>((words + 255) / 256, 64L * di.sm_count), 256, 0, s>>>(
       packed, packed_row_bytes, sh, codebook != 0, reinterpret_cast<uint32_t*>(packed_out));
   NSM_CHECK_CUDA(cudaGetLastError());
@@ -561,16 +737,18 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
   // it to fp16 (2^-12 of a value at most, random over the columns: about 1e-4 of the output,
   // half an fp16 rounding), which halves the table reads that bound the kernel
   const int mode = w->code ? (out_dtype == NSM_F32 ? kCodeExact : kCode) : (w->zeros ? kIntZeros : kInt);
-  Lin4Fn fn = mode == kCode        ? lin4_pick_npg<kCode>(sh.npg, pl.cols)
-              : mode == kCodeExact ? lin4_pick_npg<kCodeExact>(sh.npg, pl.cols)
-              : mode == kInt       ? lin4_pick_npg<kInt>(sh.npg, pl.cols)
-                                   : lin4_pick_npg<kIntZeros>(sh.npg, pl.cols);
-  const size_t smem = w->code ? (size_t)kLutBytes : 0;
-  static SmemOnce once[2][3][3];
-  if (smem > 0)
-    NSM_CHECK_CUDA(once[mode][sh.npg / 2][pl.cols <= 8 ? 0 : pl.cols <= 16 ? 1 : 2].set(fn, (int)smem, di.device));
-  lin4_prep_kernel<<<rows, 1024, 0, s>>>(x, x_dtype, x_row_stride, sh.K, sh.kp, rows, x_dtype == NSM_F32, w->code, xh,
-                                         scale);
+  const int cc = lin4_col_case(pl.cols);
+  Lin4Fn fn = mode == kCode        ? lin4_pick_npg<kCode>(sh.npg, cc)
+              : mode == kCodeExact ? lin4_pick_npg<kCodeExact>(sh.npg, cc)
+              : mode == kInt       ? lin4_pick_npg<kInt>(sh.npg, cc)
+                                   : lin4_pick_npg<kIntZeros>(sh.npg, cc);
+  const size_t smem = (w->code ? (size_t)kLutBytes : 0) + (size_t)kL4Stages * pl.col_groups * 8 * kL4TileCols * 2 + 1024 +
+                      sizeof(Lin4Bars);
+  static SmemOnce once[4][3][6];
+  NSM_CHECK_CUDA(once[mode][sh.npg / 2][cc].set(fn, (int)smem, di.device));
+  const int slices = std::max(1, std::min(8, sh.kp / 2048));
+  lin4_prep_kernel<<<dim3(slices, rows), 256, 0, s>>>(x, x_dtype, x_row_stride, sh.K, sh.kp, rows, pl.col_groups, w->code,
+                                                      xh, scale);
   NSM_CHECK_CUDA(cudaGetLastError());
   Lin4Params p;
   p.w = w->packed;
@@ -583,11 +761,11 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
   p.steps = sh.steps;
   p.scale_steps = sh.scale_steps;
   p.div = sh.div;
-  p.kp = sh.kp;
   p.cols = pl.cols;
   p.units = pl.units;
   p.ctas = pl.ctas;
   p.max_segs = pl.max_segs;
+  p.wait_limit = copy_wait_spins();
   NSM_CHECK_CUDA(launch_pdl(fn, dim3(pl.ctas), dim3(kL4Threads), smem, s, p));
   NSM_CHECK_CUDA(launch_pdl(lin4_finalize_kernel, dim3(sh.row_blocks, rows), dim3(kL4BlockRows), 0, s,
                             (const float*)part, (const float*)scale, pl.units, pl.ctas, sh.steps, pl.max_segs, pl.cols,

@@ -19,12 +19,12 @@ def lib():
 @pytest.mark.parametrize("N,K,gs", [(1, 2, 32), (16, 128, 64), (17, 130, 64), (1001, 2086, 128), (257, 1026, 96),
                                     (512, 4096, 4096)])
 def test_packed_sizes(lib, N, K, gs):
-    tiles = -(-N // 16) * -(-K // 128)                     # 16 x 128 weights, 1 KB each
-    assert lib.nsm_linear4bit_packed_bytes(N, K) == 1024 * tiles
+    tiles = -(-N // 128) * -(-K // 128)                    # 128 x 128 weights, 8 KB each
+    assert lib.nsm_linear4bit_packed_bytes(N, K) == 8192 * tiles
     per_tile = 1 if gs % 128 == 0 else 2 if gs % 64 == 0 else 4
     steps = -(-K // 128)
     entries = -(-steps // (gs // 128)) if per_tile == 1 else steps
-    assert lib.nsm_linear4bit_scale_count(N, K, gs) == -(-N // 16) * 16 * entries * per_tile
+    assert lib.nsm_linear4bit_scale_count(N, K, gs) == -(-N // 128) * 128 * entries * per_tile
 
 
 def test_sizes_that_are_refused(lib):
