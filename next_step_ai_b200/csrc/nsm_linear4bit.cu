@@ -17,17 +17,18 @@
 //     down to 2^-38 of the row's largest); an fp32 x becomes two fp16 columns
 //     (value and remainder, 22 bits).  x is written as the 8 x 16-byte core matrices of a
 //     K-major tensor-core operand;
-//  2. lin4_kernel: two CTAs per SM.  A unit is 256 rows x 128 columns; the units, row block
-//     by row block, are cut into equal contiguous runs, one per CTA, so no CTA
-//     finishes late.  Each of two warpgroups turns the 4-bit weights of its 128 rows into fp16
-//     (a byte -> half2 table for codebooks, mask and subtract for integers: both
-//     exact but for the codebook's rounding) and stores them to tensor memory, 32 or 64
-//     columns at a time, in two slots; a ninth warp multiplies them with x from shared
-//     memory (tcgen05.mma, M = 128 rows, N = the columns of x, fp32 accumulation),
-//     and the warpgroup adds scale * product to its fp32 sums in registers one slot later.
-//     With weights as the M operand in tensor memory x never passes through registers, so one
-//     row of x or 32 cost the threads the same but for the sums.  Each CTA leaves one fp32
-//     partial per row block that it touched;
+//  2. lin4_kernel: one CTA per SM, four warpgroups of 128 rows each.  A unit is 512 rows x
+//     128 columns; the units, row block by row block, are cut into equal contiguous runs,
+//     one per CTA, so no CTA finishes late.  Bulk copies bring each warpgroup's tile and
+//     scales into its own ring, and x into a ring that all share.  A warpgroup turns its
+//     tile into fp16 (a byte -> half2 table for codebooks, mask and subtract for
+//     integers: both exact but for the codebook's rounding), stores it to tensor
+//     memory, and one of its threads multiplies it with x (tcgen05.mma, M = 128 rows, N =
+//     the columns of x, fp32 accumulation); then it adds scale * product to its
+//     fp32 sums in registers.  The four warpgroups are in different phases of this, so one's round
+//     trip is another's arithmetic.  With weights as the M operand in tensor memory x never
+//     passes through registers: one row of x or 32 cost the threads the same but for the sums.
+//     Each CTA leaves one fp32 partial per row block that it touched;
 //  3. lin4_finalize_kernel: the partials of a row block in CTA order (the same
 //     bits every time), times the scale of x, + bias, in the output's type.
 #include <algorithm>
@@ -39,16 +40,17 @@
 namespace nsm {
 namespace {
 
-constexpr int kL4Groups = 2;                          // warpgroups of a CTA
-constexpr int kL4Threads = kL4Groups * 128 + 32;      // + the warp that issues copies and MMAs
+constexpr int kL4Groups = 4;                          // warpgroups of a CTA
+constexpr int kL4Threads = kL4Groups * 128 + 32;      // + the warp that copies x
 constexpr int kL4TileRows = 128;
 constexpr int kL4TileCols = 128;
 constexpr int kL4TileBytes = kL4TileRows * kL4TileCols / 2;
 constexpr int kL4BlockRows = kL4TileRows * kL4Groups;  // rows of a unit
 constexpr int kL4MaxCols = 32;                        // fp16 columns of x in one call
 constexpr int kL4MaxSegs = 32;                        // CTAs that share one row block
-constexpr int kL4Stages = 4;                          // x tiles in flight
-constexpr int kL4TmemCols = 256;                      // of 512: two CTAs per SM
+constexpr int kL4XStages = 4;                         // x tiles in flight
+// tensor memory: per warpgroup 64 columns of weights (fp16 pairs) and 64 of products
+constexpr uint32_t kL4TmemA = 64, kL4TmemGroup = 128;
 
 // Kinds of weights: codebook rounded to fp16; codebook as fp16 value +
 // remainder (22 bits, two table reads and two MMAs: outputs in fp32); integers
@@ -264,6 +266,12 @@ __device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t* r) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                  : "r"(addr)
                  : "memory");
+  } else if constexpr (N == 16) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr)
+                 : "memory");
   } else {
     static_assert(N == 8, "columns at a time");
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -285,86 +293,93 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-struct Lin4Bars {
-  unsigned long long full[kL4Groups][2];  // a slot of weights is in tensor memory
-  unsigned long long done[kL4Groups][2];  // its MMAs are done
-  unsigned long long x_full[kL4Stages];   // a tile of x is in shared memory
-  unsigned long long x_free[kL4Stages];   // the MMAs that read it are done
-  uint32_t tmem;
+// What a kernel variant holds, for device and host.  NPG: scale granules per tile of 128
+// columns.  NC: columns of x that the sums hold.
+template <int MODE, int NPG, int NC>
+struct Lin4Config {
+  static constexpr bool kIsCode = MODE == kCode || MODE == kCodeExact;
+  static constexpr int kXGroups = NC <= 8 ? 1 : NC / 8;                    // groups of eight columns of x
+  static constexpr int kXBytes = kXGroups * 8 * kL4TileCols * 2;           // of a tile
+  static constexpr int kN = NC <= 16 ? 16 : 32;                            // of the MMA
+  // weight columns stored before the MMAs: what fits 64 + 64 columns of tensor memory
+  static constexpr int kSlotCols = (MODE == kCodeExact || (NPG == 4 && kN == 32)) ? 64 : 128;
+  static constexpr int kScaleBytes = kL4TileRows * NPG * 4;
+  static constexpr int kStageBytes = kL4TileBytes + kScaleBytes + (MODE == kIntZeros ? kL4TileRows * NPG : 0);
+  static constexpr int kStages = kIsCode ? 3 : 4;                          // weight tiles in flight per warpgroup
+  static constexpr int kLut = kIsCode ? kLutBytes : 0;
+  static constexpr int kRing = kLut, kX = kRing + kL4Groups * kStages * kStageBytes;
+  static constexpr int kBars = kX + kL4XStages * kXBytes + 1024;  // the last tile of x is read 128 bytes over
+  static constexpr int kSmem = kBars + 256;
+  static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
-// NPG: scale granules per tile of 128 columns.  NC: columns of x that the sums hold.
+struct Lin4Bars {
+  unsigned long long w_full[kL4Groups][4];  // a tile of weights and its scales are in shared memory
+  unsigned long long done[kL4Groups];       // the MMAs of a slot are done
+  unsigned long long x_full[kL4XStages];    // a tile of x is in shared memory
+  unsigned long long x_free[kL4XStages];    // all warpgroups' MMAs that read it are done
+  uint32_t tmem;
+};
+static_assert(sizeof(Lin4Bars) <= 256, "barriers");
+
 template <int MODE, int NPG, int NC>
-__global__ void __launch_bounds__(kL4Threads, 2) lin4_kernel(const __grid_constant__ Lin4Params p) {
+__global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_constant__ Lin4Params p) {
   extern __shared__ __align__(1024) uint32_t l4_smem[];
-  constexpr bool kIsCode = MODE == kCode || MODE == kCodeExact;
-  constexpr int kSlotCols = (NPG == 4 || MODE == kCodeExact) ? 32 : 64;  // weight columns per slot
-  constexpr int kSlots = kL4TileCols / kSlotCols;                        // per tile
-  constexpr int kSlotsPerScale = kSlots / NPG;
-  constexpr int kXGroups = NC <= 8 ? 1 : NC / 8;                         // groups of eight columns of x
-  constexpr int kXBytes = kXGroups * 8 * kL4TileCols * 2;                // of a tile
-  constexpr int kN = NC <= 16 ? 16 : 32;
+  using C = Lin4Config<MODE, NPG, NC>;
+  constexpr int kSlotCols = C::kSlotCols, kSlots = kL4TileCols / kSlotCols;
+  constexpr int kScalesPerSlot = NPG >= kSlots ? NPG / kSlots : 1, kSlotsPerScale = NPG >= kSlots ? 1 : kSlots / NPG;
+  constexpr int kScaleCols = kSlotCols / kScalesPerSlot;  // columns of one product
+  constexpr int kLd = NC < 32 ? NC : 16;                  // products read at a time
   // fp32 accumulators, fp16 operands, both K-major, N / 8 and M / 16 in bits 17 and 24
-  constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(kN / 8) << 17) | ((128u / 16) << 24);
+  constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(C::kN / 8) << 17) | ((128u / 16) << 24);
 
   unsigned char* smem = reinterpret_cast<unsigned char*>(l4_smem);
-  unsigned char* xs = smem + (kIsCode ? kLutBytes : 0);
-  Lin4Bars& bars = *reinterpret_cast<Lin4Bars*>(xs + kL4Stages * kXBytes + 1024);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Lin4Bars& bars = *reinterpret_cast<Lin4Bars*>(smem + C::kBars);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2, row = threadIdx.x & 127;
   const int u0 = stream_begin(p.units, p.ctas, blockIdx.x), u1 = stream_begin(p.units, p.ctas, blockIdx.x + 1);
   pdl_trigger();
 
-  // the first tile of this thread's row is on its way while the tables are built
-  const int wg = warp >> 2, row = threadIdx.x & 127;
-  uint4 nw[4];
-  float ns[NPG];
-  uint32_t nz = 0;
-  auto load = [&](int rb, int step) {
-    const int rt = rb * kL4Groups + wg;
-    if (rt >= p.row_tiles) return;
-    const uint8_t* w = p.w + ((int64_t)rt * p.steps + step) * kL4TileBytes + row * 16;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) nw[c] = ldg_stream_u4(w + c * kL4TileRows * 16);
-    const int ss = (NPG == 1 && p.div > 1) ? step / p.div : step;
-    const int64_t e = (((int64_t)rt * p.scale_steps + ss) * kL4TileRows + row) * NPG;
-    if constexpr (NPG == 1) {
-      ns[0] = __ldg(p.s + e);
-      if (MODE == kIntZeros) nz = __ldg(p.z + e);
-    } else if constexpr (NPG == 2) {
-      const float2 v = __ldg(reinterpret_cast<const float2*>(p.s + e));
-      ns[0] = v.x;
-      ns[1] = v.y;
-      if (MODE == kIntZeros) nz = __ldg(reinterpret_cast<const unsigned short*>(p.z + e));
-    } else {
-      const float4 v = ldg_f4(p.s + e);
-      ns[0] = v.x;
-      ns[1] = v.y;
-      ns[2] = v.z;
-      ns[3] = v.w;
-      if (MODE == kIntZeros) nz = __ldg(reinterpret_cast<const uint32_t*>(p.z + e));
-    }
-  };
-  int rb = u0 / p.steps, step = u0 - rb * p.steps;
-  if (warp < 4 * kL4Groups && u0 < u1) load(rb, step);
-
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem)),
-                 "r"((uint32_t)kL4TmemCols)
+                 "r"(kL4Groups * kL4TmemGroup)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (threadIdx.x == 32) {
-    for (int i = 0; i < kL4Groups * 2; ++i) {
-      mbar_init(smem_u32(&bars.full[i / 2][i % 2]), 4);  // the group's four warps
-      mbar_init(smem_u32(&bars.done[i / 2][i % 2]), 1);
+    for (int g = 0; g < kL4Groups; ++g) {
+      for (int i = 0; i < C::kStages; ++i) mbar_init(smem_u32(&bars.w_full[g][i]), 1);
+      mbar_init(smem_u32(&bars.done[g]), 1);
     }
-    for (int i = 0; i < kL4Stages; ++i) {
+    for (int i = 0; i < kL4XStages; ++i) {
       mbar_init(smem_u32(&bars.x_full[i]), 1);
-      mbar_init(smem_u32(&bars.x_free[i]), 1);
+      mbar_init(smem_u32(&bars.x_free[i]), kL4Groups);
     }
     mbar_init_fence();
   }
-  if constexpr (kIsCode) {  // byte -> half2 table, one copy per lane (conflict-free); the second holds the remainders
+  __syncthreads();
+  int rb = u0 / p.steps, step = u0 - rb * p.steps;
+
+  // The warpgroup's issuing thread: a warp of another number in each, since warps of equal
+  // number share a scheduler.
+  const bool issuer = warp < 4 * kL4Groups && (warp & 3) == wg && lane == 0;
+  const uint64_t once = l2_evict_first_policy();
+  auto copy_tile = [&](int u) {  // tile, scales and zero points of unit u
+    const int at_rb = u / p.steps, at = u - at_rb * p.steps;
+    const int64_t rt = (int64_t)at_rb * kL4Groups + wg;
+    if (rt >= p.row_tiles) return;
+    const int st = (u - u0) % C::kStages;
+    const uint32_t bar = smem_u32(&bars.w_full[wg][st]);
+    const uint32_t dst = smem_u32(smem + C::kRing + (wg * C::kStages + st) * C::kStageBytes);
+    const int64_t e = (rt * p.scale_steps + ((NPG == 1 && p.div > 1) ? at / p.div : at)) * (kL4TileRows * NPG);
+    mbar_arrive_expect_tx(bar, C::kStageBytes);
+    bulk_g2s(dst, p.w + (rt * p.steps + at) * kL4TileBytes, kL4TileBytes, bar, once);
+    bulk_g2s(dst + kL4TileBytes, p.s + e, C::kScaleBytes, bar, once);
+    if (MODE == kIntZeros) bulk_g2s(dst + kL4TileBytes + C::kScaleBytes, p.z + e, kL4TileRows * NPG, bar, once);
+  };
+  if (issuer)
+    for (int u = u0; u < min(u1, u0 + C::kStages); ++u) copy_tile(u);
+
+  if constexpr (C::kIsCode) {  // byte -> half2 table, one copy per lane (conflict-free); the second holds the remainders
     const float cs = code_scale(p.code);
     uint4* lut4 = reinterpret_cast<uint4*>(smem);
     for (int i = threadIdx.x; i < 256 * 16; i += kL4Threads) {
@@ -384,149 +399,99 @@ __global__ void __launch_bounds__(kL4Threads, 2) lin4_kernel(const __grid_consta
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = bars.tmem;
-  // per group: two slots of weights (32 columns of fp16 pairs each), two products
-  constexpr uint32_t kA = 32, kD = 32, kPerGroup = 128;
 
+  // Every wait is bounded.  One that runs out makes its thread go on without waiting, and
+  // leaves NaN in the warpgroup's partials.
   if (warp == 4 * kL4Groups) {
-    // ---- copies of x and MMAs: one thread; every wait is bounded, and one that runs out
-    // ends the issue (the warpgroups' own waits then run out, and leave NaN)
-    if (lane == 0) {
+    if (lane == 0) {  // ---- copies of x
       pdl_wait();
       fence_proxy_async_global();
       const uint64_t keep = l2_evict_last_policy();
-      auto copy = [&](int u) {  // the tile of x of unit u
-        const int st = (u - u0) % kL4Stages;
-        const uint32_t bar = smem_u32(&bars.x_full[st]);
-        mbar_arrive_expect_tx(bar, kXBytes);
-        bulk_g2s(smem_u32(xs + st * kXBytes), reinterpret_cast<const unsigned char*>(p.xh) + (int64_t)(u % p.steps) * kXBytes,
-                 kXBytes, bar, keep);
-      };
-      for (int u = u0; u < min(u1, u0 + kL4Stages); ++u) copy(u);
-      int copied = min(u1, u0 + kL4Stages), landed = u0, issued = u0;
       bool ok = true;
-      int n[kL4Groups] = {0, 0}, scales[kL4Groups] = {0, 0};  // slots and scale granules issued so far
-      for (int u = u0; u < u1 && ok; ++u) {
-        const int st = (u - u0) % kL4Stages;
-        ok = mbar_wait(smem_u32(&bars.x_full[st]), ((u - u0) / kL4Stages) & 1, p.wait_limit);
-        landed = u + (ok ? 1 : 0);
-        const uint32_t x0 = smem_u32(xs + st * kXBytes);
-        for (int t = 0; t < kSlots && ok; ++t) {
-          for (int g = 0; g < kL4Groups && ok; ++g) {
-            if (rb * kL4Groups + g >= p.row_tiles) continue;
-            const int slot = n[g] & 1;
-            ok = mbar_wait(smem_u32(&bars.full[g][slot]), (n[g] >> 1) & 1, p.wait_limit);
-            if (!ok) break;
-            tmem_fence_after();
-            const uint32_t d = tmem + g * kPerGroup + 2 * kA + (scales[g] & 1) * kD;
-            const uint32_t a = tmem + g * kPerGroup + slot * kA;
-#pragma unroll
-            for (int half = 0; half < (MODE == kCodeExact ? 2 : 1); ++half) {
-#pragma unroll
-              for (int k = 0; k < kSlotCols / 16; ++k) {
-                // K-major without swizzle: 8 columns of the weight are kXGroups x 128 bytes on, 8 columns of
-                // x 128 bytes (with one group the upper eight of N = 16 are never read back)
-                const uint32_t at = x0 + (uint32_t)(t * (kSlotCols / 8) + 2 * k) * (kXGroups * 128u);
-                const uint64_t desc = (uint64_t)((at >> 4) & 0x3fff) | ((uint64_t)(kXGroups * 128 / 16) << 16) |
-                                      ((uint64_t)(128 / 16) << 32) | (1ull << 46);
-                mma_f16_ts(d, a + half * (kSlotCols / 2) + k * 8, desc, kIdesc,
-                           !(t % kSlotsPerScale == 0 && half == 0 && k == 0));
-              }
-            }
-            mma_commit(smem_u32(&bars.done[g][slot]));
-            ++n[g];
-            if (t % kSlotsPerScale == kSlotsPerScale - 1) ++scales[g];
-          }
-        }
-        mma_commit(smem_u32(&bars.x_free[st]));
-        issued = u + 1;
-        if (++step == p.steps) {
-          step = 0;
-          ++rb;
-        }
-        // the tile before this one is read: its place takes the next copy
-        if (ok && u > u0 && copied < u1) {
-          const int pt = (u - 1 - u0) % kL4Stages;
-          ok = mbar_wait(smem_u32(&bars.x_free[pt]), ((u - 1 - u0) / kL4Stages) & 1, p.wait_limit);
-          if (ok) copy(copied++);
-        }
+      int copied = 0;
+      for (int u = u0; u < u1; ++u) {
+        const int i = u - u0, st = i % kL4XStages;
+        if (i >= kL4XStages) ok = mbar_wait(smem_u32(&bars.x_free[st]), (i / kL4XStages - 1) & 1, p.wait_limit);
+        if (!ok) break;
+        const uint32_t bar = smem_u32(&bars.x_full[st]);
+        mbar_arrive_expect_tx(bar, C::kXBytes);
+        bulk_g2s(smem_u32(smem + C::kX + st * C::kXBytes),
+                 reinterpret_cast<const unsigned char*>(p.xh) + (int64_t)step * C::kXBytes, C::kXBytes, bar, keep);
+        copied = i + 1;
+        if (++step == p.steps) step = 0;
       }
-      // nothing may arrive in shared memory that is gone: the last commits, and after a failure copies
-      for (int u = max(u0, issued - kL4Stages); u < issued; ++u)
-        mbar_wait(smem_u32(&bars.x_free[(u - u0) % kL4Stages]), ((u - u0) / kL4Stages) & 1);
-      for (int u = landed; u < copied; ++u)
-        mbar_wait(smem_u32(&bars.x_full[(u - u0) % kL4Stages]), ((u - u0) / kL4Stages) & 1);
+      // nothing may arrive in shared memory that is gone: the last copies and commits
+      for (int i = max(0, copied - kL4XStages); i < copied; ++i) {
+        mbar_wait(smem_u32(&bars.x_full[i % kL4XStages]), (i / kL4XStages) & 1);
+        if (ok) ok = mbar_wait(smem_u32(&bars.x_free[i % kL4XStages]), (i / kL4XStages) & 1, p.wait_limit);
+      }
     }
     __syncwarp();
   } else {
-    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of tensor memory
-    const uint32_t a0 = tmem + lanes + wg * kPerGroup, d0 = a0 + 2 * kA;
+    const uint32_t a0 = tmem + wg * kL4TmemGroup;                    // lane 0: the MMAs' address
+    const uint32_t mine = a0 + ((uint32_t)(warp & 3) << 21);         // this warp's 32 lanes
     const uint32_t lanebase = (uint32_t)lane * 4u;
     float acc[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) acc[c] = 0.f;
     bool ok = true;
-    int n = 0, scales = 0;  // slots stored and scale granules finished
-    float last_scale = 0.f;
-    int open = -1;          // row block of the sums, and of the slot that is not added yet
-    auto add_scaled = [&](float s) {  // the products of the granule that is done, scaled
-      const uint32_t d = d0 + (scales & 1) * kD;
-#pragma unroll
-      for (int c0 = 0; c0 < NC; c0 += 8) {
-        uint32_t r[8];
-        tmem_ld<(NC < 8 ? NC : 8)>(d + c0, r);
-        tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < (NC < 8 ? NC : 8); ++c) acc[c0 + c] = fmaf(s, __uint_as_float(r[c]), acc[c0 + c]);
-      }
-      ++scales;
-    };
-    auto wait_slot = [&](int i) {  // the MMAs of slot number i are done
-      if (ok) ok = mbar_wait(smem_u32(&bars.done[wg][i & 1]), (i >> 1) & 1, p.wait_limit);
-      __syncwarp();
-      tmem_fence_after();
-    };
-    auto flush = [&]() {
-      const int seg = (int)blockIdx.x - stream_owner(p.units, p.ctas, open * p.steps);
-      float* dst = p.part + ((int64_t)(open * p.max_segs + seg) * p.cols) * kL4BlockRows + wg * kL4TileRows + row;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        if (c < p.cols) dst[(int64_t)c * kL4BlockRows] = ok ? acc[c] : __int_as_float(0x7fc00000);
-        acc[c] = 0.f;
-      }
-    };
+    int slots = 0;  // MMA rounds so far
+    int copied = min(u1, u0 + C::kStages);
     for (int u = u0; u < u1; ++u) {
-      if (rb * kL4Groups + wg >= p.row_tiles) break;  // only in the last row block
-      uint4 w[4];
-      float s[NPG];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) w[c] = nw[c];
-#pragma unroll
-      for (int c = 0; c < NPG; ++c) s[c] = ns[c];
-      const uint32_t z = nz;
-      int nrb = rb, nstep = step + 1;
-      if (nstep == p.steps) {
-        nstep = 0;
-        ++nrb;
+      const int i = u - u0, st = i % C::kStages, xst = i % kL4XStages;
+      const bool last = step + 1 == p.steps || u + 1 == u1;
+      if (rb * kL4Groups + wg >= p.row_tiles) {  // no rows here (in the last row block): only x goes by
+        if (issuer) {
+          if (ok) ok = mbar_wait(smem_u32(&bars.x_full[xst]), (i / kL4XStages) & 1, p.wait_limit);
+          mbar_arrive(smem_u32(&bars.x_free[xst]));
+        }
+        continue;
       }
-      if (u + 1 < u1) load(nrb, nstep);
+      const unsigned char* stage = smem + C::kRing + (wg * C::kStages + st) * C::kStageBytes;
+      if (ok) ok = mbar_wait(smem_u32(&bars.w_full[wg][st]), (i / C::kStages) & 1, p.wait_limit);
+      float s[NPG];
+      uint32_t z = 0;
+      {
+        const uint32_t sa = smem_u32(stage + kL4TileBytes) + row * NPG * 4;
+        if constexpr (NPG == 1) {
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s[0]) : "r"(sa));
+        } else if constexpr (NPG == 2) {
+          asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(s[0]), "=f"(s[1]) : "r"(sa));
+        } else {
+          const float4 v = lds_f4(sa);
+          s[0] = v.x;
+          s[1] = v.y;
+          s[2] = v.z;
+          s[3] = v.w;
+        }
+        if (MODE == kIntZeros) {
+          const unsigned char* za = stage + kL4TileBytes + C::kScaleBytes + row * NPG;
+          if constexpr (NPG == 1) {
+            z = *za;
+          } else if constexpr (NPG == 2) {
+            z = *reinterpret_cast<const unsigned short*>(za);
+          } else {
+            z = *reinterpret_cast<const uint32_t*>(za);
+          }
+        }
+      }
 #pragma unroll
       for (int t = 0; t < kSlots; ++t) {
-        const uint32_t a = a0 + (n & 1) * kA;
-        uint32_t za = 0x64086408u, zb = 0xd480d480u;  // 1024 + 8, -(64 + 8)
-        if constexpr (MODE == kIntZeros) {
-          za = (0x6400u | ((z >> (8 * (t / kSlotsPerScale))) & 255u)) * 0x10001u;
-          zb = hsub2_u32(0x63806380u, za);  // 960 - (1024 + z)
-        }
 #pragma unroll
         for (int c = 0; c < kSlotCols / 32; ++c) {
-          const uint4 q = w[t * (kSlotCols / 32) + c];
+          const uint4 q = lds_u4(smem_u32(stage) + ((t * (kSlotCols / 32) + c) * kL4TileRows + row) * 16);
           const uint32_t word[4] = {q.x, q.y, q.z, q.w};
+          uint32_t za = 0x64086408u, zb = 0xd480d480u;  // 1024 + 8, -(64 + 8)
+          if constexpr (MODE == kIntZeros) {
+            za = (0x6400u | ((z >> (8 * ((t * kSlotCols + c * 32) * NPG / kL4TileCols))) & 255u)) * 0x10001u;
+            zb = hsub2_u32(0x63806380u, za);  // 960 - (1024 + z)
+          }
 #pragma unroll
           for (int half = 0; half < (MODE == kCodeExact ? 2 : 1); ++half) {
             uint32_t r[16];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              if constexpr (kIsCode) {
+              if constexpr (C::kIsCode) {
 #pragma unroll
                 for (int b = 0; b < 4; ++b) r[4 * j + b] = lut_lookup_rt(l4_smem, word[j], lanebase, b, half);
               } else {
@@ -536,41 +501,81 @@ __global__ void __launch_bounds__(kL4Threads, 2) lin4_kernel(const __grid_consta
                 r[4 * j + 3] = int_pair<3>(word[j], za, zb);
               }
             }
-            tmem_st16(a + half * (kSlotCols / 2) + c * 16, r);
+            tmem_st16(mine + half * (kSlotCols / 2) + c * 16, r);
           }
         }
         tmem_wait_st();
         tmem_fence_before();
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
+        if (issuer) {
+          if (t == kSlots - 1 && u + C::kStages < u1 && ok) {  // the tile is read: its place takes the next copy
+            fence_proxy_async_smem();
+            copy_tile(u + C::kStages);
+            copied = u + C::kStages + 1;
+          }
+          if (t == 0 && ok) ok = mbar_wait(smem_u32(&bars.x_full[xst]), (i / kL4XStages) & 1, p.wait_limit);
+          tmem_fence_after();
+          const uint32_t x0 = smem_u32(smem + C::kX + xst * C::kXBytes) + t * (kSlotCols / 8) * (C::kXGroups * 128);
+          // K-major without swizzle: 8 columns of the weight are kXGroups x 128 bytes on, 8 columns
+          // of x 128 bytes (with one group the upper eight of N = 16 are never read back)
+          const uint64_t desc = (uint64_t)((x0 >> 4) & 0x3fff) | ((uint64_t)(C::kXGroups * 128 / 16) << 16) |
+                                ((uint64_t)(128 / 16) << 32) | (1ull << 46);
+#pragma unroll
+          for (int k = 0; k < kSlotCols / 16; ++k) {
+            const uint32_t d = a0 + kL4TmemA + (16 * k / kScaleCols) * C::kN;
+#pragma unroll
+            for (int half = 0; half < (MODE == kCodeExact ? 2 : 1); ++half)
+              mma_f16_ts(d, a0 + half * (kSlotCols / 2) + k * 8, desc + (uint64_t)(k * 2 * C::kXGroups * 128 / 16), kIdesc,
+                         !(t % kSlotsPerScale == 0 && half == 0 && 16 * k % kScaleCols == 0));
+          }
+          mma_commit(smem_u32(&bars.done[wg]));
+          if (t == kSlots - 1) mma_commit(smem_u32(&bars.x_free[xst]));
+        }
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bars.full[wg][n & 1]));
-        // the slot before this one: its products are done, or soon
-        if (n > 0) {
-          wait_slot(n - 1);
-          if (t == 0) {
-            add_scaled(last_scale);
-            if (open != rb) flush();
-          } else if (t % kSlotsPerScale == 0) {
-            add_scaled(s[t / kSlotsPerScale - 1]);
+        if (ok) ok = mbar_wait(smem_u32(&bars.done[wg]), slots & 1, p.wait_limit);
+        __syncwarp();
+        tmem_fence_after();
+        ++slots;
+        if (t % kSlotsPerScale == kSlotsPerScale - 1) {
+#pragma unroll
+          for (int g = 0; g < kScalesPerSlot; ++g) {
+            const float sc = s[t * NPG / kSlots + g];
+#pragma unroll
+            for (int c0 = 0; c0 < NC; c0 += kLd) {
+              uint32_t r[kLd];
+              tmem_ld<kLd>(mine + kL4TmemA + g * C::kN + c0, r);
+              tmem_wait_ld();
+#pragma unroll
+              for (int c = 0; c < kLd; ++c) acc[c0 + c] = fmaf(sc, __uint_as_float(r[c]), acc[c0 + c]);
+            }
           }
         }
-        if (t == 0) open = rb;
-        ++n;
       }
-      last_scale = s[NPG - 1];
-      rb = nrb;
-      step = nstep;
+      if (last) {
+        const int seg = (int)blockIdx.x - stream_owner(p.units, p.ctas, rb * p.steps);
+        float* dst = p.part + ((int64_t)(rb * p.max_segs + seg) * p.cols) * kL4BlockRows + wg * kL4TileRows + row;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          if (c < p.cols) dst[(int64_t)c * kL4BlockRows] = ok ? acc[c] : __int_as_float(0x7fc00000);
+          acc[c] = 0.f;
+        }
+      }
+      if (++step == p.steps) {
+        step = 0;
+        ++rb;
+      }
     }
-    if (n > 0) {
-      wait_slot(n - 1);
-      add_scaled(last_scale);
-      flush();
-    }
+    if (issuer && !ok)  // after a failure: no copy may land in shared memory that is gone
+      for (int u = max(u0, copied - C::kStages); u < copied; ++u)
+        if (u / p.steps * kL4Groups + wg < p.row_tiles)
+          mbar_wait(smem_u32(&bars.w_full[wg][(u - u0) % C::kStages]), ((u - u0) / C::kStages) & 1);
+    __syncwarp();
     tmem_fence_before();
   }
   __syncthreads();
   tmem_fence_after();
   if (warp == 0)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kL4TmemCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kL4Groups * kL4TmemGroup) : "memory");
 }
 
 __global__ void __launch_bounds__(kL4BlockRows) lin4_finalize_kernel(const float* part, const float* scale, int units,
@@ -605,7 +610,7 @@ Lin4Plan lin4_plan(const Lin4Shape& sh, int rows, int x_dtype, int sm_count) {
   Lin4Plan pl;
   pl.cols = x_dtype == NSM_F32 ? 2 * rows : rows;
   pl.units = sh.row_blocks * sh.steps;
-  pl.ctas = std::max(1, std::min({2 * sm_count, pl.units, sh.row_blocks * (kL4MaxSegs - 2)}));
+  pl.ctas = std::max(1, std::min({sm_count, pl.units, sh.row_blocks * (kL4MaxSegs - 2)}));
   const int least = pl.units / pl.ctas;  // units of the shortest run
   pl.max_segs = (sh.steps - 1 + least - 1) / least + 1;
   pl.col_groups = pl.cols <= 8 ? 1 : pl.cols <= 16 ? 2 : 4;
@@ -622,15 +627,22 @@ bool lin4_size_ok(int N, int K, int group) {
 
 int lin4_max_rows(int x_dtype) { return x_dtype == NSM_F32 ? kL4MaxCols / 2 : kL4MaxCols; }
 
-using Lin4Fn = void (*)(Lin4Params);
+struct Lin4Fn {
+  void (*fn)(Lin4Params);
+  int smem;
+};
 
 // Columns of x that the sums hold: the next of 1, 2, 4, 8, 16, 32.
 int lin4_col_case(int cols) { return cols <= 1 ? 0 : cols <= 2 ? 1 : cols <= 4 ? 2 : cols <= 8 ? 3 : cols <= 16 ? 4 : 5; }
 
+template <int MODE, int NPG, int NC>
+constexpr Lin4Fn lin4_fn() {
+  return {lin4_kernel<MODE, NPG, NC>, Lin4Config<MODE, NPG, NC>::kSmem};
+}
 template <int MODE, int NPG>
 Lin4Fn lin4_pick_cols(int c) {
-  constexpr Lin4Fn fns[6] = {lin4_kernel<MODE, NPG, 1>, lin4_kernel<MODE, NPG, 2>,  lin4_kernel<MODE, NPG, 4>,
-                             lin4_kernel<MODE, NPG, 8>, lin4_kernel<MODE, NPG, 16>, lin4_kernel<MODE, NPG, 32>};
+  constexpr Lin4Fn fns[6] = {lin4_fn<MODE, NPG, 1>(), lin4_fn<MODE, NPG, 2>(),  lin4_fn<MODE, NPG, 4>(),
+                             lin4_fn<MODE, NPG, 8>(), lin4_fn<MODE, NPG, 16>(), lin4_fn<MODE, NPG, 32>()};
   return fns[c];
 }
 template <int MODE>
@@ -738,14 +750,12 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
   // half an fp16 rounding), which halves the table reads that bound the kernel
   const int mode = w->code ? (out_dtype == NSM_F32 ? kCodeExact : kCode) : (w->zeros ? kIntZeros : kInt);
   const int cc = lin4_col_case(pl.cols);
-  Lin4Fn fn = mode == kCode        ? lin4_pick_npg<kCode>(sh.npg, cc)
-              : mode == kCodeExact ? lin4_pick_npg<kCodeExact>(sh.npg, cc)
-              : mode == kInt       ? lin4_pick_npg<kInt>(sh.npg, cc)
-                                   : lin4_pick_npg<kIntZeros>(sh.npg, cc);
-  const size_t smem = (w->code ? (size_t)kLutBytes : 0) + (size_t)kL4Stages * pl.col_groups * 8 * kL4TileCols * 2 + 1024 +
-                      sizeof(Lin4Bars);
+  const Lin4Fn f = mode == kCode        ? lin4_pick_npg<kCode>(sh.npg, cc)
+                   : mode == kCodeExact ? lin4_pick_npg<kCodeExact>(sh.npg, cc)
+                   : mode == kInt       ? lin4_pick_npg<kInt>(sh.npg, cc)
+                                        : lin4_pick_npg<kIntZeros>(sh.npg, cc);
   static SmemOnce once[4][3][6];
-  NSM_CHECK_CUDA(once[mode][sh.npg / 2][cc].set(fn, (int)smem, di.device));
+  NSM_CHECK_CUDA(once[mode][sh.npg / 2][cc].set(f.fn, f.smem, di.device));
   const int slices = std::max(1, std::min(8, sh.kp / 2048));
   lin4_prep_kernel<<<dim3(slices, rows), 256, 0, s>>>(x, x_dtype, x_row_stride, sh.K, sh.kp, rows, pl.col_groups, w->code,
                                                       xh, scale);
@@ -766,7 +776,7 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
   p.ctas = pl.ctas;
   p.max_segs = pl.max_segs;
   p.wait_limit = copy_wait_spins();
-  NSM_CHECK_CUDA(launch_pdl(fn, dim3(pl.ctas), dim3(kL4Threads), smem, s, p));
+  NSM_CHECK_CUDA(launch_pdl(f.fn, dim3(pl.ctas), dim3(kL4Threads), (size_t)f.smem, s, p));
   NSM_CHECK_CUDA(launch_pdl(lin4_finalize_kernel, dim3(sh.row_blocks, rows), dim3(kL4BlockRows), 0, s,
                             (const float*)part, (const float*)scale, pl.units, pl.ctas, sh.steps, pl.max_segs, pl.cols,
                             (int)rows, sh.N, w->bias, (int)w->bias_dtype, out, (int)out_dtype, out_row_stride));
