@@ -22,11 +22,11 @@
 //     one per CTA, so no CTA finishes late.  Bulk copies bring each warpgroup's tile and
 //     scales into its own ring, and x into a ring that all share.  A warpgroup turns its
 //     tile into fp16 (a byte -> half2 table for codebooks, mask and subtract for
-//     integers: both exact but for the codebook's rounding), stores it to tensor
-//     memory, and one of its threads multiplies it with x (tcgen05.mma, M = 128 rows, N =
-//     the columns of x, fp32 accumulation); then it adds scale * product to its
-//     fp32 sums in registers.  The four warpgroups are in different phases of this, so one's round
-//     trip is another's arithmetic.  With weights as the M operand in tensor memory x never
+//     integers: both exact but for the codebook's rounding) and stores it to tensor
+//     memory, 64 columns at a time in two slots; a warp of its own multiplies them with x
+//     (tcgen05.mma, M = 128 rows, N = the columns of x, fp32 accumulation) while the
+//     warpgroup works on the next slot, and then the warpgroup adds scale * product to
+//     its fp32 sums in registers.  With weights as the M operand in tensor memory x never
 //     passes through registers: one row of x or 32 cost the threads the same but for the sums.
 //     Each CTA leaves one fp32 partial per row block that it touched;
 //  3. lin4_finalize_kernel: the partials of a row block in CTA order (the same
@@ -41,7 +41,7 @@ namespace nsm {
 namespace {
 
 constexpr int kL4Groups = 4;                          // warpgroups of a CTA
-constexpr int kL4Threads = kL4Groups * 128 + 32;      // + the warp that copies x
+constexpr int kL4Threads = kL4Groups * 160 + 32;      // each with a warp that issues its copies and MMAs; + copies of x
 constexpr int kL4TileRows = 128;
 constexpr int kL4TileCols = 128;
 constexpr int kL4TileBytes = kL4TileRows * kL4TileCols / 2;
@@ -49,7 +49,8 @@ constexpr int kL4BlockRows = kL4TileRows * kL4Groups;  // rows of a unit
 constexpr int kL4MaxCols = 32;                        // fp16 columns of x in one call
 constexpr int kL4MaxSegs = 32;                        // CTAs that share one row block
 constexpr int kL4XStages = 4;                         // x tiles in flight
-// tensor memory: per warpgroup 64 columns of weights (fp16 pairs) and 64 of products
+// tensor memory: per warpgroup two slots of 32 columns of weights (fp16 pairs) and 64 columns
+// of products
 constexpr uint32_t kL4TmemA = 64, kL4TmemGroup = 128;
 
 // Kinds of weights: codebook rounded to fp16; codebook as fp16 value +
@@ -301,26 +302,26 @@ struct Lin4Config {
   static constexpr int kXGroups = NC <= 8 ? 1 : NC / 8;                    // groups of eight columns of x
   static constexpr int kXBytes = kXGroups * 8 * kL4TileCols * 2;           // of a tile
   static constexpr int kN = NC <= 16 ? 16 : 32;                            // of the MMA
-  // weight columns stored before the MMAs: what fits 64 + 64 columns of tensor memory
-  static constexpr int kSlotCols = (MODE == kCodeExact || (NPG == 4 && kN == 32)) ? 64 : 128;
+  static constexpr int kSlotCols = MODE == kCodeExact ? 32 : 64;           // weight columns of a slot
   static constexpr int kScaleBytes = kL4TileRows * NPG * 4;
   static constexpr int kStageBytes = kL4TileBytes + kScaleBytes + (MODE == kIntZeros ? kL4TileRows * NPG : 0);
   static constexpr int kStages = kIsCode ? 3 : 4;                          // weight tiles in flight per warpgroup
   static constexpr int kLut = kIsCode ? kLutBytes : 0;
   static constexpr int kRing = kLut, kX = kRing + kL4Groups * kStages * kStageBytes;
   static constexpr int kBars = kX + kL4XStages * kXBytes + 1024;  // the last tile of x is read 128 bytes over
-  static constexpr int kSmem = kBars + 256;
+  static constexpr int kSmem = kBars + 320;
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
 struct Lin4Bars {
   unsigned long long w_full[kL4Groups][4];  // a tile of weights and its scales are in shared memory
-  unsigned long long done[kL4Groups];       // the MMAs of a slot are done
+  unsigned long long full[kL4Groups];       // a slot of weights is in tensor memory
+  unsigned long long done[kL4Groups];       // its MMAs are done
   unsigned long long x_full[kL4XStages];    // a tile of x is in shared memory
   unsigned long long x_free[kL4XStages];    // all warpgroups' MMAs that read it are done
   uint32_t tmem;
 };
-static_assert(sizeof(Lin4Bars) <= 256, "barriers");
+static_assert(sizeof(Lin4Bars) <= 320, "barriers");
 
 template <int MODE, int NPG, int NC>
 __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_constant__ Lin4Params p) {
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
 
   unsigned char* smem = reinterpret_cast<unsigned char*>(l4_smem);
   Lin4Bars& bars = *reinterpret_cast<Lin4Bars*>(smem + C::kBars);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2, row = threadIdx.x & 127;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = threadIdx.x & 127;
   const int u0 = stream_begin(p.units, p.ctas, blockIdx.x), u1 = stream_begin(p.units, p.ctas, blockIdx.x + 1);
   pdl_trigger();
 
@@ -348,6 +349,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
   if (threadIdx.x == 32) {
     for (int g = 0; g < kL4Groups; ++g) {
       for (int i = 0; i < C::kStages; ++i) mbar_init(smem_u32(&bars.w_full[g][i]), 1);
+      mbar_init(smem_u32(&bars.full[g]), 4);  // the group's four warps
       mbar_init(smem_u32(&bars.done[g]), 1);
     }
     for (int i = 0; i < kL4XStages; ++i) {
@@ -359,25 +361,33 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
   __syncthreads();
   int rb = u0 / p.steps, step = u0 - rb * p.steps;
 
-  // The warpgroup's issuing thread: a warp of another number in each, since warps of equal
-  // number share a scheduler.
-  const bool issuer = warp < 4 * kL4Groups && (warp & 3) == wg && lane == 0;
+  // warps 0-15: the warpgroups; 16-19: one that issues for each; 20: copies of x
+  const int my_warp = __shfl_sync(0xffffffffu, warp, 0);
+  const bool issuing = my_warp >= 4 * kL4Groups && my_warp < 5 * kL4Groups;
+  const int wg = issuing ? my_warp - 4 * kL4Groups : my_warp >> 2;
   const uint64_t once = l2_evict_first_policy();
-  auto copy_tile = [&](int u) {  // tile, scales and zero points of unit u
-    const int at_rb = u / p.steps, at = u - at_rb * p.steps;
-    const int64_t rt = (int64_t)at_rb * kL4Groups + wg;
-    if (rt >= p.row_tiles) return;
-    const int st = (u - u0) % C::kStages;
-    const uint32_t bar = smem_u32(&bars.w_full[wg][st]);
-    const uint32_t dst = smem_u32(smem + C::kRing + (wg * C::kStages + st) * C::kStageBytes);
-    const int64_t e = (rt * p.scale_steps + ((NPG == 1 && p.div > 1) ? at / p.div : at)) * (kL4TileRows * NPG);
-    mbar_arrive_expect_tx(bar, C::kStageBytes);
-    bulk_g2s(dst, p.w + (rt * p.steps + at) * kL4TileBytes, kL4TileBytes, bar, once);
-    bulk_g2s(dst + kL4TileBytes, p.s + e, C::kScaleBytes, bar, once);
-    if (MODE == kIntZeros) bulk_g2s(dst + kL4TileBytes + C::kScaleBytes, p.z + e, kL4TileRows * NPG, bar, once);
+  int copy_rb = rb, copy_step = step, copied = 0;  // the unit to copy next, units copied
+  auto copy_tile = [&]() {  // one lane: tile, scales and zero points of the next unit
+    const int64_t rt = (int64_t)copy_rb * kL4Groups + wg;
+    if (rt < p.row_tiles) {
+      const int st = copied % C::kStages;
+      const uint32_t bar = smem_u32(&bars.w_full[wg][st]);
+      const uint32_t dst = smem_u32(smem + C::kRing + (wg * C::kStages + st) * C::kStageBytes);
+      const int64_t e =
+          (rt * p.scale_steps + ((NPG == 1 && p.div > 1) ? copy_step / p.div : copy_step)) * (kL4TileRows * NPG);
+      mbar_arrive_expect_tx(bar, C::kStageBytes);
+      bulk_g2s(dst, p.w + (rt * p.steps + copy_step) * kL4TileBytes, kL4TileBytes, bar, once);
+      bulk_g2s(dst + kL4TileBytes, p.s + e, C::kScaleBytes, bar, once);
+      if (MODE == kIntZeros) bulk_g2s(dst + kL4TileBytes + C::kScaleBytes, p.z + e, kL4TileRows * NPG, bar, once);
+    }
+    ++copied;
+    if (++copy_step == p.steps) {
+      copy_step = 0;
+      ++copy_rb;
+    }
   };
-  if (issuer)
-    for (int u = u0; u < min(u1, u0 + C::kStages); ++u) copy_tile(u);
+  if (issuing && lane == 0)
+    for (int u = u0; u < min(u1, u0 + C::kStages); ++u) copy_tile();
 
   if constexpr (C::kIsCode) {  // byte -> half2 table, one copy per lane (conflict-free); the second holds the remainders
     const float cs = code_scale(p.code);
@@ -402,13 +412,12 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
 
   // Every wait is bounded.  One that runs out makes its thread go on without waiting, and
   // leaves NaN in the warpgroup's partials.
-  if (warp == 4 * kL4Groups) {
+  if (my_warp == 5 * kL4Groups) {
     if (lane == 0) {  // ---- copies of x
       pdl_wait();
       fence_proxy_async_global();
       const uint64_t keep = l2_evict_last_policy();
       bool ok = true;
-      int copied = 0;
       for (int u = u0; u < u1; ++u) {
         const int i = u - u0, st = i % kL4XStages;
         if (i >= kL4XStages) ok = mbar_wait(smem_u32(&bars.x_free[st]), (i / kL4XStages - 1) & 1, p.wait_limit);
@@ -427,59 +436,136 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
       }
     }
     __syncwarp();
+  } else if (issuing) {
+    // ---- MMAs and copies of the warpgroup's tiles
+    const uint32_t a0 = tmem + wg * kL4TmemGroup;
+    const uint32_t full_bar = smem_u32(&bars.full[wg]), done_bar = smem_u32(&bars.done[wg]);
+    bool ok = true;
+    int slots = 0, xst = 0, x_phase = 0;
+    for (int u = u0; u < u1; ++u) {
+      const uint32_t xfree = smem_u32(&bars.x_free[xst]);
+      if (ok) ok = mbar_wait(smem_u32(&bars.x_full[xst]), x_phase, p.wait_limit);
+      if (rb * kL4Groups + wg < p.row_tiles) {
+        const uint32_t x0 = smem_u32(smem + C::kX + xst * C::kXBytes);
+        // K-major without swizzle: 8 columns of the weight are kXGroups x 128 bytes on, 8 columns of
+        // x 128 bytes (with one group the upper eight of N = 16 are never read back)
+        const uint64_t desc0 = (uint64_t)((x0 >> 4) & 0x3fff) | ((uint64_t)(C::kXGroups * 128 / 16) << 16) |
+                               ((uint64_t)(128 / 16) << 32) | (1ull << 46);
+#pragma unroll
+        for (int t = 0; t < kSlots; ++t) {
+          if (ok) ok = mbar_wait(full_bar, slots & 1, p.wait_limit);
+          __syncwarp();
+          tmem_fence_after();
+          const uint32_t a = a0 + (uint32_t)(slots & 1) * (kL4TmemA / 2);
+          if (lane == 0) {
+#pragma unroll
+            for (int k = 0; k < kSlotCols / 16; ++k) {
+              const uint32_t d = a0 + kL4TmemA + (16 * k / kScaleCols) * C::kN;
+#pragma unroll
+              for (int half = 0; half < (MODE == kCodeExact ? 2 : 1); ++half)
+                mma_f16_ts(d, a + half * (kSlotCols / 2) + k * 8,
+                           desc0 + (uint64_t)((t * (kSlotCols / 8) + 2 * k) * C::kXGroups * 128 / 16), kIdesc,
+                           !(t % kSlotsPerScale == 0 && half == 0 && 16 * k % kScaleCols == 0));
+            }
+            mma_commit(done_bar);
+            if (t == kSlots - 1) {
+              mma_commit(xfree);
+              if (copied < u1 - u0 && ok) {  // the tile is read: its place takes the next copy
+                fence_proxy_async_smem();
+                copy_tile();
+              }
+            }
+          }
+          __syncwarp();
+          ++slots;
+        }
+      } else if (lane == 0) {  // no rows here (in the last row block): only x goes by
+        mbar_arrive(xfree);
+      }
+      if (++xst == kL4XStages) {
+        xst = 0;
+        x_phase ^= 1;
+      }
+      if (++step == p.steps) {
+        step = 0;
+        ++rb;
+      }
+    }
+    if (lane == 0 && !ok)  // after a failure: no copy may land in shared memory that is gone
+      for (int i = max(0, copied - C::kStages); i < copied; ++i)
+        if ((u0 + i) / p.steps * kL4Groups + wg < p.row_tiles)
+          mbar_wait(smem_u32(&bars.w_full[wg][i % C::kStages]), (i / C::kStages) & 1);
+    __syncwarp();
   } else {
-    const uint32_t a0 = tmem + wg * kL4TmemGroup;                    // lane 0: the MMAs' address
-    const uint32_t mine = a0 + ((uint32_t)(warp & 3) << 21);         // this warp's 32 lanes
+    // ---- the warpgroup: 4 bits -> fp16 -> tensor memory, and the sums
+    const uint32_t mine = tmem + wg * kL4TmemGroup + ((uint32_t)(my_warp & 3) << 21);  // this warp's 32 lanes
     const uint32_t lanebase = (uint32_t)lane * 4u;
+    const uint32_t done_bar = smem_u32(&bars.done[wg]);
     float acc[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) acc[c] = 0.f;
     bool ok = true;
-    int slots = 0;  // MMA rounds so far
-    int copied = min(u1, u0 + C::kStages);
-    for (int u = u0; u < u1; ++u) {
-      const int i = u - u0, st = i % C::kStages, xst = i % kL4XStages;
-      const bool last = step + 1 == p.steps || u + 1 == u1;
-      if (rb * kL4Groups + wg >= p.row_tiles) {  // no rows here (in the last row block): only x goes by
-        if (issuer) {
-          if (ok) ok = mbar_wait(smem_u32(&bars.x_full[xst]), (i / kL4XStages) & 1, p.wait_limit);
-          mbar_arrive(smem_u32(&bars.x_free[xst]));
+    int slots = 0;       // MMA rounds so far
+    float last_s[kScalesPerSlot];  // scales of the last round's products
+    int open = -1;       // row block of the sums and of the last round
+    // waits for the last round; its products, scaled, join the sums if they are whole
+    auto add_last = [&](bool whole, const float* s) {
+      if (ok) ok = mbar_wait(done_bar, (slots - 1) & 1, p.wait_limit);
+      __syncwarp();
+      tmem_fence_after();
+      if (whole) {
+#pragma unroll
+        for (int g = 0; g < kScalesPerSlot; ++g) {
+#pragma unroll
+          for (int c0 = 0; c0 < NC; c0 += kLd) {
+            uint32_t r[kLd];
+            tmem_ld<kLd>(mine + kL4TmemA + g * C::kN + c0, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < kLd; ++c) acc[c0 + c] = fmaf(s[g], __uint_as_float(r[c]), acc[c0 + c]);
+          }
         }
-        continue;
       }
-      const unsigned char* stage = smem + C::kRing + (wg * C::kStages + st) * C::kStageBytes;
-      if (ok) ok = mbar_wait(smem_u32(&bars.w_full[wg][st]), (i / C::kStages) & 1, p.wait_limit);
+    };
+    auto flush = [&]() {
+      const int seg = (int)blockIdx.x - stream_owner(p.units, p.ctas, open * p.steps);
+      float* dst = p.part + ((int64_t)(open * p.max_segs + seg) * p.cols) * kL4BlockRows + wg * kL4TileRows + row;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        if (c < p.cols) dst[(int64_t)c * kL4BlockRows] = ok ? acc[c] : __int_as_float(0x7fc00000);
+        acc[c] = 0.f;
+      }
+    };
+    int st = 0, w_phase = 0;
+    for (int u = u0; u < u1; ++u) {
+      if (rb * kL4Groups + wg >= p.row_tiles) break;  // no rows here, nor later
+      const uint32_t stage = smem_u32(smem + C::kRing + (wg * C::kStages + st) * C::kStageBytes);
+      if (ok) ok = mbar_wait(smem_u32(&bars.w_full[wg][st]), w_phase, p.wait_limit);
       float s[NPG];
       uint32_t z = 0;
       {
-        const uint32_t sa = smem_u32(stage + kL4TileBytes) + row * NPG * 4;
+        const uint32_t sa = stage + kL4TileBytes + row * NPG * 4, za = stage + kL4TileBytes + C::kScaleBytes + row * NPG;
         if constexpr (NPG == 1) {
           asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s[0]) : "r"(sa));
+          if (MODE == kIntZeros) asm volatile("ld.shared.u8 %0, [%1];" : "=r"(z) : "r"(za));
         } else if constexpr (NPG == 2) {
           asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(s[0]), "=f"(s[1]) : "r"(sa));
+          if (MODE == kIntZeros) asm volatile("ld.shared.u16 %0, [%1];" : "=r"(z) : "r"(za));
         } else {
           const float4 v = lds_f4(sa);
           s[0] = v.x;
           s[1] = v.y;
           s[2] = v.z;
           s[3] = v.w;
-        }
-        if (MODE == kIntZeros) {
-          const unsigned char* za = stage + kL4TileBytes + C::kScaleBytes + row * NPG;
-          if constexpr (NPG == 1) {
-            z = *za;
-          } else if constexpr (NPG == 2) {
-            z = *reinterpret_cast<const unsigned short*>(za);
-          } else {
-            z = *reinterpret_cast<const uint32_t*>(za);
-          }
+          if (MODE == kIntZeros) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(z) : "r"(za));
         }
       }
 #pragma unroll
       for (int t = 0; t < kSlots; ++t) {
+        const uint32_t slot_col = (uint32_t)(slots & 1) * (kL4TmemA / 2);
 #pragma unroll
         for (int c = 0; c < kSlotCols / 32; ++c) {
-          const uint4 q = lds_u4(smem_u32(stage) + ((t * (kSlotCols / 32) + c) * kL4TileRows + row) * 16);
+          const uint4 q = lds_u4(stage + ((t * (kSlotCols / 32) + c) * kL4TileRows + row) * 16);
           const uint32_t word[4] = {q.x, q.y, q.z, q.w};
           uint32_t za = 0x64086408u, zb = 0xd480d480u;  // 1024 + 8, -(64 + 8)
           if constexpr (MODE == kIntZeros) {
@@ -501,74 +587,40 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
                 r[4 * j + 3] = int_pair<3>(word[j], za, zb);
               }
             }
-            tmem_st16(mine + half * (kSlotCols / 2) + c * 16, r);
+            tmem_st16(mine + slot_col + half * (kSlotCols / 2) + c * 16, r);
+          }
+        }
+        // the round before this one went on meanwhile
+        if (slots > 0) {
+          if (t == 0) {
+            add_last(true, last_s);
+            if (open != rb) flush();
+          } else {
+            add_last(t % kSlotsPerScale == 0, s + (t * NPG / kSlots - kScalesPerSlot));
           }
         }
         tmem_wait_st();
         tmem_fence_before();
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
-        if (issuer) {
-          if (t == kSlots - 1 && u + C::kStages < u1 && ok) {  // the tile is read: its place takes the next copy
-            fence_proxy_async_smem();
-            copy_tile(u + C::kStages);
-            copied = u + C::kStages + 1;
-          }
-          if (t == 0 && ok) ok = mbar_wait(smem_u32(&bars.x_full[xst]), (i / kL4XStages) & 1, p.wait_limit);
-          tmem_fence_after();
-          const uint32_t x0 = smem_u32(smem + C::kX + xst * C::kXBytes) + t * (kSlotCols / 8) * (C::kXGroups * 128);
-          // K-major without swizzle: 8 columns of the weight are kXGroups x 128 bytes on, 8 columns
-          // of x 128 bytes (with one group the upper eight of N = 16 are never read back)
-          const uint64_t desc = (uint64_t)((x0 >> 4) & 0x3fff) | ((uint64_t)(C::kXGroups * 128 / 16) << 16) |
-                                ((uint64_t)(128 / 16) << 32) | (1ull << 46);
-#pragma unroll
-          for (int k = 0; k < kSlotCols / 16; ++k) {
-            const uint32_t d = a0 + kL4TmemA + (16 * k / kScaleCols) * C::kN;
-#pragma unroll
-            for (int half = 0; half < (MODE == kCodeExact ? 2 : 1); ++half)
-              mma_f16_ts(d, a0 + half * (kSlotCols / 2) + k * 8, desc + (uint64_t)(k * 2 * C::kXGroups * 128 / 16), kIdesc,
-                         !(t % kSlotsPerScale == 0 && half == 0 && 16 * k % kScaleCols == 0));
-          }
-          mma_commit(smem_u32(&bars.done[wg]));
-          if (t == kSlots - 1) mma_commit(smem_u32(&bars.x_free[xst]));
-        }
         __syncwarp();
-        if (ok) ok = mbar_wait(smem_u32(&bars.done[wg]), slots & 1, p.wait_limit);
-        __syncwarp();
-        tmem_fence_after();
+        if (lane == 0) mbar_arrive(smem_u32(&bars.full[wg]));
+        if (t == 0) open = rb;
         ++slots;
-        if (t % kSlotsPerScale == kSlotsPerScale - 1) {
-#pragma unroll
-          for (int g = 0; g < kScalesPerSlot; ++g) {
-            const float sc = s[t * NPG / kSlots + g];
-#pragma unroll
-            for (int c0 = 0; c0 < NC; c0 += kLd) {
-              uint32_t r[kLd];
-              tmem_ld<kLd>(mine + kL4TmemA + g * C::kN + c0, r);
-              tmem_wait_ld();
-#pragma unroll
-              for (int c = 0; c < kLd; ++c) acc[c0 + c] = fmaf(sc, __uint_as_float(r[c]), acc[c0 + c]);
-            }
-          }
-        }
       }
-      if (last) {
-        const int seg = (int)blockIdx.x - stream_owner(p.units, p.ctas, rb * p.steps);
-        float* dst = p.part + ((int64_t)(rb * p.max_segs + seg) * p.cols) * kL4BlockRows + wg * kL4TileRows + row;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          if (c < p.cols) dst[(int64_t)c * kL4BlockRows] = ok ? acc[c] : __int_as_float(0x7fc00000);
-          acc[c] = 0.f;
-        }
+      for (int g = 0; g < kScalesPerSlot; ++g) last_s[g] = s[NPG - kScalesPerSlot + g];
+      if (++st == C::kStages) {
+        st = 0;
+        w_phase ^= 1;
       }
       if (++step == p.steps) {
         step = 0;
         ++rb;
       }
     }
-    if (issuer && !ok)  // after a failure: no copy may land in shared memory that is gone
-      for (int u = max(u0, copied - C::kStages); u < copied; ++u)
-        if (u / p.steps * kL4Groups + wg < p.row_tiles)
-          mbar_wait(smem_u32(&bars.w_full[wg][(u - u0) % C::kStages]), ((u - u0) / C::kStages) & 1);
+    if (slots > 0) {
+      add_last(true, last_s);
+      flush();
+    }
     __syncwarp();
     tmem_fence_before();
   }
