@@ -11,12 +11,13 @@
 // row, and a warp's 16-byte loads are 512 contiguous bytes.  Scales and zero points lie
 // as [row tile][tile][128 rows][granules], a granule being the group or 128 columns.
 //
-// Three launches, linked by programmatic dependent launch:
-//  1. lin4_prep_kernel: per row of x a power-of-two scale that brings the
-//     largest finite |x| to [2^14, 2^15) and x as fp16 (exact for fp16, and for bf16
+// Two or three launches, linked by programmatic dependent launch:
+//  1. for more than 8 columns of x, lin4_prep_kernel: per row of x a power-of-two scale that
+//     brings the largest finite |x| to [2^14, 2^15) and x as fp16 (exact for fp16, and for bf16
 //     down to 2^-38 of the row's largest); an fp32 x becomes two fp16 columns
 //     (value and remainder, 22 bits).  x is written as the 8 x 16-byte core matrices of a
-//     K-major tensor-core operand;
+//     K-major tensor-core operand.  For up to 8 columns lin4_kernel does this itself, with a
+//     scale for each 128 columns of a row: one launch and 5 us less at 16384 columns;
 //  2. lin4_kernel: one CTA per SM, four warpgroups of 128 rows each.  A unit is 512 rows x
 //     128 columns; the units, row block by row block, are cut into equal contiguous runs,
 //     one per CTA, so no CTA finishes late.  Bulk copies bring each warpgroup's tile and
@@ -41,17 +42,15 @@ namespace nsm {
 namespace {
 
 constexpr int kL4Groups = 4;                          // warpgroups of a CTA
-constexpr int kL4Threads = kL4Groups * 160 + 32;      // each with a warp that issues its copies and MMAs; + copies of x
+constexpr int kL4XStages = 4;                         // x tiles in flight, and warps that bring them
+constexpr int kL4Threads = kL4Groups * 160 + kL4XStages * 32;  // each group with a warp that issues its copies and MMAs
 constexpr int kL4TileRows = 128;
 constexpr int kL4TileCols = 128;
 constexpr int kL4TileBytes = kL4TileRows * kL4TileCols / 2;
 constexpr int kL4BlockRows = kL4TileRows * kL4Groups;  // rows of a unit
 constexpr int kL4MaxCols = 32;                        // fp16 columns of x in one call
 constexpr int kL4MaxSegs = 32;                        // CTAs that share one row block
-constexpr int kL4XStages = 4;                         // x tiles in flight
-// tensor memory: per warpgroup two slots of 32 columns of weights (fp16 pairs) and 64 columns
-// of products
-constexpr uint32_t kL4TmemA = 64, kL4TmemGroup = 128;
+constexpr uint32_t kL4TmemGroup = 128;                // columns of tensor memory per warpgroup
 
 // Kinds of weights: codebook rounded to fp16; codebook as fp16 value +
 // remainder (22 bits, two table reads and two MMAs: outputs in fp32); integers
@@ -215,8 +214,11 @@ struct Lin4Params {
   const float* s;
   const uint8_t* z;
   const float* code;
-  const __half* xh;
-  float* part;  // [row block][segment][column of x][256]
+  const void* x;     // [rows][K], read by the kernel itself (NC <= 8)
+  const __half* xh;  // or its tiles from lin4_prep_kernel
+  int64_t x_stride;
+  int x_dtype, rows, K;
+  float* part;  // [row block][segment][column of x][512]
   int row_tiles, steps, scale_steps, div, cols;
   int units, ctas, max_segs, wait_limit;
 };
@@ -233,16 +235,24 @@ __device__ __forceinline__ uint32_t hfma2_u32(uint32_t a, uint32_t b, uint32_t c
 // Nibbles k and k + 4 (k = kPair) of an integer word as half2 {q - z, q' - z}:
 // 0x6400 | q is 1024 + q in fp16; the odd pairs are taken 4 bits higher (1024 +
 // 16 q) and brought down by 1/16.  za = 1024 + z, zb = -(64 + z): all exact.
+template <uint32_t kMask>
+__device__ __forceinline__ uint32_t masked_1024(uint32_t v) {  // (v & kMask) | 0x64006400 in one instruction
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(v), "n"(kMask), "r"(0x64006400u));
+  return r;
+}
 template <int kPair>
 __device__ __forceinline__ uint32_t int_pair(uint32_t w, uint32_t za, uint32_t zb) {
   const uint32_t v = kPair >= 2 ? w >> 8 : w;
-  if (kPair % 2 == 0) return hsub2_u32((v & 0x000f000fu) | 0x64006400u, za);
-  return hfma2_u32((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, zb);
+  if (kPair % 2 == 0) return hsub2_u32(masked_1024<0x000f000fu>(v), za);
+  return hfma2_u32(masked_1024<0x00f000f0u>(v), 0x2c002c00u, zb);
 }
 
 // ---- tensor memory and the 5th-generation tensor core ----
-__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// Volatile, so that they keep their order; no memory clobber, so that the compiler may
+// move table reads over them (tensor memory is nothing that C++ code reads or writes).
+__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;"); }
+__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;"); }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -251,34 +261,36 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
 }
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;"); }
+// The loaded registers pass through the wait, so that nothing uses them before it.
+template <int N>
+__device__ __forceinline__ void tmem_wait_ld(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]));
+#pragma unroll
+  for (int i = 1; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
 template <int N>
 __device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t* r) {
   if constexpr (N == 1) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r[0]) : "r"(addr) : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r[0]) : "r"(addr));
   } else if constexpr (N == 2) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr));
   } else if constexpr (N == 4) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
+                 : "r"(addr));
   } else if constexpr (N == 16) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
                    "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(addr)
-                 : "memory");
+                 : "r"(addr));
   } else {
     static_assert(N == 8, "columns at a time");
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(addr)
-                 : "memory");
+                 : "r"(addr));
   }
 }
 // D[128 lanes][N] (+)= A (tensor memory, fp16 pairs along K) x B (shared memory, K-major)
@@ -294,6 +306,69 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
+// Eight columns of a row of x on their way to an operand tile.
+struct XRun {
+  uint32_t r[8];  // fp32 values, or four words of 16-bit pairs
+  __device__ __forceinline__ void load(const Lin4Params& p, int row, int col) {
+    const int es = p.x_dtype == NSM_F32 ? 4 : 2;
+    const char* at = static_cast<const char*>(p.x) + ((int64_t)row * p.x_stride + col) * es;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = 0;
+    if (row >= p.rows || col >= p.K) return;
+    if (((uintptr_t)at & 15) == 0 && col + 8 <= p.K) {
+      const uint4 a = *reinterpret_cast<const uint4*>(at);
+      r[0] = a.x, r[1] = a.y, r[2] = a.z, r[3] = a.w;
+      if (es == 4) {
+        const uint4 b = *reinterpret_cast<const uint4*>(at + 16);
+        r[4] = b.x, r[5] = b.y, r[6] = b.z, r[7] = b.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (col + i < p.K) {
+          if (es == 4) {
+            r[i] = reinterpret_cast<const uint32_t*>(at)[i];
+          } else {
+            r[i / 2] |= (uint32_t) reinterpret_cast<const unsigned short*>(at)[i] << (16 * (i % 2));
+          }
+        }
+      }
+    }
+  }
+  // As fp16 (and, for fp32, the remainders), divided by the returned power of two, which
+  // brings the largest finite value of the half-warp's 128 columns to [2^14, 2^15).
+  __device__ __forceinline__ float to_half(int dtype, uint4& hi, uint4& lo) const {
+    if (dtype == NSM_F16) {
+      hi = make_uint4(r[0], r[1], r[2], r[3]);
+      return 1.f;
+    }
+    float v[8], m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = dtype == NSM_F32 ? __uint_as_float(r[i]) : __uint_as_float(i % 2 ? r[i / 2] & 0xffff0000u : r[i / 2] << 16);
+      const float a = fabsf(v[i]);
+      m = fmaxf(m, a <= 3.4028234e38f ? a : 0.f);  // infinities and NaN stay what they are
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float s = m > 0.f ? ldexpf(1.f, max(-120, min(120, ilogbf(m) - 14))) : 1.f, inv = 1.f / s;
+    __half h[8], l[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = v[i] * inv;
+      h[i] = __float2half_rn(x);
+      const float rem = x - __half2float(h[i]);
+      l[i] = __float2half_rn(fabsf(rem) <= 3.4028234e38f ? rem : 0.f);
+    }
+    auto pair = [](const __half* q, int i) {
+      return (uint32_t)__half_as_ushort(q[2 * i]) | ((uint32_t)__half_as_ushort(q[2 * i + 1]) << 16);
+    };
+    hi = make_uint4(pair(h, 0), pair(h, 1), pair(h, 2), pair(h, 3));
+    if (dtype == NSM_F32) lo = make_uint4(pair(l, 0), pair(l, 1), pair(l, 2), pair(l, 3));
+    return s;
+  }
+};
+
 // What a kernel variant holds, for device and host.  NPG: scale granules per tile of 128
 // columns.  NC: columns of x that the sums hold.
 template <int MODE, int NPG, int NC>
@@ -301,34 +376,46 @@ struct Lin4Config {
   static constexpr bool kIsCode = MODE == kCode || MODE == kCodeExact;
   static constexpr int kXGroups = NC <= 8 ? 1 : NC / 8;                    // groups of eight columns of x
   static constexpr int kXBytes = kXGroups * 8 * kL4TileCols * 2;           // of a tile
+  static constexpr bool kOwnX = NC <= 8;                                   // the kernel makes x's tiles itself
   static constexpr int kN = NC <= 16 ? 16 : 32;                            // of the MMA
   static constexpr int kSlotCols = MODE == kCodeExact ? 32 : 64;           // weight columns of a slot
+  static constexpr int kSlots = kL4TileCols / kSlotCols;                   // per tile
+  static constexpr int kScalesPerSlot = NPG >= kSlots ? NPG / kSlots : 1;
+  static constexpr int kSlotsPerScale = NPG >= kSlots ? 1 : kSlots / NPG;
+  // Rounds of MMAs under way while the warpgroup fills the next slot: a slot takes 32
+  // columns of tensor memory (fp16 pairs), its products kN for each scale; three slots and two
+  // sets of products where they fit, else two and one.
+  static constexpr int kDCols = kScalesPerSlot * kN;
+  static constexpr int kLag = 3 * 32 + 2 * kDCols <= (int)kL4TmemGroup ? 2 : 1;
+  static constexpr uint32_t kD = (kLag + 1) * 32;  // where the products begin
+  static_assert((int)kD + kLag * kDCols <= (int)kL4TmemGroup, "tensor memory");
   static constexpr int kScaleBytes = kL4TileRows * NPG * 4;
   static constexpr int kStageBytes = kL4TileBytes + kScaleBytes + (MODE == kIntZeros ? kL4TileRows * NPG : 0);
   static constexpr int kStages = kIsCode ? 3 : 4;                          // weight tiles in flight per warpgroup
   static constexpr int kLut = kIsCode ? kLutBytes : 0;
   static constexpr int kRing = kLut, kX = kRing + kL4Groups * kStages * kStageBytes;
   static constexpr int kBars = kX + kL4XStages * kXBytes + 1024;  // the last tile of x is read 128 bytes over
-  static constexpr int kSmem = kBars + 320;
+  static constexpr int kSmem = kBars + 512;
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
 struct Lin4Bars {
   unsigned long long w_full[kL4Groups][4];  // a tile of weights and its scales are in shared memory
-  unsigned long long full[kL4Groups];       // a slot of weights is in tensor memory
-  unsigned long long done[kL4Groups];       // its MMAs are done
+  unsigned long long full[kL4Groups][2];    // a slot of weights is in tensor memory (rounds in turn)
+  unsigned long long done[kL4Groups][2];    // its MMAs are done
   unsigned long long x_full[kL4XStages];    // a tile of x is in shared memory
   unsigned long long x_free[kL4XStages];    // all warpgroups' MMAs that read it are done
+  float x_scale[kL4XStages][8];             // kOwnX: what a tile's columns of x were divided by
   uint32_t tmem;
 };
-static_assert(sizeof(Lin4Bars) <= 320, "barriers");
+static_assert(sizeof(Lin4Bars) <= 512, "barriers");
 
 template <int MODE, int NPG, int NC>
 __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_constant__ Lin4Params p) {
   extern __shared__ __align__(1024) uint32_t l4_smem[];
   using C = Lin4Config<MODE, NPG, NC>;
-  constexpr int kSlotCols = C::kSlotCols, kSlots = kL4TileCols / kSlotCols;
-  constexpr int kScalesPerSlot = NPG >= kSlots ? NPG / kSlots : 1, kSlotsPerScale = NPG >= kSlots ? 1 : kSlots / NPG;
+  constexpr int kSlotCols = C::kSlotCols, kSlots = C::kSlots;
+  constexpr int kScalesPerSlot = C::kScalesPerSlot, kSlotsPerScale = C::kSlotsPerScale, kLag = C::kLag;
   constexpr int kScaleCols = kSlotCols / kScalesPerSlot;  // columns of one product
   constexpr int kLd = NC < 32 ? NC : 16;                  // products read at a time
   // fp32 accumulators, fp16 operands, both K-major, N / 8 and M / 16 in bits 17 and 24
@@ -349,8 +436,10 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
   if (threadIdx.x == 32) {
     for (int g = 0; g < kL4Groups; ++g) {
       for (int i = 0; i < C::kStages; ++i) mbar_init(smem_u32(&bars.w_full[g][i]), 1);
-      mbar_init(smem_u32(&bars.full[g]), 4);  // the group's four warps
-      mbar_init(smem_u32(&bars.done[g]), 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(smem_u32(&bars.full[g][i]), 4);  // the group's four warps
+        mbar_init(smem_u32(&bars.done[g][i]), 1);
+      }
     }
     for (int i = 0; i < kL4XStages; ++i) {
       mbar_init(smem_u32(&bars.x_full[i]), 1);
@@ -358,6 +447,9 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
     }
     mbar_init_fence();
   }
+  // Without lin4_prep_kernel in front, nothing in global memory is read or written before the
+  // kernel before this one is done; with it, only x waits (the weights are not its work).
+  if (C::kOwnX) pdl_wait();
   __syncthreads();
   int rb = u0 / p.steps, step = u0 - rb * p.steps;
 
@@ -412,36 +504,68 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
 
   // Every wait is bounded.  One that runs out makes its thread go on without waiting, and
   // leaves NaN in the warpgroup's partials.
-  if (my_warp == 5 * kL4Groups) {
-    if (lane == 0) {  // ---- copies of x
+  if (my_warp >= 5 * kL4Groups) {
+    // ---- tiles of x: each of these warps fills one place of the ring
+    const int st = my_warp - 5 * kL4Groups;
+    const uint32_t full = smem_u32(&bars.x_full[st]), free = smem_u32(&bars.x_free[st]);
+    unsigned char* dst = smem + C::kX + st * C::kXBytes;
+    bool ok = true;
+    int n = 0;  // tiles so far
+    if constexpr (C::kOwnX) {
+      const float icode = C::kIsCode ? 1.f / code_scale(p.code) : 1.f;  // a power of two
+      for (int u = u0 + st; u < u1; u += kL4XStages, ++n) {
+        const int col0 = u % p.steps * kL4TileCols;
+        XRun v[NC <= 2 ? 1 : NC / 2];  // lanes 0-15: 8 columns each of row 2i, lanes 16-31: of row 2i + 1
+#pragma unroll
+        for (int i = 0; i < (NC <= 2 ? 1 : NC / 2); ++i) {
+          const int r = 2 * i + (lane >> 4);
+          v[i].load(p, r, col0 + 8 * (lane & 15));
+        }
+        if (n > 0 && ok) ok = mbar_wait(free, (n - 1) & 1, p.wait_limit);
+        __syncwarp();
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < (NC <= 2 ? 1 : NC / 2); ++i) {
+          const int r = 2 * i + (lane >> 4);
+          uint4 hi, lo;
+          const float s = v[i].to_half(p.x_dtype, hi, lo);
+          if (r < p.rows) {
+            // core matrices of 8 columns of x by 8 of the weight: [k / 8][c][k % 8]
+            *reinterpret_cast<uint4*>(dst + ((lane & 15) * 8 + r) * 16) = hi;
+            if ((lane & 15) == 0) bars.x_scale[st][r] = s * icode;
+            if (p.x_dtype == NSM_F32) {
+              *reinterpret_cast<uint4*>(dst + ((lane & 15) * 8 + p.rows + r) * 16) = lo;
+              if ((lane & 15) == 0) bars.x_scale[st][p.rows + r] = s * icode;
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full);
+      }
+    } else if (lane == 0) {
       pdl_wait();
       fence_proxy_async_global();
       const uint64_t keep = l2_evict_last_policy();
-      bool ok = true;
-      for (int u = u0; u < u1; ++u) {
-        const int i = u - u0, st = i % kL4XStages;
-        if (i >= kL4XStages) ok = mbar_wait(smem_u32(&bars.x_free[st]), (i / kL4XStages - 1) & 1, p.wait_limit);
+      for (int u = u0 + st; u < u1; u += kL4XStages, ++n) {
+        if (n > 0) ok = mbar_wait(free, (n - 1) & 1, p.wait_limit);
         if (!ok) break;
-        const uint32_t bar = smem_u32(&bars.x_full[st]);
-        mbar_arrive_expect_tx(bar, C::kXBytes);
-        bulk_g2s(smem_u32(smem + C::kX + st * C::kXBytes),
-                 reinterpret_cast<const unsigned char*>(p.xh) + (int64_t)step * C::kXBytes, C::kXBytes, bar, keep);
-        copied = i + 1;
-        if (++step == p.steps) step = 0;
+        mbar_arrive_expect_tx(full, C::kXBytes);
+        bulk_g2s(smem_u32(dst), reinterpret_cast<const unsigned char*>(p.xh) + (int64_t)(u % p.steps) * C::kXBytes, C::kXBytes,
+                 full, keep);
       }
-      // nothing may arrive in shared memory that is gone: the last copies and commits
-      for (int i = max(0, copied - kL4XStages); i < copied; ++i) {
-        mbar_wait(smem_u32(&bars.x_full[i % kL4XStages]), (i / kL4XStages) & 1);
-        if (ok) ok = mbar_wait(smem_u32(&bars.x_free[i % kL4XStages]), (i / kL4XStages) & 1, p.wait_limit);
-      }
+      if (n > 0) mbar_wait(full, (n - 1) & 1);
     }
+    // nothing may arrive in shared memory that is gone: the last commits
+    if (lane == 0 && n > 0 && ok) mbar_wait(free, (n - 1) & 1, p.wait_limit);
     __syncwarp();
   } else if (issuing) {
     // ---- MMAs and copies of the warpgroup's tiles
     const uint32_t a0 = tmem + wg * kL4TmemGroup;
-    const uint32_t full_bar = smem_u32(&bars.full[wg]), done_bar = smem_u32(&bars.done[wg]);
+    const uint32_t full_bar = smem_u32(&bars.full[wg][0]), done_bar = smem_u32(&bars.done[wg][0]);
     bool ok = true;
-    int slots = 0, xst = 0, x_phase = 0;
+    int slots = 0, xst = 0, x_phase = 0;  // rounds so far, ring position of x
+    uint32_t a_col = 0, d_col = C::kD;    // of this round
     for (int u = u0; u < u1; ++u) {
       const uint32_t xfree = smem_u32(&bars.x_free[xst]);
       if (ok) ok = mbar_wait(smem_u32(&bars.x_full[xst]), x_phase, p.wait_limit);
@@ -453,21 +577,21 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
                                ((uint64_t)(128 / 16) << 32) | (1ull << 46);
 #pragma unroll
         for (int t = 0; t < kSlots; ++t) {
-          if (ok) ok = mbar_wait(full_bar, slots & 1, p.wait_limit);
+          if (ok) ok = mbar_wait(full_bar + 8 * (slots & 1), (slots >> 1) & 1, p.wait_limit);
           __syncwarp();
           tmem_fence_after();
-          const uint32_t a = a0 + (uint32_t)(slots & 1) * (kL4TmemA / 2);
+          const uint32_t a = a0 + a_col;
           if (lane == 0) {
 #pragma unroll
             for (int k = 0; k < kSlotCols / 16; ++k) {
-              const uint32_t d = a0 + kL4TmemA + (16 * k / kScaleCols) * C::kN;
+              const uint32_t d = a0 + d_col + (16 * k / kScaleCols) * C::kN;
 #pragma unroll
               for (int half = 0; half < (MODE == kCodeExact ? 2 : 1); ++half)
                 mma_f16_ts(d, a + half * (kSlotCols / 2) + k * 8,
                            desc0 + (uint64_t)((t * (kSlotCols / 8) + 2 * k) * C::kXGroups * 128 / 16), kIdesc,
                            !(t % kSlotsPerScale == 0 && half == 0 && 16 * k % kScaleCols == 0));
             }
-            mma_commit(done_bar);
+            mma_commit(done_bar + 8 * (slots & 1));
             if (t == kSlots - 1) {
               mma_commit(xfree);
               if (copied < u1 - u0 && ok) {  // the tile is read: its place takes the next copy
@@ -478,6 +602,8 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
           }
           __syncwarp();
           ++slots;
+          a_col = a_col == kLag * 32 ? 0 : a_col + 32;
+          if (kLag == 2 && t % kSlotsPerScale == kSlotsPerScale - 1) d_col ^= C::kD ^ (C::kD + C::kDCols);
         }
       } else if (lane == 0) {  // no rows here (in the last row block): only x goes by
         mbar_arrive(xfree);
@@ -500,17 +626,19 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
     // ---- the warpgroup: 4 bits -> fp16 -> tensor memory, and the sums
     const uint32_t mine = tmem + wg * kL4TmemGroup + ((uint32_t)(my_warp & 3) << 21);  // this warp's 32 lanes
     const uint32_t lanebase = (uint32_t)lane * 4u;
-    const uint32_t done_bar = smem_u32(&bars.done[wg]);
+    const uint32_t full_bar = smem_u32(&bars.full[wg][0]), done_bar = smem_u32(&bars.done[wg][0]);
     float acc[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) acc[c] = 0.f;
     bool ok = true;
-    int slots = 0;       // MMA rounds so far
-    float last_s[kScalesPerSlot];  // scales of the last round's products
-    int open = -1;       // row block of the sums and of the last round
-    // waits for the last round; its products, scaled, join the sums if they are whole
-    auto add_last = [&](bool whole, const float* s) {
-      if (ok) ok = mbar_wait(done_bar, (slots - 1) & 1, p.wait_limit);
+    int slots = 0;                         // rounds so far
+    uint32_t a_col = 0, d_col = C::kD;     // of this round; of the products to add next
+    constexpr int kXs = C::kOwnX ? NC : 1;
+    float ps[NPG], pxs[kXs];               // the scales of the tile before, its weights' and x's
+    int open = -1;                         // its row block: that of the sums
+    // waits for round i; its products, scaled, join the sums if they are whole
+    auto add_round = [&](int i, bool whole, const float* s, const float* xs) {
+      if (ok) ok = mbar_wait(done_bar + 8 * (i & 1), (i >> 1) & 1, p.wait_limit);
       __syncwarp();
       tmem_fence_after();
       if (whole) {
@@ -519,12 +647,16 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
 #pragma unroll
           for (int c0 = 0; c0 < NC; c0 += kLd) {
             uint32_t r[kLd];
-            tmem_ld<kLd>(mine + kL4TmemA + g * C::kN + c0, r);
-            tmem_wait_ld();
+            tmem_ld<kLd>(mine + d_col + g * C::kN + c0, r);
+            tmem_wait_ld<kLd>(r);
 #pragma unroll
-            for (int c = 0; c < kLd; ++c) acc[c0 + c] = fmaf(s[g], __uint_as_float(r[c]), acc[c0 + c]);
+            for (int c = 0; c < kLd; ++c) {
+              const float sc = C::kOwnX ? s[g] * xs[c0 + c] : s[g];  // (x's are powers of two)
+              acc[c0 + c] = fmaf(sc, __uint_as_float(r[c]), acc[c0 + c]);
+            }
           }
         }
+        if (kLag == 2) d_col ^= C::kD ^ (C::kD + C::kDCols);
       }
     };
     auto flush = [&]() {
@@ -536,12 +668,22 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
         acc[c] = 0.f;
       }
     };
-    int st = 0, w_phase = 0;
+    int st = 0, w_phase = 0, xst = 0, x_phase = 0;  // ring positions
     for (int u = u0; u < u1; ++u) {
       if (rb * kL4Groups + wg >= p.row_tiles) break;  // no rows here, nor later
       const uint32_t stage = smem_u32(smem + C::kRing + (wg * C::kStages + st) * C::kStageBytes);
       if (ok) ok = mbar_wait(smem_u32(&bars.w_full[wg][st]), w_phase, p.wait_limit);
-      float s[NPG];
+      float s[NPG], xs[kXs];
+      if constexpr (C::kOwnX) {
+        if (ok) ok = mbar_wait(smem_u32(&bars.x_full[xst]), x_phase, p.wait_limit);
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(xs[c]) : "r"(smem_u32(&bars.x_scale[xst][c])));
+        if (++xst == kL4XStages) {
+          xst = 0;
+          x_phase ^= 1;
+        }
+      }
       uint32_t z = 0;
       {
         const uint32_t sa = stage + kL4TileBytes + row * NPG * 4, za = stage + kL4TileBytes + C::kScaleBytes + row * NPG;
@@ -562,7 +704,6 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
       }
 #pragma unroll
       for (int t = 0; t < kSlots; ++t) {
-        const uint32_t slot_col = (uint32_t)(slots & 1) * (kL4TmemA / 2);
 #pragma unroll
         for (int c = 0; c < kSlotCols / 32; ++c) {
           const uint4 q = lds_u4(stage + ((t * (kSlotCols / 32) + c) * kL4TileRows + row) * 16);
@@ -587,27 +728,30 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
                 r[4 * j + 3] = int_pair<3>(word[j], za, zb);
               }
             }
-            tmem_st16(mine + slot_col + half * (kSlotCols / 2) + c * 16, r);
+            tmem_st16(mine + a_col + half * (kSlotCols / 2) + c * 16, r);
           }
         }
-        // the round before this one went on meanwhile
-        if (slots > 0) {
-          if (t == 0) {
-            add_last(true, last_s);
-            if (open != rb) flush();
-          } else {
-            add_last(t % kSlotsPerScale == 0, s + (t * NPG / kSlots - kScalesPerSlot));
-          }
+        // the round kLag before this one went on meanwhile
+        const int was = (t + kSlots - kLag) % kSlots;  // its slot: of this tile, or of the one before
+        constexpr int kLast = kSlotsPerScale - 1;
+        if (t >= kLag) {
+          add_round(slots - kLag, was % kSlotsPerScale == kLast, s + was * NPG / kSlots, xs);
+        } else if (open >= 0) {
+          add_round(slots - kLag, was % kSlotsPerScale == kLast, ps + was * NPG / kSlots, pxs);
+          if (was == kSlots - 1 && open != rb) flush();
         }
         tmem_wait_st();
         tmem_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bars.full[wg]));
-        if (t == 0) open = rb;
+        if (lane == 0) mbar_arrive(full_bar + 8 * (slots & 1));
         ++slots;
+        a_col = a_col == kLag * 32 ? 0 : a_col + 32;
       }
+      open = rb;
 #pragma unroll
-      for (int g = 0; g < kScalesPerSlot; ++g) last_s[g] = s[NPG - kScalesPerSlot + g];
+      for (int g = 0; g < NPG; ++g) ps[g] = s[g];
+#pragma unroll
+      for (int c = 0; c < kXs; ++c) pxs[c] = xs[c];
       if (++st == C::kStages) {
         st = 0;
         w_phase ^= 1;
@@ -617,8 +761,10 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
         ++rb;
       }
     }
-    if (slots > 0) {
-      add_last(true, last_s);
+    if (open >= 0) {
+#pragma unroll
+      for (int t = kSlots - kLag; t < kSlots; ++t)
+        add_round(slots - kSlots + t, t % kSlotsPerScale == kSlotsPerScale - 1, ps + t * NPG / kSlots, pxs);
       flush();
     }
     __syncwarp();
@@ -634,6 +780,7 @@ __global__ void __launch_bounds__(kL4BlockRows) lin4_finalize_kernel(const float
                                                                      int ctas, int steps, int max_segs, int cols,
                                                                      int rows, int N, const void* bias, int bias_dt,
                                                                      void* out, int out_dt, int64_t out_stride) {
+  pdl_trigger();
   pdl_wait();
   const int rb = blockIdx.x, r = blockIdx.y, n = rb * kL4BlockRows + threadIdx.x;
   if (n >= N) return;
@@ -648,12 +795,13 @@ __global__ void __launch_bounds__(kL4BlockRows) lin4_finalize_kernel(const float
     if (cols > rows) e += __ldcg(q + (int64_t)rows * kL4BlockRows);  // the remainders of an fp32 x
     v += e;
   }
-  v *= __ldcg(scale + r);
+  if (scale) v *= __ldcg(scale + r);
   if (bias) v += load_as_f32(bias, bias_dt, n);
   store_from_f32(out, out_dt, (int64_t)r * out_stride + n, v);
 }
 
 struct Lin4Plan {
+  bool own_x = false;  // few columns: the kernel reads x itself
   int cols = 0, col_groups = 1, units = 0, ctas = 0, max_segs = 0;
   size_t scale_off = 0, part_off = 0, bytes = 0;
 };
@@ -666,8 +814,9 @@ Lin4Plan lin4_plan(const Lin4Shape& sh, int rows, int x_dtype, int sm_count) {
   const int least = pl.units / pl.ctas;  // units of the shortest run
   pl.max_segs = (sh.steps - 1 + least - 1) / least + 1;
   pl.col_groups = pl.cols <= 8 ? 1 : pl.cols <= 16 ? 2 : 4;
-  pl.scale_off = align_up((size_t)pl.col_groups * 8 * sh.kp * 2, 256);
-  pl.part_off = pl.scale_off + align_up((size_t)rows * 4, 256);
+  pl.own_x = pl.cols <= 8;
+  pl.scale_off = pl.own_x ? 0 : align_up((size_t)pl.col_groups * 8 * sh.kp * 2, 256);
+  pl.part_off = pl.scale_off + (pl.own_x ? 0 : align_up((size_t)rows * 4, 256));
   pl.bytes = pl.part_off + (size_t)sh.row_blocks * pl.max_segs * pl.cols * kL4BlockRows * 4;
   return pl;
 }
@@ -808,16 +957,23 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
                                         : lin4_pick_npg<kIntZeros>(sh.npg, cc);
   static SmemOnce once[4][3][6];
   NSM_CHECK_CUDA(once[mode][sh.npg / 2][cc].set(f.fn, f.smem, di.device));
-  const int slices = std::max(1, std::min(8, sh.kp / 2048));
-  lin4_prep_kernel<<<dim3(slices, rows), 256, 0, s>>>(x, x_dtype, x_row_stride, sh.K, sh.kp, rows, pl.col_groups, w->code,
-                                                      xh, scale);
-  NSM_CHECK_CUDA(cudaGetLastError());
+  if (!pl.own_x) {
+    const int slices = std::max(1, std::min(8, sh.kp / 2048));
+    lin4_prep_kernel<<<dim3(slices, rows), 256, 0, s>>>(x, x_dtype, x_row_stride, sh.K, sh.kp, rows, pl.col_groups,
+                                                        w->code, xh, scale);
+    NSM_CHECK_CUDA(cudaGetLastError());
+  }
   Lin4Params p;
   p.w = w->packed;
   p.s = w->scales;
   p.z = w->zeros;
   p.code = w->code;
+  p.x = x;
   p.xh = xh;
+  p.x_stride = x_row_stride;
+  p.x_dtype = x_dtype;
+  p.rows = rows;
+  p.K = sh.K;
   p.part = part;
   p.row_tiles = sh.row_tiles;
   p.steps = sh.steps;
@@ -830,7 +986,7 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
   p.wait_limit = copy_wait_spins();
   NSM_CHECK_CUDA(launch_pdl(f.fn, dim3(pl.ctas), dim3(kL4Threads), (size_t)f.smem, s, p));
   NSM_CHECK_CUDA(launch_pdl(lin4_finalize_kernel, dim3(sh.row_blocks, rows), dim3(kL4BlockRows), 0, s,
-                            (const float*)part, (const float*)scale, pl.units, pl.ctas, sh.steps, pl.max_segs, pl.cols,
+                            (const float*)part, (const float*)(pl.own_x ? nullptr : scale), pl.units, pl.ctas, sh.steps, pl.max_segs, pl.cols,
                             (int)rows, sh.N, w->bias, (int)w->bias_dtype, out, (int)out_dtype, out_row_stride));
   return NSM_OK;
 }
