@@ -301,6 +301,13 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b_de
       "r"(a), "l"(b_desc), "r"(idesc), "r"((uint32_t)add)
       : "memory");
 }
+// One lane of a converged warp; the compiler keeps the operands of what it guards in uniform
+// registers, which tcgen05 instructions take.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+  return r != 0;
+}
 // The barrier is arrived at when the MMAs issued so far by this thread are done.
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -453,33 +460,29 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
   __syncthreads();
   int rb = u0 / p.steps, step = u0 - rb * p.steps;
 
-  // warps 0-15: the warpgroups; 16-19: one that issues for each; 20: copies of x
+  // warps 0-15: the warpgroups; 16-19: one that issues MMAs for each; 20-23: bring the tiles
   const int my_warp = __shfl_sync(0xffffffffu, warp, 0);
   const bool issuing = my_warp >= 4 * kL4Groups && my_warp < 5 * kL4Groups;
   const int wg = issuing ? my_warp - 4 * kL4Groups : my_warp >> 2;
   const uint64_t once = l2_evict_first_policy();
-  int copy_rb = rb, copy_step = step, copied = 0;  // the unit to copy next, units copied
-  auto copy_tile = [&]() {  // one lane: tile, scales and zero points of the next unit
-    const int64_t rt = (int64_t)copy_rb * kL4Groups + wg;
-    if (rt < p.row_tiles) {
-      const int st = copied % C::kStages;
-      const uint32_t bar = smem_u32(&bars.w_full[wg][st]);
-      const uint32_t dst = smem_u32(smem + C::kRing + (wg * C::kStages + st) * C::kStageBytes);
-      const int64_t e =
-          (rt * p.scale_steps + ((NPG == 1 && p.div > 1) ? copy_step / p.div : copy_step)) * (kL4TileRows * NPG);
+  auto copy_weights = [&](int i) {  // lanes 0-3, one for each warpgroup: tile, scales and zero points of unit u0 + i
+    const int at_rb = (u0 + i) / p.steps, at = u0 + i - at_rb * p.steps;
+    const int64_t rt = (int64_t)at_rb * kL4Groups + lane;
+    if (lane < kL4Groups && rt < p.row_tiles) {
+      const uint32_t bar = smem_u32(&bars.w_full[lane][i % C::kStages]);
+      const uint32_t dst = smem_u32(smem + C::kRing + (lane * C::kStages + i % C::kStages) * C::kStageBytes);
+      const int64_t e = (rt * p.scale_steps + ((NPG == 1 && p.div > 1) ? at / p.div : at)) * (kL4TileRows * NPG);
       mbar_arrive_expect_tx(bar, C::kStageBytes);
-      bulk_g2s(dst, p.w + (rt * p.steps + copy_step) * kL4TileBytes, kL4TileBytes, bar, once);
+      bulk_g2s(dst, p.w + (rt * p.steps + at) * kL4TileBytes, kL4TileBytes, bar, once);
       bulk_g2s(dst + kL4TileBytes, p.s + e, C::kScaleBytes, bar, once);
       if (MODE == kIntZeros) bulk_g2s(dst + kL4TileBytes + C::kScaleBytes, p.z + e, kL4TileRows * NPG, bar, once);
     }
-    ++copied;
-    if (++copy_step == p.steps) {
-      copy_step = 0;
-      ++copy_rb;
-    }
   };
-  if (issuing && lane == 0)
-    for (int u = u0; u < min(u1, u0 + C::kStages); ++u) copy_tile();
+  if (my_warp >= 5 * kL4Groups) {
+    const int i = my_warp - 5 * kL4Groups;
+    if (i < C::kStages && i < u1 - u0) copy_weights(i);
+    __syncwarp();
+  }
 
   if constexpr (C::kIsCode) {  // byte -> half2 table, one copy per lane (conflict-free); the second holds the remainders
     const float cs = code_scale(p.code);
@@ -500,35 +503,55 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
-  const uint32_t tmem = bars.tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, bars.tmem, 0);
 
   // Every wait is bounded.  One that runs out makes its thread go on without waiting, and
   // leaves NaN in the warpgroup's partials.
   if (my_warp >= 5 * kL4Groups) {
-    // ---- tiles of x: each of these warps fills one place of the ring
-    const int st = my_warp - 5 * kL4Groups;
+    // ---- tiles: each of these warps fills one place of x's ring, and when all MMAs that read it
+    // are done, so that all warpgroups have read their weights of that unit too, the place of those
+    const int st = my_warp - 5 * kL4Groups, count = u1 - u0;
     const uint32_t full = smem_u32(&bars.x_full[st]), free = smem_u32(&bars.x_free[st]);
     unsigned char* dst = smem + C::kX + st * C::kXBytes;
+    const uint64_t keep = l2_evict_last_policy();
+    const float icode = C::kOwnX && C::kIsCode ? 1.f / code_scale(p.code) : 1.f;  // a power of two
+    constexpr int kRuns = C::kOwnX ? (NC + 1) / 2 : 1;
     bool ok = true;
-    int n = 0;  // tiles so far
-    if constexpr (C::kOwnX) {
-      const float icode = C::kIsCode ? 1.f / code_scale(p.code) : 1.f;  // a power of two
-      for (int u = u0 + st; u < u1; u += kL4XStages, ++n) {
-        const int col0 = u % p.steps * kL4TileCols;
-        XRun v[NC <= 2 ? 1 : NC / 2];  // lanes 0-15: 8 columns each of row 2i, lanes 16-31: of row 2i + 1
+    int w_last = st < min(C::kStages, count) ? st : -1;  // the last unit whose weights it brought
+    if (!C::kOwnX) {
+      pdl_wait();
+      fence_proxy_async_global();
+    }
+    for (int i = st; i < count + kL4XStages - C::kStages; i += kL4XStages) {
+      const int step_i = (u0 + i) % p.steps;
+      XRun v[kRuns];  // lanes 0-15: 8 columns each of row 2q, lanes 16-31: of row 2q + 1
+      if constexpr (C::kOwnX) {
+        if (i < count) {
 #pragma unroll
-        for (int i = 0; i < (NC <= 2 ? 1 : NC / 2); ++i) {
-          const int r = 2 * i + (lane >> 4);
-          v[i].load(p, r, col0 + 8 * (lane & 15));
+          for (int q = 0; q < kRuns; ++q) v[q].load(p, 2 * q + (lane >> 4), step_i * kL4TileCols + 8 * (lane & 15));
         }
-        if (n > 0 && ok) ok = mbar_wait(free, (n - 1) & 1, p.wait_limit);
-        __syncwarp();
-        if (!ok) break;
+      }
+      if (i >= kL4XStages) {
+        ok = mbar_wait(free, (i / kL4XStages - 1) & 1, p.wait_limit);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        const int j = i - kL4XStages + C::kStages;
+        if (j < count) {
+          fence_proxy_async_smem();
+          copy_weights(j);
+          w_last = j;
+          __syncwarp();
+        }
+      }
+      if (i >= count) break;
+      if constexpr (C::kOwnX) {
 #pragma unroll
-        for (int i = 0; i < (NC <= 2 ? 1 : NC / 2); ++i) {
-          const int r = 2 * i + (lane >> 4);
+        for (int q = 0; q < kRuns; ++q) {
+          const int r = 2 * q + (lane >> 4);
           uint4 hi, lo;
-          const float s = v[i].to_half(p.x_dtype, hi, lo);
+          const float s = v[q].to_half(p.x_dtype, hi, lo);
           if (r < p.rows) {
             // core matrices of 8 columns of x by 8 of the weight: [k / 8][c][k % 8]
             *reinterpret_cast<uint4*>(dst + ((lane & 15) * 8 + r) * 16) = hi;
@@ -542,25 +565,25 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(full);
-      }
-    } else if (lane == 0) {
-      pdl_wait();
-      fence_proxy_async_global();
-      const uint64_t keep = l2_evict_last_policy();
-      for (int u = u0 + st; u < u1; u += kL4XStages, ++n) {
-        if (n > 0) ok = mbar_wait(free, (n - 1) & 1, p.wait_limit);
-        if (!ok) break;
+      } else if (lane == 0) {
         mbar_arrive_expect_tx(full, C::kXBytes);
-        bulk_g2s(smem_u32(dst), reinterpret_cast<const unsigned char*>(p.xh) + (int64_t)(u % p.steps) * C::kXBytes, C::kXBytes,
-                 full, keep);
+        bulk_g2s(smem_u32(dst), reinterpret_cast<const unsigned char*>(p.xh) + (int64_t)step_i * C::kXBytes, C::kXBytes, full,
+                 keep);
       }
-      if (n > 0) mbar_wait(full, (n - 1) & 1);
     }
-    // nothing may arrive in shared memory that is gone: the last commits
-    if (lane == 0 && n > 0 && ok) mbar_wait(free, (n - 1) & 1, p.wait_limit);
+    // Nothing may arrive in shared memory that is gone: the last commits (they come after the
+    // copies they waited for), and after a failure the copies under way.
+    const int last = count > st ? (count - 1 - st) / kL4XStages : -1;  // this place's last round
+    if (lane == 0 && last >= 0 && ok) ok = mbar_wait(free, last & 1, p.wait_limit);
+    ok = __shfl_sync(0xffffffffu, ok, 0);
+    if (!ok) {
+      if (lane < kL4Groups && w_last >= 0 && (u0 + w_last) / p.steps * kL4Groups + lane < p.row_tiles)
+        mbar_wait(smem_u32(&bars.w_full[lane][w_last % C::kStages]), (w_last / C::kStages) & 1);
+      if (!C::kOwnX && lane == 0) mbar_wait(full, last & 1);
+    }
     __syncwarp();
   } else if (issuing) {
-    // ---- MMAs and copies of the warpgroup's tiles
+    // ---- the warpgroup's MMAs
     const uint32_t a0 = tmem + wg * kL4TmemGroup;
     const uint32_t full_bar = smem_u32(&bars.full[wg][0]), done_bar = smem_u32(&bars.done[wg][0]);
     bool ok = true;
@@ -581,7 +604,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
           __syncwarp();
           tmem_fence_after();
           const uint32_t a = a0 + a_col;
-          if (lane == 0) {
+          if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < kSlotCols / 16; ++k) {
               const uint32_t d = a0 + d_col + (16 * k / kScaleCols) * C::kN;
@@ -592,13 +615,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
                            !(t % kSlotsPerScale == 0 && half == 0 && 16 * k % kScaleCols == 0));
             }
             mma_commit(done_bar + 8 * (slots & 1));
-            if (t == kSlots - 1) {
-              mma_commit(xfree);
-              if (copied < u1 - u0 && ok) {  // the tile is read: its place takes the next copy
-                fence_proxy_async_smem();
-                copy_tile();
-              }
-            }
+            if (t == kSlots - 1) mma_commit(xfree);
           }
           __syncwarp();
           ++slots;
@@ -617,10 +634,6 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
         ++rb;
       }
     }
-    if (lane == 0 && !ok)  // after a failure: no copy may land in shared memory that is gone
-      for (int i = max(0, copied - C::kStages); i < copied; ++i)
-        if ((u0 + i) / p.steps * kL4Groups + wg < p.row_tiles)
-          mbar_wait(smem_u32(&bars.w_full[wg][i % C::kStages]), (i / C::kStages) & 1);
     __syncwarp();
   } else {
     // ---- the warpgroup: 4 bits -> fp16 -> tensor memory, and the sums
