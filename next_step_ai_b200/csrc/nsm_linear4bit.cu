@@ -385,16 +385,18 @@ struct Lin4Config {
   static constexpr int kXBytes = kXGroups * 8 * kL4TileCols * 2;           // of a tile
   static constexpr bool kOwnX = NC <= 8;                                   // the kernel makes x's tiles itself
   static constexpr int kN = NC <= 16 ? 16 : 32;                            // of the MMA
-  static constexpr int kSlotCols = MODE == kCodeExact ? 32 : 64;           // weight columns of a slot
+  // A whole tile as one slot (64 columns of tensor memory) whose MMAs the other warpgroups' work
+  // hides, where the products fit beside it; else slots of 32 columns, two or three of them.
+  static constexpr bool kWhole = MODE != kCodeExact && NPG * kN <= 64;
+  static constexpr int kSlotCols = kWhole ? 128 : MODE == kCodeExact ? 32 : 64;  // weight columns of a slot
   static constexpr int kSlots = kL4TileCols / kSlotCols;                   // per tile
   static constexpr int kScalesPerSlot = NPG >= kSlots ? NPG / kSlots : 1;
   static constexpr int kSlotsPerScale = NPG >= kSlots ? 1 : kSlots / NPG;
-  // Rounds of MMAs under way while the warpgroup fills the next slot: a slot takes 32
-  // columns of tensor memory (fp16 pairs), its products kN for each scale; three slots and two
-  // sets of products where they fit, else two and one.
+  // Rounds of MMAs under way while the warpgroup fills the next slot
   static constexpr int kDCols = kScalesPerSlot * kN;
-  static constexpr int kLag = 3 * 32 + 2 * kDCols <= (int)kL4TmemGroup ? 2 : 1;
-  static constexpr uint32_t kD = (kLag + 1) * 32;  // where the products begin
+  static constexpr int kLag = !kWhole && 3 * 32 + 2 * kDCols <= (int)kL4TmemGroup ? 2 : 1;
+  static constexpr int kASlots = kWhole ? 1 : kLag + 1;
+  static constexpr uint32_t kD = kWhole ? 64 : kASlots * 32;  // where the products begin
   static_assert((int)kD + kLag * kDCols <= (int)kL4TmemGroup, "tensor memory");
   static constexpr int kScaleBytes = kL4TileRows * NPG * 4;
   static constexpr int kStageBytes = kL4TileBytes + kScaleBytes + (MODE == kIntZeros ? kL4TileRows * NPG : 0);
@@ -619,7 +621,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
           }
           __syncwarp();
           ++slots;
-          a_col = a_col == kLag * 32 ? 0 : a_col + 32;
+          a_col = a_col == (C::kASlots - 1) * 32 ? 0 : a_col + 32;
           if (kLag == 2 && t % kSlotsPerScale == kSlotsPerScale - 1) d_col ^= C::kD ^ (C::kD + C::kDCols);
         }
       } else if (lane == 0) {  // no rows here (in the last row block): only x goes by
@@ -715,6 +717,16 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
           if (MODE == kIntZeros) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(z) : "r"(za));
         }
       }
+      auto add_earlier = [&](int t) {  // the round kLag before slot t's, which went on meanwhile
+        const int was = (t + kSlots - kLag) % kSlots;  // its slot: of this tile, or of the one before
+        constexpr int kLast = kSlotsPerScale - 1;
+        if (t >= kLag) {
+          add_round(slots - kLag, was % kSlotsPerScale == kLast, s + was * NPG / kSlots, xs);
+        } else if (open >= 0) {
+          add_round(slots - kLag, was % kSlotsPerScale == kLast, ps + was * NPG / kSlots, pxs);
+          if (was == kSlots - 1 && open != rb) flush();
+        }
+      };
 #pragma unroll
       for (int t = 0; t < kSlots; ++t) {
 #pragma unroll
@@ -741,24 +753,17 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
                 r[4 * j + 3] = int_pair<3>(word[j], za, zb);
               }
             }
+            if (C::kWhole && c == 0) add_earlier(t);  // the slot is free
             tmem_st16(mine + a_col + half * (kSlotCols / 2) + c * 16, r);
           }
         }
-        // the round kLag before this one went on meanwhile
-        const int was = (t + kSlots - kLag) % kSlots;  // its slot: of this tile, or of the one before
-        constexpr int kLast = kSlotsPerScale - 1;
-        if (t >= kLag) {
-          add_round(slots - kLag, was % kSlotsPerScale == kLast, s + was * NPG / kSlots, xs);
-        } else if (open >= 0) {
-          add_round(slots - kLag, was % kSlotsPerScale == kLast, ps + was * NPG / kSlots, pxs);
-          if (was == kSlots - 1 && open != rb) flush();
-        }
+        if (!C::kWhole) add_earlier(t);
         tmem_wait_st();
         tmem_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(full_bar + 8 * (slots & 1));
         ++slots;
-        a_col = a_col == kLag * 32 ? 0 : a_col + 32;
+        a_col = a_col == (C::kASlots - 1) * 32 ? 0 : a_col + 32;
       }
       open = rb;
 #pragma unroll
