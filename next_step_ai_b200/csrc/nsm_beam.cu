@@ -227,7 +227,8 @@ __device__ __forceinline__ void load_block(const T* row, int64_t at, int left, R
 
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kBsThreads, 4) beam_scan_kernel(ScanParams p) {
-  pdl_trigger();
+  pdl_wait();
+  pdl_trigger();  // not before: the merge reads the scores before it waits
   const int lane = threadIdx.x & 31;
   const int64_t unit = (int64_t)blockIdx.x * kBsWarps + (threadIdx.x >> 5);
   const int row = (int)(unit / p.segs), sg = (int)(unit - (int64_t)row * p.segs);
@@ -395,6 +396,46 @@ struct MergeView {
   }
 };
 
+// Cuts a list of more than kBmRank candidates down before they are ranked by counting (which
+// costs their number squared): by the groups' threshold, and if very many scores are equal
+// exactly.
+constexpr int kBmRank = 256;
+__device__ __noinline__ void shrink_list(const MergeView& v, int* count) {
+  MergeShared& sh = v.sh;
+  constexpr int kMine = kBmCap / kBmThreads;
+  u64 key[kMine], id[kMine];
+  const int n = *count;
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int e = i * kBmThreads + threadIdx.x;
+    key[i] = e < n ? sh.key[e] : 0ull;
+    id[i] = e < n ? sh.id[e] : 0ull;
+  }
+  if (threadIdx.x < kBmGroups) sh.group[threadIdx.x] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) put_group(sh, i * kBmThreads + threadIdx.x, key[i]);
+  __syncthreads();
+  u64 ck = (u64)group_threshold(sh, v.mp.k) << 32, cf = ~0ull;
+  for (int exact = 0; exact < 2; ++exact) {
+    if (exact) {
+      kth_best(sh, v.mp.k, [&](auto use) {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+          if (key[i]) use(key[i], id[i]);
+      }, ck, cf);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) *count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+      if (key[i] && (key[i] > ck || (key[i] == ck && id[i] <= cf))) v.append(count, key[i], id[i]);
+    __syncthreads();
+    if (*count <= kBmRank) break;
+  }
+}
+
 // The k best blocks when very many have equal maxima.
 __device__ __noinline__ void entries_again(const MergeView& v) {
   const int n = v.mp.scan.W * (v.mp.scan.entries + 1);
@@ -518,6 +559,7 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(const __grid_
   }
   __syncthreads();
   if (sh.entries_listed > kBmCap) entries_again(view);
+  if (sh.entries_listed > kBmRank) shrink_list(view, &sh.entries_listed);
   const int listed = sh.entries_listed, blocks = min(listed, mp.k);
   rank_list(sh, listed, mp.k, [&](int rank, u64 key, u64 id) {
     sh.best_key[rank] = key;
@@ -588,6 +630,7 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(const __grid_
   }
   __syncthreads();
   if (sh.values_listed > kBmCap) values_again<T>(view, blocks, least);
+  if (sh.values_listed > kBmRank) shrink_list(view, &sh.values_listed);
   const int n = sh.values_listed;
   const int64_t out = (int64_t)b * mp.k;
   rank_list(sh, n, mp.k, [&](int rank, u64 key, u64 id) {
@@ -811,8 +854,7 @@ int nsm_beam_select(const void* logits, int32_t logits_dtype, int64_t batch_stri
   else
     beam_pick<__nv_bfloat16>(vec, &scan, &merge);
   const int64_t warps = (int64_t)rows * pl.segs;
-  scan<<<(unsigned)((warps + kBsWarps - 1) / kBsWarps), kBsThreads, 0, s>>>(sp);
-  NSM_CHECK_CUDA(cudaGetLastError());
+  NSM_CHECK_CUDA(launch_pdl(scan, dim3((unsigned)((warps + kBsWarps - 1) / kBsWarps)), dim3(kBsThreads), 0, s, sp));
   static SmemOnce once[6];
   NSM_CHECK_CUDA(once[logits_dtype * 2 + vec].set(merge, kMergeMaxSmem, di.device));
   NSM_CHECK_CUDA(launch_pdl(merge, dim3(batch), dim3(kBmThreads), pl.merge_smem, s, mp));

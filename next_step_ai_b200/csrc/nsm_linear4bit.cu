@@ -798,7 +798,6 @@ __global__ void __launch_bounds__(kL4BlockRows) lin4_finalize_kernel(const float
                                                                      int ctas, int steps, int max_segs, int cols,
                                                                      int rows, int N, const void* bias, int bias_dt,
                                                                      void* out, int out_dt, int64_t out_stride) {
-  pdl_trigger();
   pdl_wait();
   const int rb = blockIdx.x, r = blockIdx.y, n = rb * kL4BlockRows + threadIdx.x;
   if (n >= N) return;

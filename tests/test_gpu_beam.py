@@ -419,3 +419,16 @@ def test_search_over_the_sparse_mlp_and_nf4_head(dev):
         scores = search.scores.clone()
         hidden = embed[tokens.reshape(-1)]
     assert search.sequences().shape == (B, W, 4)
+
+
+@pytest.mark.parametrize("W,V,k", [(1, 800, 32), (1, 1024, 64), (16, 900, 32), (3, 1500, 64), (32, 500, 64)])
+def test_small_vocabularies(dev, W, V, k):
+    """Fewer blocks of the vocabulary than candidates, with spread and with few values."""
+    from next_step_ai_b200 import beam_select
+
+    x, s, gen = _inputs(3, W, V, FS, dev, V + k)
+    _check(beam_select(x, s, num_candidates=k), x, s, k)
+    x = torch.randint(0, 4, (3, W, V), device=dev, generator=gen).to(FH)
+    s = torch.zeros((3, W), device=dev)
+    same = x[:, :1].expand(3, W, V)
+    _check(beam_select(same, s, num_candidates=k), same, s, k, exact=True)
