@@ -67,8 +67,14 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, num_candidates: i
 _WS_BYTES: dict[tuple[int, int, int, int, int], int] = {}  # by device and sizes
 
 
+_LIB = None
+
+
 def _select(logits, code, scores, fin, B, W, V, k, pad_token, dev):
-    lib = _lib.load()
+    global _LIB
+    lib = _LIB
+    if lib is None:
+        lib = _LIB = _lib.load()
     out_s = torch.empty(B, k, dtype=torch.float32, device=dev)
     out_t = torch.empty(B, k, dtype=torch.int64, device=dev)
     out_p = torch.empty_like(out_t)

@@ -436,35 +436,9 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
   const int u0 = stream_begin(p.units, p.ctas, blockIdx.x), u1 = stream_begin(p.units, p.ctas, blockIdx.x + 1);
   pdl_trigger();
 
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem)),
-                 "r"(kL4Groups * kL4TmemGroup)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  if (threadIdx.x == 32) {
-    for (int g = 0; g < kL4Groups; ++g) {
-      for (int i = 0; i < C::kStages; ++i) mbar_init(smem_u32(&bars.w_full[g][i]), 1);
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(smem_u32(&bars.full[g][i]), 4);  // the group's four warps
-        mbar_init(smem_u32(&bars.done[g][i]), 1);
-      }
-    }
-    for (int i = 0; i < kL4XStages; ++i) {
-      mbar_init(smem_u32(&bars.x_full[i]), 1);
-      mbar_init(smem_u32(&bars.x_free[i]), kL4Groups);
-    }
-    mbar_init_fence();
-  }
-  // Without lin4_prep_kernel in front, nothing in global memory is read or written before the
-  // kernel before this one is done; with it, only x waits (the weights are not its work).
-  if (C::kOwnX) pdl_wait();
-  __syncthreads();
-  int rb = u0 / p.steps, step = u0 - rb * p.steps;
-
   // warps 0-15: the warpgroups; 16-19: one that issues MMAs for each; 20-23: bring the tiles
   const int my_warp = __shfl_sync(0xffffffffu, warp, 0);
-  const bool issuing = my_warp >= 4 * kL4Groups && my_warp < 5 * kL4Groups;
+  const bool issuing = my_warp >= 4 * kL4Groups && my_warp < 5 * kL4Groups, bringing = my_warp >= 5 * kL4Groups;
   const int wg = issuing ? my_warp - 4 * kL4Groups : my_warp >> 2;
   const uint64_t once = l2_evict_first_policy();
   auto copy_weights = [&](int i) {  // lanes 0-3, one for each warpgroup: tile, scales and zero points of unit u0 + i
@@ -480,16 +454,49 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
       if (MODE == kIntZeros) bulk_g2s(dst + kL4TileBytes + C::kScaleBytes, p.z + e, kL4TileRows * NPG, bar, once);
     }
   };
-  if (my_warp >= 5 * kL4Groups) {
-    const int i = my_warp - 5 * kL4Groups;
-    if (i < C::kStages && i < u1 - u0) copy_weights(i);
+  constexpr int kRuns = C::kOwnX ? (NC + 1) / 2 : 1;
+  XRun v[kRuns];  // of a warp that brings x: lanes 0-15 8 columns each of row 2q, lanes 16-31 of row 2q + 1
+  auto load_x = [&](int i) {
+    const int col = (u0 + i) % p.steps * kL4TileCols + 8 * (lane & 15);
+#pragma unroll
+    for (int q = 0; q < kRuns; ++q) v[q].load(p, 2 * q + (lane >> 4), col);
+  };
+
+  // Without lin4_prep_kernel in front, nothing in global memory is read or written before the
+  // kernel before this one is done; with it, only x waits (the weights are not its work).
+  if (C::kOwnX) pdl_wait();
+  if (my_warp == 5 * kL4Groups) {  // the first copies are under way while the rest is set up
+    if (lane == 0) {
+      for (int g = 0; g < kL4Groups; ++g) {
+        for (int i = 0; i < C::kStages; ++i) mbar_init(smem_u32(&bars.w_full[g][i]), 1);
+        for (int i = 0; i < 2; ++i) {
+          mbar_init(smem_u32(&bars.full[g][i]), 4);  // the group's four warps
+          mbar_init(smem_u32(&bars.done[g][i]), 1);
+        }
+      }
+      for (int i = 0; i < kL4XStages; ++i) {
+        mbar_init(smem_u32(&bars.x_full[i]), 1);
+        mbar_init(smem_u32(&bars.x_free[i]), kL4Groups);
+      }
+      mbar_init_fence();
+    }
+    __syncwarp();
+    for (int i = 0; i < min(C::kStages, u1 - u0); ++i) copy_weights(i);
     __syncwarp();
   }
+  if (C::kOwnX && bringing && my_warp - 5 * kL4Groups < u1 - u0) load_x(my_warp - 5 * kL4Groups);
+  if (my_warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem)),
+                 "r"(kL4Groups * kL4TmemGroup)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  int rb = u0 / p.steps, step = u0 - rb * p.steps;
 
   if constexpr (C::kIsCode) {  // byte -> half2 table, one copy per lane (conflict-free); the second holds the remainders
     const float cs = code_scale(p.code);
     uint4* lut4 = reinterpret_cast<uint4*>(smem);
-    for (int i = threadIdx.x; i < 256 * 16; i += kL4Threads) {
+    for (int i = bringing ? 256 * 16 : threadIdx.x; i < 256 * 16; i += kL4Groups * 160) {
       const int e = i >> 4;
       if (MODE == kCode && (i & 8)) continue;
       const float c0 = __ldg(p.code + (e >> 4)) * cs, c1 = __ldg(p.code + (e & 15)) * cs;
@@ -509,7 +516,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
 
   // Every wait is bounded.  One that runs out makes its thread go on without waiting, and
   // leaves NaN in the warpgroup's partials.
-  if (my_warp >= 5 * kL4Groups) {
+  if (bringing) {
     // ---- tiles: each of these warps fills one place of x's ring, and when all MMAs that read it
     // are done, so that all warpgroups have read their weights of that unit too, the place of those
     const int st = my_warp - 5 * kL4Groups, count = u1 - u0;
@@ -517,22 +524,13 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
     unsigned char* dst = smem + C::kX + st * C::kXBytes;
     const uint64_t keep = l2_evict_last_policy();
     const float icode = C::kOwnX && C::kIsCode ? 1.f / code_scale(p.code) : 1.f;  // a power of two
-    constexpr int kRuns = C::kOwnX ? (NC + 1) / 2 : 1;
     bool ok = true;
-    int w_last = st < min(C::kStages, count) ? st : -1;  // the last unit whose weights it brought
+    int w_last = st < min(C::kStages, count) ? st : -1;  // the last unit of this place whose weights were asked for
     if (!C::kOwnX) {
       pdl_wait();
       fence_proxy_async_global();
     }
     for (int i = st; i < count + kL4XStages - C::kStages; i += kL4XStages) {
-      const int step_i = (u0 + i) % p.steps;
-      XRun v[kRuns];  // lanes 0-15: 8 columns each of row 2q, lanes 16-31: of row 2q + 1
-      if constexpr (C::kOwnX) {
-        if (i < count) {
-#pragma unroll
-          for (int q = 0; q < kRuns; ++q) v[q].load(p, 2 * q + (lane >> 4), step_i * kL4TileCols + 8 * (lane & 15));
-        }
-      }
       if (i >= kL4XStages) {
         ok = mbar_wait(free, (i / kL4XStages - 1) & 1, p.wait_limit);
         if (!__all_sync(0xffffffffu, ok)) {
@@ -567,9 +565,10 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(full);
+        if (i + kL4XStages < count) load_x(i + kL4XStages);
       } else if (lane == 0) {
         mbar_arrive_expect_tx(full, C::kXBytes);
-        bulk_g2s(smem_u32(dst), reinterpret_cast<const unsigned char*>(p.xh) + (int64_t)step_i * C::kXBytes, C::kXBytes, full,
+        bulk_g2s(smem_u32(dst), reinterpret_cast<const unsigned char*>(p.xh) + (int64_t)((u0 + i) % p.steps) * C::kXBytes, C::kXBytes, full,
                  keep);
       }
     }
