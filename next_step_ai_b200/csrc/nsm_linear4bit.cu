@@ -132,8 +132,12 @@ __global__ void lin4_pack_scales_kernel(const void* __restrict__ scales, int dt,
 }
 
 // ---- activations ----------------------------------------------------------------
-// Power of two that brings the largest |code| to [64, 128): the remainders of the
+// Power of two that brings the largest |code| (m) to [64, 128): the remainders of the
 // exact codebook then stay normal fp16 numbers.
+__device__ __forceinline__ float code_scale_of(float m) {
+  if (!(m > 0.f)) return 1.f;
+  return ldexpf(1.f, max(-120, min(120, 6 - ilogbf(m))));
+}
 __device__ __forceinline__ float code_scale(const float* code) {
   float m = 0.f;
 #pragma unroll
@@ -141,8 +145,15 @@ __device__ __forceinline__ float code_scale(const float* code) {
     const float a = fabsf(__ldg(code + i));
     if (a <= 3.4e38f) m = fmaxf(m, a);
   }
-  if (!(m > 0.f)) return 1.f;
-  return ldexpf(1.f, max(-120, min(120, 6 - ilogbf(m))));
+  return code_scale_of(m);
+}
+
+// The power of two (and its reciprocal) that brings m, the largest of some values, to [2^14,
+// 2^15), from its exponent bits; m below 2^-111 (0 too) is left smaller.
+__device__ __forceinline__ float x_scale_for(float m, float& inv) {
+  const int e = max(16, min(240, (int)(__float_as_uint(m) >> 23)));
+  inv = __uint_as_float((uint32_t)(268 - e) << 23);
+  return __uint_as_float((uint32_t)(e - 14) << 23);
 }
 
 // Halves of column c of x, column k of the weight: [tile][k / 8][c / 8][c % 8][k % 8].
@@ -162,7 +173,7 @@ __global__ void __launch_bounds__(256) lin4_prep_kernel(const void* x, int dt, i
   const int es = dt == NSM_F32 ? 4 : 2;
   const char* row = static_cast<const char*>(x) + base * es;
   const bool vec = ((uintptr_t)row & 15) == 0;
-  float s = 1.f;
+  float s = 1.f, inv = 1.f;
   auto finite = [](float v) {  // infinities and NaN stay what they are
     const float a = fabsf(v);
     return a <= 3.4028234e38f ? a : 0.f;
@@ -187,10 +198,8 @@ __global__ void __launch_bounds__(256) lin4_prep_kernel(const void* x, int dt, i
     m = warp_max(m);
     if ((threadIdx.x & 31) == 0) wmax[threadIdx.x >> 5] = m;
     __syncthreads();
-    m = warp_max(wmax[threadIdx.x & 7]);
-    if (m > 0.f) s = ldexpf(1.f, max(-120, min(120, ilogbf(m) - 14)));
+    s = x_scale_for(warp_max(wmax[threadIdx.x & 7]), inv);
   }
-  const float inv = 1.f / s;  // a power of two: exact
   const int runs = kp / 8;
   for (int q = blockIdx.x * 256 + threadIdx.x; q < runs; q += gridDim.x * 256) {
     __half hi[8], lo[8];
@@ -358,7 +367,8 @@ struct XRun {
     }
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float s = m > 0.f ? ldexpf(1.f, max(-120, min(120, ilogbf(m) - 14))) : 1.f, inv = 1.f / s;
+    float inv;
+    const float s = x_scale_for(m, inv);
     __half h[8], l[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -441,12 +451,12 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
   const bool issuing = my_warp >= 4 * kL4Groups && my_warp < 5 * kL4Groups, bringing = my_warp >= 5 * kL4Groups;
   const int wg = issuing ? my_warp - 4 * kL4Groups : my_warp >> 2;
   const uint64_t once = l2_evict_first_policy();
-  auto copy_weights = [&](int i) {  // lanes 0-3, one for each warpgroup: tile, scales and zero points of unit u0 + i
+  auto copy_weights = [&](int i, int g) {  // a lane's: tile, scales and zero points of unit u0 + i, warpgroup g
     const int at_rb = (u0 + i) / p.steps, at = u0 + i - at_rb * p.steps;
-    const int64_t rt = (int64_t)at_rb * kL4Groups + lane;
-    if (lane < kL4Groups && rt < p.row_tiles) {
-      const uint32_t bar = smem_u32(&bars.w_full[lane][i % C::kStages]);
-      const uint32_t dst = smem_u32(smem + C::kRing + (lane * C::kStages + i % C::kStages) * C::kStageBytes);
+    const int64_t rt = (int64_t)at_rb * kL4Groups + g;
+    if (rt < p.row_tiles) {
+      const uint32_t bar = smem_u32(&bars.w_full[g][i % C::kStages]);
+      const uint32_t dst = smem_u32(smem + C::kRing + (g * C::kStages + i % C::kStages) * C::kStageBytes);
       const int64_t e = (rt * p.scale_steps + ((NPG == 1 && p.div > 1) ? at / p.div : at)) * (kL4TileRows * NPG);
       mbar_arrive_expect_tx(bar, C::kStageBytes);
       bulk_g2s(dst, p.w + (rt * p.steps + at) * kL4TileBytes, kL4TileBytes, bar, once);
@@ -466,22 +476,13 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
   // kernel before this one is done; with it, only x waits (the weights are not its work).
   if (C::kOwnX) pdl_wait();
   if (my_warp == 5 * kL4Groups) {  // the first copies are under way while the rest is set up
-    if (lane == 0) {
-      for (int g = 0; g < kL4Groups; ++g) {
-        for (int i = 0; i < C::kStages; ++i) mbar_init(smem_u32(&bars.w_full[g][i]), 1);
-        for (int i = 0; i < 2; ++i) {
-          mbar_init(smem_u32(&bars.full[g][i]), 4);  // the group's four warps
-          mbar_init(smem_u32(&bars.done[g][i]), 1);
-        }
-      }
-      for (int i = 0; i < kL4XStages; ++i) {
-        mbar_init(smem_u32(&bars.x_full[i]), 1);
-        mbar_init(smem_u32(&bars.x_free[i]), kL4Groups);
-      }
-      mbar_init_fence();
-    }
+    // the barriers in the order of Lin4Bars, and what they count
+    constexpr int kFull = kL4Groups * 4, kDone = kFull + kL4Groups * 2, kXFree = kDone + kL4Groups * 2 + kL4XStages;
+    for (int i = lane; i < kXFree + kL4XStages; i += 32)
+      mbar_init(smem_u32(&bars) + 8 * i, i >= kXFree ? kL4Groups : i >= kFull && i < kDone ? 4 : 1);
+    mbar_init_fence();
     __syncwarp();
-    for (int i = 0; i < min(C::kStages, u1 - u0); ++i) copy_weights(i);
+    if (lane < kL4Groups * C::kStages && lane / kL4Groups < u1 - u0) copy_weights(lane / kL4Groups, lane % kL4Groups);
     __syncwarp();
   }
   if (C::kOwnX && bringing && my_warp - 5 * kL4Groups < u1 - u0) load_x(my_warp - 5 * kL4Groups);
@@ -493,20 +494,20 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
   }
   int rb = u0 / p.steps, step = u0 - rb * p.steps;
 
-  if constexpr (C::kIsCode) {  // byte -> half2 table, one copy per lane (conflict-free); the second holds the remainders
-    const float cs = code_scale(p.code);
+  if (C::kIsCode && !bringing) {  // byte -> half2 table, one copy per lane (conflict-free); the second holds the remainders
+    const float code = __ldg(p.code + (lane & 15));
+    const float mine = fabsf(code) <= 3.4e38f ? fabsf(code) : 0.f;
+    const float scaled = code * code_scale_of(warp_max(mine));
     uint4* lut4 = reinterpret_cast<uint4*>(smem);
-    for (int i = bringing ? 256 * 16 : threadIdx.x; i < 256 * 16; i += kL4Groups * 160) {
-      const int e = i >> 4;
-      if (MODE == kCode && (i & 8)) continue;
-      const float c0 = __ldg(p.code + (e >> 4)) * cs, c1 = __ldg(p.code + (e & 15)) * cs;
+    for (int e = my_warp; e < 256; e += kL4Groups * 5) {  // a warp per byte: 8 lanes fill a table's 32 words
+      const float c0 = __shfl_sync(0xffffffffu, scaled, e >> 4), c1 = __shfl_sync(0xffffffffu, scaled, e & 15);
       __half h0 = __float2half_rn(c0), h1 = __float2half_rn(c1);
-      if (i & 8) {
+      if (lane & 8) {
         h0 = __float2half_rn(c0 - __half2float(h0));
         h1 = __float2half_rn(c1 - __half2float(h1));
       }
       const uint32_t v = (uint32_t)__half_as_ushort(h0) | ((uint32_t)__half_as_ushort(h1) << 16);
-      lut4[i] = make_uint4(v, v, v, v);
+      if (lane < (MODE == kCodeExact ? 16 : 8)) lut4[e * 16 + lane] = make_uint4(v, v, v, v);
     }
   }
   tmem_fence_before();
@@ -540,7 +541,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
         const int j = i - kL4XStages + C::kStages;
         if (j < count) {
           fence_proxy_async_smem();
-          copy_weights(j);
+          if (lane < kL4Groups) copy_weights(j, lane);
           w_last = j;
           __syncwarp();
         }
@@ -793,24 +794,38 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kL4Groups * kL4TmemGroup) : "memory");
 }
 
+// kShare threads share the segments of an output (their loads are under way together), and
+// their sums are added in order: the same bits every time.  Four where an output has more than
+// four segments and the threads of all outputs fit the GPU at once (4096 outputs of one row: 3.7
+// -> 1.5 us), else one (16384 outputs of 32 rows would take 10 us more with four).
+template <int kShare>
 __global__ void __launch_bounds__(kL4BlockRows) lin4_finalize_kernel(const float* part, const float* scale, int units,
-                                                                     int ctas, int steps, int max_segs, int cols,
-                                                                     int rows, int N, const void* bias, int bias_dt,
-                                                                     void* out, int out_dt, int64_t out_stride) {
-  pdl_wait();
-  const int rb = blockIdx.x, r = blockIdx.y, n = rb * kL4BlockRows + threadIdx.x;
-  if (n >= N) return;
+                                                                       int ctas, int steps, int max_segs, int cols,
+                                                                       int rows, int N, const void* bias, int bias_dt,
+                                                                       void* out, int out_dt, int64_t out_stride) {
+  constexpr int kRows = kL4BlockRows / kShare;
+  __shared__ float sums[kShare][kRows];
+  const int i = threadIdx.x % kRows, q = threadIdx.x / kRows;
+  const int n = blockIdx.x * kRows + i, rb = n / kL4BlockRows, r = blockIdx.y;
   const int first = stream_owner(units, ctas, rb * steps);
   const int segs = stream_owner(units, ctas, (rb + 1) * steps - 1) - first + 1;
-  const float* src = part + ((int64_t)rb * max_segs * cols + r) * kL4BlockRows + threadIdx.x;
+  pdl_wait();
+  const float* src = part + ((int64_t)rb * max_segs * cols + r) * kL4BlockRows + n % kL4BlockRows;
   float v = 0.f;
-#pragma unroll 4
-  for (int k = 0; k < segs; ++k) {
-    const float* q = src + (int64_t)k * cols * kL4BlockRows;
-    float e = __ldcg(q);
-    if (cols > rows) e += __ldcg(q + (int64_t)rows * kL4BlockRows);  // the remainders of an fp32 x
+#pragma unroll 8
+  for (int k = q; k < segs; k += kShare) {
+    const float* at = src + (int64_t)k * cols * kL4BlockRows;
+    float e = __ldcg(at);
+    if (cols > rows) e += __ldcg(at + (int64_t)rows * kL4BlockRows);  // the remainders of an fp32 x
     v += e;
   }
+  if constexpr (kShare > 1) {
+    sums[q][i] = v;
+    __syncthreads();
+#pragma unroll
+    for (int j = 1; j < kShare; ++j) v += sums[j][i];
+  }
+  if (q != 0 || n >= N) return;
   if (scale) v *= __ldcg(scale + r);
   if (bias) v += load_as_f32(bias, bias_dt, n);
   store_from_f32(out, out_dt, (int64_t)r * out_stride + n, v);
@@ -1001,8 +1016,11 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
   p.max_segs = pl.max_segs;
   p.wait_limit = copy_wait_spins();
   NSM_CHECK_CUDA(launch_pdl(f.fn, dim3(pl.ctas), dim3(kL4Threads), (size_t)f.smem, s, p));
-  NSM_CHECK_CUDA(launch_pdl(lin4_finalize_kernel, dim3(sh.row_blocks, rows), dim3(kL4BlockRows), 0, s,
-                            (const float*)part, (const float*)(pl.own_x ? nullptr : scale), pl.units, pl.ctas, sh.steps, pl.max_segs, pl.cols,
+  const int share = pl.max_segs > 4 && 4LL * sh.N * rows <= 2048LL * di.sm_count ? 4 : 1;
+  const int fin_rows = kL4BlockRows / share;
+  NSM_CHECK_CUDA(launch_pdl(share == 4 ? lin4_finalize_kernel<4> : lin4_finalize_kernel<1>,
+                            dim3((sh.N + fin_rows - 1) / fin_rows, rows), dim3(kL4BlockRows), 0, s, (const float*)part,
+                            (const float*)(pl.own_x ? nullptr : scale), pl.units, pl.ctas, sh.steps, pl.max_segs, pl.cols,
                             (int)rows, sh.N, w->bias, (int)w->bias_dtype, out, (int)out_dtype, out_row_stride));
   return NSM_OK;
 }
