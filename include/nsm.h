@@ -521,11 +521,14 @@ int nsm_lm_head_nf4(const void* x, int32_t x_dtype, int32_t tokens, const uint8_
  *
  * x rows are x_row_stride elements apart, out rows out_row_stride (each row
  * contiguous).  x, bias and out may be fp32 / fp16 / bf16.  Accumulation is
- * fp32; x enters as fp16 scaled by a power of two per row (fp32 x as value +
- * remainder), the codebook as fp16 for fp16 / bf16 outputs and to 22 bits for
- * fp32 ones.  Results do not depend on the other rows of the call and are the
- * same bits every time.  The workspace needs no initialisation; calls that
- * share one must not overlap on the GPU. */
+ * fp32; x enters as fp16 scaled by a power of two (fp32 x as value + remainder):
+ * bf16 is exact down to 2^-31 of the row's largest value, smaller ones are off by
+ * at most 2^-39 of it.  The codebook enters as fp16 for fp16 / bf16 outputs and
+ * to 22 bits for fp32 ones.  A result does not depend on the other rows of the
+ * call and has the same bits every time (and for any number of rows, but for x's
+ * values below that border).  The workspace needs no initialisation; calls that
+ * share one must not overlap on the GPU.  A wait inside the kernel that runs out
+ * (nsm_set_copy_wait_limit) leaves NaN in the outputs it concerns. */
 typedef struct nsm_linear4bit_weights {
   const uint8_t* packed; /* tiled, from nsm_linear4bit_pack */
   const float* scales;   /* tiled */
@@ -562,7 +565,8 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
  * are not read.  finished [batch][beams] (bytes, may be NULL): a finished beam is one
  * candidate, pad_token at its own score; its logits are not read either.  A logit
  * of -infinity or NaN is no candidate; +infinity counts as the largest finite
- * value.  Sums and scores are compared in 64 bits.  Outputs [batch]
+ * value.  The logsumexp is taken from fp32 sums (equal rows give equal bits); scores
+ * are formed and compared in 64 bits.  Outputs [batch]
  * [candidates]: scores, tokens and parents (the beam w); where fewer candidates
  * exist, score -infinity, token -1, parent 0.  1..32 beams, 1..64 candidates.  The
  * workspace needs no initialisation. */
@@ -575,7 +579,7 @@ int nsm_beam_select(const void* logits, int32_t logits_dtype, int64_t batch_stri
 /* One per-beam state: row b * beams + w (row_stride bytes apart) holds outer0 x
  * outer1 runs of run_bytes contiguous bytes.  With position_bytes > 0 a run is
  * `positions` entries of that size (a cache's or a history's positions), of which
- * a call may move the first `length` only.  Rows must not overlap. */
+ * a call may move the first `length` only.  Neither rows nor states may overlap. */
 typedef struct nsm_beam_state {
   void* data;
   int64_t row_stride;

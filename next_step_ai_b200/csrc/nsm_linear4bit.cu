@@ -13,27 +13,34 @@
 //
 // Two or three launches, linked by programmatic dependent launch:
 //  1. for more than 8 columns of x, lin4_prep_kernel: per row of x a power-of-two scale that
-//     brings the largest finite |x| to [2^14, 2^15) and x as fp16 (exact for fp16, and for bf16
-//     down to 2^-38 of the row's largest); an fp32 x becomes two fp16 columns
-//     (value and remainder, 22 bits).  x is written as the 8 x 16-byte core matrices of a
-//     K-major tensor-core operand.  For up to 8 columns lin4_kernel does this itself, with a
-//     scale for each 128 columns of a row: one launch and 5 us less at 16384 columns;
+//     brings the largest finite |x| to [2^14, 2^15), and x as fp16: exact for fp16, for bf16 exact
+//     down to 2^-31 of the row's largest value (below that off by at most 2^-39 of it); an
+//     fp32 x becomes two fp16 columns, value and remainder: 22 bits.  x is written as the 8 x
+//     16-byte core matrices of a K-major tensor-core operand.  For up to 8 columns lin4_kernel
+//     does this itself, with a scale for each 128 columns of a row: one launch and 5 us less at
+//     16384 columns;
 //  2. lin4_kernel: one CTA per SM, four warpgroups of 128 rows each.  A unit is 512 rows x
 //     128 columns; the units, row block by row block, are cut into equal contiguous runs,
 //     one per CTA, so no CTA finishes late.  Bulk copies bring each warpgroup's tile and
 //     scales into its own ring, and x into a ring that all share.  A warpgroup turns its
 //     tile into fp16 (a byte -> half2 table for codebooks, mask and subtract for
 //     integers: both exact but for the codebook's rounding) and stores it to tensor
-//     memory, 64 columns at a time in two slots; a warp of its own multiplies them with x
-//     (tcgen05.mma, M = 128 rows, N = the columns of x, fp32 accumulation) while the
-//     warpgroup works on the next slot, and then the warpgroup adds scale * product to
-//     its fp32 sums in registers.  With weights as the M operand in tensor memory x never
-//     passes through registers: one row of x or 32 cost the threads the same but for the sums.
-//     Each CTA leaves one fp32 partial per row block that it touched;
-//  3. lin4_finalize_kernel: the partials of a row block in CTA order (the same
+//     memory; a warp of its own multiplies it with x (tcgen05.mma, M = 128 rows, N = the
+//     columns of x, fp32 accumulation), and then the warpgroup adds scale * product to its
+//     fp32 sums in registers, after it has converted what comes next.  With weights as the M
+//     operand in tensor memory x never passes through registers: one row of x or 32 cost the
+//     threads the same but for the sums.  Each CTA leaves one fp32 partial per row block that it
+//     touched;
+//  3. lin4_finalize_kernel: the partials of a row block in a fixed order (the same
 //     bits every time), times the scale of x, + bias, in the output's type.
+//
+// Measured, 16384 x 16384 with weights larger than L2: NF4, one row of x in bf16, 32 us; integers
+// with groups of 128, 30 us for one row and 44 us for 32.  In its steady state a unit of NF4
+// takes 0.94 us and one of integers 0.88 us with 32 rows, 85% and 87% of the copy bandwidth; the
+// rest is a start of 3 us, the last CTAs' tail with the partials (3 us), and prep.  Where an
+// fp32 output keeps the codebook to 22 bits, the two table reads per byte from shared memory
+// bound a unit at 1.64 us (48 us in all).
 #include <algorithm>
-#include <mutex>
 
 #include "nsm_common.cuh"
 #include "nsm_internal.h"
@@ -149,12 +156,75 @@ __device__ __forceinline__ float code_scale(const float* code) {
 }
 
 // The power of two (and its reciprocal) that brings m, the largest of some values, to [2^14,
-// 2^15), from its exponent bits; m below 2^-111 (0 too) is left smaller.
+// 2^15), from its exponent bits; m below 2^-111 (0 too) is left smaller.  m is finite.
 __device__ __forceinline__ float x_scale_for(float m, float& inv) {
-  const int e = max(16, min(240, (int)(__float_as_uint(m) >> 23)));
+  const int e = max(16, (int)(__float_as_uint(m) >> 23));
   inv = __uint_as_float((uint32_t)(268 - e) << 23);
   return __uint_as_float((uint32_t)(e - 14) << 23);
 }
+
+// Eight columns of a row of x on their way to an operand tile.
+struct XRun {
+  uint32_t r[8];  // fp32 values, or four words of 16-bit pairs
+  __device__ __forceinline__ void load(const void* x, int dtype, int64_t stride, int rows, int K, int row, int col) {
+    const int es = dtype == NSM_F32 ? 4 : 2;
+    const char* at = static_cast<const char*>(x) + ((int64_t)row * stride + col) * es;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = 0;
+    if (row >= rows || col >= K) return;
+    if (((uintptr_t)at & 15) == 0 && col + 8 <= K) {
+      const uint4 a = *reinterpret_cast<const uint4*>(at);
+      r[0] = a.x, r[1] = a.y, r[2] = a.z, r[3] = a.w;
+      if (es == 4) {
+        const uint4 b = *reinterpret_cast<const uint4*>(at + 16);
+        r[4] = b.x, r[5] = b.y, r[6] = b.z, r[7] = b.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (col + i < K) {
+          if (es == 4) {
+            r[i] = reinterpret_cast<const uint32_t*>(at)[i];
+          } else {
+            r[i / 2] |= (uint32_t) reinterpret_cast<const unsigned short*>(at)[i] << (16 * (i % 2));
+          }
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ float value(int dtype, int i) const {  // fp32 or bf16
+    return dtype == NSM_F32 ? __uint_as_float(r[i]) : __uint_as_float(i % 2 ? r[i / 2] & 0xffff0000u : r[i / 2] << 16);
+  }
+  __device__ __forceinline__ float largest(int dtype) const {  // infinities and NaN stay what they are
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float a = fabsf(value(dtype, i));
+      m = fmaxf(m, a <= 3.4028234e38f ? a : 0.f);
+    }
+    return m;
+  }
+  // As fp16 (and, for fp32, the remainders), times inv, a power of two.
+  __device__ __forceinline__ void to_half(int dtype, float inv, uint4& hi, uint4& lo) const {
+    if (dtype == NSM_F16) {
+      hi = make_uint4(r[0], r[1], r[2], r[3]);
+      return;
+    }
+    __half h[8], l[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = value(dtype, i) * inv;
+      h[i] = __float2half_rn(x);
+      const float rem = x - __half2float(h[i]);
+      l[i] = __float2half_rn(fabsf(rem) <= 3.4028234e38f ? rem : 0.f);
+    }
+    auto pair = [](const __half* q, int i) {
+      return (uint32_t)__half_as_ushort(q[2 * i]) | ((uint32_t)__half_as_ushort(q[2 * i + 1]) << 16);
+    };
+    hi = make_uint4(pair(h, 0), pair(h, 1), pair(h, 2), pair(h, 3));
+    if (dtype == NSM_F32) lo = make_uint4(pair(l, 0), pair(l, 1), pair(l, 2), pair(l, 3));
+  }
+};
 
 // Halves of column c of x, column k of the weight: [tile][k / 8][c / 8][c % 8][k % 8].
 __device__ __forceinline__ int64_t x_index(int c, int k, int groups) {
@@ -168,51 +238,28 @@ __global__ void __launch_bounds__(256) lin4_prep_kernel(const void* x, int dt, i
                                                         int groups, const float* code, __half* xh, float* scale) {
   pdl_trigger();
   __shared__ float wmax[8];
-  const int r = blockIdx.y;
-  const int64_t base = (int64_t)r * stride;
-  const int es = dt == NSM_F32 ? 4 : 2;
-  const char* row = static_cast<const char*>(x) + base * es;
-  const bool vec = ((uintptr_t)row & 15) == 0;
+  const int r = blockIdx.y, runs = kp / 8;
   float s = 1.f, inv = 1.f;
-  auto finite = [](float v) {  // infinities and NaN stay what they are
-    const float a = fabsf(v);
-    return a <= 3.4028234e38f ? a : 0.f;
-  };
   if (dt != NSM_F16) {
     float m = 0.f;
-    const int per = 16 / es, nv = vec ? K / per : 0;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < nv; i += 256) {
-      const uint4 q = ldg_u4(row + 16 * (int64_t)i);
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (dt == NSM_F32) {
-          m = fmaxf(m, finite(__uint_as_float(w[j])));
-        } else {
-          m = fmaxf(m, fmaxf(finite(__uint_as_float(w[j] << 16)), finite(__uint_as_float(w[j] & 0xffff0000u))));
-        }
-      }
+    for (int q = threadIdx.x; q < runs; q += 256) {
+      XRun v;
+      v.load(x, dt, stride, rows, K, r, 8 * q);
+      m = fmaxf(m, v.largest(dt));
     }
-    for (int k = nv * per + threadIdx.x; k < K; k += 256) m = fmaxf(m, finite(load_as_f32(x, dt, base + k)));
     m = warp_max(m);
     if ((threadIdx.x & 31) == 0) wmax[threadIdx.x >> 5] = m;
     __syncthreads();
     s = x_scale_for(warp_max(wmax[threadIdx.x & 7]), inv);
   }
-  const int runs = kp / 8;
   for (int q = blockIdx.x * 256 + threadIdx.x; q < runs; q += gridDim.x * 256) {
-    __half hi[8], lo[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int k = 8 * q + j;
-      const float v = k < K ? load_as_f32(x, dt, base + k) * inv : 0.f;
-      hi[j] = __float2half_rn(v);
-      const float rem = v - __half2float(hi[j]);
-      lo[j] = __float2half_rn(fabsf(rem) <= 3.4028234e38f ? rem : 0.f);
-    }
-    *reinterpret_cast<uint4*>(xh + x_index(r, 8 * q, groups)) = *reinterpret_cast<const uint4*>(hi);
-    if (dt == NSM_F32) *reinterpret_cast<uint4*>(xh + x_index(rows + r, 8 * q, groups)) = *reinterpret_cast<const uint4*>(lo);
+    XRun v;
+    v.load(x, dt, stride, rows, K, r, 8 * q);
+    uint4 hi, lo;
+    v.to_half(dt, inv, hi, lo);
+    *reinterpret_cast<uint4*>(xh + x_index(r, 8 * q, groups)) = hi;
+    if (dt == NSM_F32) *reinterpret_cast<uint4*>(xh + x_index(rows + r, 8 * q, groups)) = lo;
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) scale[r] = code ? s / code_scale(code) : s;
 }
@@ -322,70 +369,6 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// Eight columns of a row of x on their way to an operand tile.
-struct XRun {
-  uint32_t r[8];  // fp32 values, or four words of 16-bit pairs
-  __device__ __forceinline__ void load(const Lin4Params& p, int row, int col) {
-    const int es = p.x_dtype == NSM_F32 ? 4 : 2;
-    const char* at = static_cast<const char*>(p.x) + ((int64_t)row * p.x_stride + col) * es;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = 0;
-    if (row >= p.rows || col >= p.K) return;
-    if (((uintptr_t)at & 15) == 0 && col + 8 <= p.K) {
-      const uint4 a = *reinterpret_cast<const uint4*>(at);
-      r[0] = a.x, r[1] = a.y, r[2] = a.z, r[3] = a.w;
-      if (es == 4) {
-        const uint4 b = *reinterpret_cast<const uint4*>(at + 16);
-        r[4] = b.x, r[5] = b.y, r[6] = b.z, r[7] = b.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (col + i < p.K) {
-          if (es == 4) {
-            r[i] = reinterpret_cast<const uint32_t*>(at)[i];
-          } else {
-            r[i / 2] |= (uint32_t) reinterpret_cast<const unsigned short*>(at)[i] << (16 * (i % 2));
-          }
-        }
-      }
-    }
-  }
-  // As fp16 (and, for fp32, the remainders), divided by the returned power of two, which
-  // brings the largest finite value of the half-warp's 128 columns to [2^14, 2^15).
-  __device__ __forceinline__ float to_half(int dtype, uint4& hi, uint4& lo) const {
-    if (dtype == NSM_F16) {
-      hi = make_uint4(r[0], r[1], r[2], r[3]);
-      return 1.f;
-    }
-    float v[8], m = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = dtype == NSM_F32 ? __uint_as_float(r[i]) : __uint_as_float(i % 2 ? r[i / 2] & 0xffff0000u : r[i / 2] << 16);
-      const float a = fabsf(v[i]);
-      m = fmaxf(m, a <= 3.4028234e38f ? a : 0.f);  // infinities and NaN stay what they are
-    }
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float inv;
-    const float s = x_scale_for(m, inv);
-    __half h[8], l[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float x = v[i] * inv;
-      h[i] = __float2half_rn(x);
-      const float rem = x - __half2float(h[i]);
-      l[i] = __float2half_rn(fabsf(rem) <= 3.4028234e38f ? rem : 0.f);
-    }
-    auto pair = [](const __half* q, int i) {
-      return (uint32_t)__half_as_ushort(q[2 * i]) | ((uint32_t)__half_as_ushort(q[2 * i + 1]) << 16);
-    };
-    hi = make_uint4(pair(h, 0), pair(h, 1), pair(h, 2), pair(h, 3));
-    if (dtype == NSM_F32) lo = make_uint4(pair(l, 0), pair(l, 1), pair(l, 2), pair(l, 3));
-    return s;
-  }
-};
-
 // What a kernel variant holds, for device and host.  NPG: scale granules per tile of 128
 // columns.  NC: columns of x that the sums hold.
 template <int MODE, int NPG, int NC>
@@ -424,6 +407,8 @@ struct Lin4Bars {
   unsigned long long done[kL4Groups][2];    // its MMAs are done
   unsigned long long x_full[kL4XStages];    // a tile of x is in shared memory
   unsigned long long x_free[kL4XStages];    // all warpgroups' MMAs that read it are done
+  unsigned long long drained[kL4Groups];    // all of the warpgroup's MMAs are done
+  unsigned long long dead[2];               // where a warp arrives instead of at `full` after a failure
   float x_scale[kL4XStages][8];             // kOwnX: what a tile's columns of x were divided by
   uint32_t tmem;
 };
@@ -469,7 +454,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
   auto load_x = [&](int i) {
     const int col = (u0 + i) % p.steps * kL4TileCols + 8 * (lane & 15);
 #pragma unroll
-    for (int q = 0; q < kRuns; ++q) v[q].load(p, 2 * q + (lane >> 4), col);
+    for (int q = 0; q < kRuns; ++q) v[q].load(p.x, p.x_dtype, p.x_stride, p.rows, p.K, 2 * q + (lane >> 4), col);
   };
 
   // Without lin4_prep_kernel in front, nothing in global memory is read or written before the
@@ -478,8 +463,9 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
   if (my_warp == 5 * kL4Groups) {  // the first copies are under way while the rest is set up
     // the barriers in the order of Lin4Bars, and what they count
     constexpr int kFull = kL4Groups * 4, kDone = kFull + kL4Groups * 2, kXFree = kDone + kL4Groups * 2 + kL4XStages;
-    for (int i = lane; i < kXFree + kL4XStages; i += 32)
-      mbar_init(smem_u32(&bars) + 8 * i, i >= kXFree ? kL4Groups : i >= kFull && i < kDone ? 4 : 1);
+    constexpr int kDrained = kXFree + kL4XStages;
+    for (int i = lane; i < kDrained + kL4Groups + 2; i += 32)
+      mbar_init(smem_u32(&bars) + 8 * i, i >= kXFree && i < kDrained ? kL4Groups : i >= kFull && i < kDone ? 4 : 1);
     mbar_init_fence();
     __syncwarp();
     if (lane < kL4Groups * C::kStages && lane / kL4Groups < u1 - u0) copy_weights(lane / kL4Groups, lane % kL4Groups);
@@ -515,8 +501,9 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
   tmem_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, bars.tmem, 0);
 
-  // Every wait is bounded.  One that runs out makes its thread go on without waiting, and
-  // leaves NaN in the warpgroup's partials.
+  // Every wait is bounded.  After one that ran out nothing more is copied, multiplied or handed
+  // on, so the waits that depend on it run out too, and the warpgroups that saw one leave NaN in
+  // their partials.  Copies and MMAs under way are waited for before the CTA ends.
   if (bringing) {
     // ---- tiles: each of these warps fills one place of x's ring, and when all MMAs that read it
     // are done, so that all warpgroups have read their weights of that unit too, the place of those
@@ -527,6 +514,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
     const float icode = C::kOwnX && C::kIsCode ? 1.f / code_scale(p.code) : 1.f;  // a power of two
     bool ok = true;
     int w_last = st < min(C::kStages, count) ? st : -1;  // the last unit of this place whose weights were asked for
+    int x_last = -1;                                     // and the last round of x
     if (!C::kOwnX) {
       pdl_wait();
       fence_proxy_async_global();
@@ -547,12 +535,20 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
         }
       }
       if (i >= count) break;
+      x_last = i / kL4XStages;
       if constexpr (C::kOwnX) {
 #pragma unroll
         for (int q = 0; q < kRuns; ++q) {
           const int r = 2 * q + (lane >> 4);
           uint4 hi, lo;
-          const float s = v[q].to_half(p.x_dtype, hi, lo);
+          float s = 1.f, inv = 1.f;
+          if (p.x_dtype != NSM_F16) {  // a scale for the row's 128 columns: the half-warp's
+            float m = v[q].largest(p.x_dtype);
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            s = x_scale_for(m, inv);
+          }
+          v[q].to_half(p.x_dtype, inv, hi, lo);
           if (r < p.rows) {
             // core matrices of 8 columns of x by 8 of the weight: [k / 8][c][k % 8]
             *reinterpret_cast<uint4*>(dst + ((lane & 15) * 8 + r) * 16) = hi;
@@ -575,13 +571,12 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
     }
     // Nothing may arrive in shared memory that is gone: the last commits (they come after the
     // copies they waited for), and after a failure the copies under way.
-    const int last = count > st ? (count - 1 - st) / kL4XStages : -1;  // this place's last round
-    if (lane == 0 && last >= 0 && ok) ok = mbar_wait(free, last & 1, p.wait_limit);
+    if (lane == 0 && x_last >= 0 && ok) ok = mbar_wait(free, x_last & 1, p.wait_limit);
     ok = __shfl_sync(0xffffffffu, ok, 0);
     if (!ok) {
       if (lane < kL4Groups && w_last >= 0 && (u0 + w_last) / p.steps * kL4Groups + lane < p.row_tiles)
         mbar_wait(smem_u32(&bars.w_full[lane][w_last % C::kStages]), (w_last / C::kStages) & 1);
-      if (!C::kOwnX && lane == 0) mbar_wait(full, last & 1);
+      if (!C::kOwnX && lane == 0 && x_last >= 0) mbar_wait(full, x_last & 1);
     }
     __syncwarp();
   } else if (issuing) {
@@ -593,7 +588,8 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
     uint32_t a_col = 0, d_col = C::kD;    // of this round
     for (int u = u0; u < u1; ++u) {
       const uint32_t xfree = smem_u32(&bars.x_free[xst]);
-      if (ok) ok = mbar_wait(smem_u32(&bars.x_full[xst]), x_phase, p.wait_limit);
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.x_full[xst]), x_phase, p.wait_limit));
+      if (!ok) break;
       if (rb * kL4Groups + wg < p.row_tiles) {
         const uint32_t x0 = smem_u32(smem + C::kX + xst * C::kXBytes);
         // K-major without swizzle: 8 columns of the weight are kXGroups x 128 bytes on, 8 columns of
@@ -602,11 +598,11 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
                                ((uint64_t)(128 / 16) << 32) | (1ull << 46);
 #pragma unroll
         for (int t = 0; t < kSlots; ++t) {
-          if (ok) ok = mbar_wait(full_bar + 8 * (slots & 1), (slots >> 1) & 1, p.wait_limit);
+          ok = mbar_wait(full_bar + 8 * (slots & 1), (slots >> 1) & 1, p.wait_limit);
           __syncwarp();
           tmem_fence_after();
           const uint32_t a = a0 + a_col;
-          if (elect_one()) {
+          if (elect_one() && ok) {
 #pragma unroll
             for (int k = 0; k < kSlotCols / 16; ++k) {
               const uint32_t d = a0 + d_col + (16 * k / kScaleCols) * C::kN;
@@ -619,11 +615,13 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
             mma_commit(done_bar + 8 * (slots & 1));
             if (t == kSlots - 1) mma_commit(xfree);
           }
-          __syncwarp();
           ++slots;
+          ok = __all_sync(0xffffffffu, ok);  // after the MMAs: they wait for no vote
+          if (!ok) break;
           a_col = a_col == (C::kASlots - 1) * 32 ? 0 : a_col + 32;
           if (kLag == 2 && t % kSlotsPerScale == kSlotsPerScale - 1) d_col ^= C::kD ^ (C::kD + C::kDCols);
         }
+        if (!ok) break;
       } else if (lane == 0) {  // no rows here (in the last row block): only x goes by
         mbar_arrive(xfree);
       }
@@ -636,16 +634,31 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
         ++rb;
       }
     }
+    // tensor memory and the tiles of x outlive the MMAs: a barrier of their own, as after a failure
+    // the warpgroup has not waited for them
+    __syncwarp();
+    if (slots > 0) {
+      if (elect_one()) mma_commit(smem_u32(&bars.drained[wg]));
+      __syncwarp();
+      mbar_wait(smem_u32(&bars.drained[wg]), 0);
+    }
     __syncwarp();
   } else {
     // ---- the warpgroup: 4 bits -> fp16 -> tensor memory, and the sums
     const uint32_t mine = tmem + wg * kL4TmemGroup + ((uint32_t)(my_warp & 3) << 21);  // this warp's 32 lanes
     const uint32_t lanebase = (uint32_t)lane * 4u;
-    const uint32_t full_bar = smem_u32(&bars.full[wg][0]), done_bar = smem_u32(&bars.done[wg][0]);
+    uint32_t full_bar = smem_u32(&bars.full[wg][0]);
+    const uint32_t done_bar = smem_u32(&bars.done[wg][0]);
     float acc[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) acc[c] = 0.f;
     bool ok = true;
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      if (ok && !mbar_wait(bar, parity, p.wait_limit)) {
+        ok = false;
+        full_bar = smem_u32(&bars.dead[0]);  // (testing ok at each arrival took 2% more with 32 columns)
+      }
+    };
     int slots = 0;                         // rounds so far
     uint32_t a_col = 0, d_col = C::kD;     // of this round; of the products to add next
     constexpr int kXs = C::kOwnX ? NC : 1;
@@ -653,7 +666,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
     int open = -1;                         // its row block: that of the sums
     // waits for round i; its products, scaled, join the sums if they are whole
     auto add_round = [&](int i, bool whole, const float* s, const float* xs) {
-      if (ok) ok = mbar_wait(done_bar + 8 * (i & 1), (i >> 1) & 1, p.wait_limit);
+      wait(done_bar + 8 * (i & 1), (i >> 1) & 1);
       __syncwarp();
       tmem_fence_after();
       if (whole) {
@@ -687,10 +700,10 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
     for (int u = u0; u < u1; ++u) {
       if (rb * kL4Groups + wg >= p.row_tiles) break;  // no rows here, nor later
       const uint32_t stage = smem_u32(smem + C::kRing + (wg * C::kStages + st) * C::kStageBytes);
-      if (ok) ok = mbar_wait(smem_u32(&bars.w_full[wg][st]), w_phase, p.wait_limit);
+      wait(smem_u32(&bars.w_full[wg][st]), w_phase);
       float s[NPG], xs[kXs];
       if constexpr (C::kOwnX) {
-        if (ok) ok = mbar_wait(smem_u32(&bars.x_full[xst]), x_phase, p.wait_limit);
+        wait(smem_u32(&bars.x_full[xst]), x_phase);
 #pragma unroll
         for (int c = 0; c < NC; ++c)
           asm volatile("ld.shared.f32 %0, [%1];" : "=f"(xs[c]) : "r"(smem_u32(&bars.x_scale[xst][c])));
@@ -794,11 +807,13 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kL4Groups * kL4TmemGroup) : "memory");
 }
 
-// kShare threads share the segments of an output (their loads are under way together), and
-// their sums are added in order: the same bits every time.  Four where an output has more than
-// four segments and the threads of all outputs fit the GPU at once (4096 outputs of one row: 3.7
-// -> 1.5 us), else one (16384 outputs of 32 rows would take 10 us more with four).
-template <int kShare>
+// An output's segments are added as four sums, of every fourth each, and these in order: the same
+// bits every time, and whether one thread or four (kShare) do it, so whatever the number of rows.
+// Four threads where an output has more than four segments and the threads of all outputs fit the
+// GPU at once (4096 outputs of one row: 3.7 -> 1.5 us), else one (16384 outputs of 32 rows would
+// take 10 us more with four).  kMany: more than four segments; with four at most each is a sum of
+// its own, and the loop is short (104 us -> 111 with the other at 53248 outputs of 32 rows).
+template <int kShare, bool kMany>
 __global__ void __launch_bounds__(kL4BlockRows) lin4_finalize_kernel(const float* part, const float* scale, int units,
                                                                        int ctas, int steps, int max_segs, int cols,
                                                                        int rows, int N, const void* bias, int bias_dt,
@@ -811,19 +826,31 @@ __global__ void __launch_bounds__(kL4BlockRows) lin4_finalize_kernel(const float
   const int segs = stream_owner(units, ctas, (rb + 1) * steps - 1) - first + 1;
   pdl_wait();
   const float* src = part + ((int64_t)rb * max_segs * cols + r) * kL4BlockRows + n % kL4BlockRows;
-  float v = 0.f;
-#pragma unroll 8
-  for (int k = q; k < segs; k += kShare) {
+  auto load = [&](int k) {
     const float* at = src + (int64_t)k * cols * kL4BlockRows;
-    float e = __ldcg(at);
-    if (cols > rows) e += __ldcg(at + (int64_t)rows * kL4BlockRows);  // the remainders of an fp32 x
-    v += e;
-  }
-  if constexpr (kShare > 1) {
+    return cols > rows ? __ldcg(at) + __ldcg(at + (int64_t)rows * kL4BlockRows) : __ldcg(at);  // the remainders of an fp32 x
+  };
+  float v = 0.f;
+  if (kShare > 1) {
+#pragma unroll 8
+    for (int k = q; k < segs; k += kShare) v += load(k);
     sums[q][i] = v;
     __syncthreads();
 #pragma unroll
     for (int j = 1; j < kShare; ++j) v += sums[j][i];
+  } else if (!kMany) {
+#pragma unroll 4
+    for (int k = 0; k < segs; ++k) v += load(k);
+  } else {
+    float u[4] = {};
+    for (int k0 = 0; k0 < segs; k0 += 8) {  // eight loads under way
+      float e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = k0 + j < segs ? load(k0 + j) : 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j % 4] += e[j];
+    }
+    v = ((u[0] + u[1]) + u[2]) + u[3];
   }
   if (q != 0 || n >= N) return;
   if (scale) v *= __ldcg(scale + r);
@@ -1016,9 +1043,10 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
   p.max_segs = pl.max_segs;
   p.wait_limit = copy_wait_spins();
   NSM_CHECK_CUDA(launch_pdl(f.fn, dim3(pl.ctas), dim3(kL4Threads), (size_t)f.smem, s, p));
-  const int share = pl.max_segs > 4 && 4LL * sh.N * rows <= 2048LL * di.sm_count ? 4 : 1;
+  const bool many = pl.max_segs > 4;
+  const int share = many && 4LL * sh.N * rows <= 2048LL * di.sm_count ? 4 : 1;
   const int fin_rows = kL4BlockRows / share;
-  NSM_CHECK_CUDA(launch_pdl(share == 4 ? lin4_finalize_kernel<4> : lin4_finalize_kernel<1>,
+  NSM_CHECK_CUDA(launch_pdl(share == 4 ? lin4_finalize_kernel<4, true> : many ? lin4_finalize_kernel<1, true> : lin4_finalize_kernel<1, false>,
                             dim3((sh.N + fin_rows - 1) / fin_rows, rows), dim3(kL4BlockRows), 0, s, (const float*)part,
                             (const float*)(pl.own_x ? nullptr : scale), pl.units, pl.ctas, sh.steps, pl.max_segs, pl.cols,
                             (int)rows, sh.N, w->bias, (int)w->bias_dtype, out, (int)out_dtype, out_row_stride));

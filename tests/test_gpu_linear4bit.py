@@ -292,3 +292,32 @@ def test_refuses_bad_calls_before_any_launch(dev):
     assert call(at=ws.data_ptr() + 16) == _lib.NSM_ERR_WORKSPACE
     assert call(rows=0) == _lib.NSM_OK
     assert call() == _lib.NSM_OK
+
+
+def test_largest_finite_x(dev):
+    """Values next to the top of bf16's and fp32's range, scaled like any other: one and
+    many rows (the kernel's own tiles of x, and those of the kernel before it)."""
+    from next_step_ai_b200.linear4bit import Linear4bit
+
+    N, K = 130, 256
+    p, sc, _, zeros, _ = _make(N, K, 128, "zeros", dev, 12)
+    sc = sc * 2.0 ** -20
+    layer = Linear4bit(p, sc, out_features=N, in_features=K, group_size=128, zeros=zeros)
+    W = _dense(p, sc, None, zeros, N, K, 128)
+    for xd, rows in ((BF, 1), (BF, 9), (FS, 2), (FS, 16)):
+        x = torch.randn((rows, K), device=dev).clamp_(-4, 4)
+        x[:, 5] = 4.0
+        x = (x * (0.99 * 2.0 ** 126)).to(xd)
+        _check(layer(x, out_dtype=FS), x, W, None, None)
+
+
+@pytest.mark.parametrize("kind,N,K", [("code", 4096, 2048), ("sym", 2048, 16384), ("zeros", 5000, 640)])
+def test_a_row_gives_the_same_bits_alone_and_among_others(dev, kind, N, K):
+    from next_step_ai_b200.linear4bit import Linear4bit
+
+    p, sc, code, zeros, _ = _make(N, K, 64, kind, dev, 21)
+    layer = Linear4bit(p, sc, out_features=N, in_features=K, group_size=64, code=code, zeros=zeros)
+    x = torch.randn((32, K), device=dev, dtype=BF)
+    y = layer(x, out_dtype=FS)
+    for n in (1, 3, 8, 16, 17):
+        assert torch.equal(layer(x[:n], out_dtype=FS), y[:n])
