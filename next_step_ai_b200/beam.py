@@ -30,7 +30,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, num_candidates: i
     the beams.  ``finished [batch, beams]`` (bool): such a beam is one candidate,
     ``pad_token`` at its own score.  A logit of -infinity or NaN is no
     candidate; where too few exist: score -infinity, token -1, parent 0.
-    Sums and scores are compared in 64 bits."""
+    Scores are formed and compared in 64 bits, with log-sum-exps of fp32 sums."""
     require_cuda(logits, "logits")
     dev = logits.device
     if scores.dim() != 2 or scores.dtype != torch.float32 or scores.device != dev:
@@ -65,8 +65,6 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, num_candidates: i
 
 
 _WS_BYTES: dict[tuple[int, int, int, int, int], int] = {}  # by device and sizes
-
-
 _LIB = None
 
 
@@ -147,13 +145,20 @@ def _describe(t: torch.Tensor, rows: int, length_dim: int | None) -> _lib.BeamSt
                            inner * es if length_dim is not None else 0, count)
 
 
+def _check_apart(states) -> None:
+    """No state is given twice: it would be put in order twice, at the same time."""
+    first = [t.data_ptr() for t in states]
+    if len(set(first)) != len(first):
+        raise RuntimeError("two states begin at the same address: states must not overlap")
+
+
 class BeamStates:
     """The per-beam states of a decode (caches, histories, residuals), reordered in
     place and in one launch after each selection.
 
     ``states``: CUDA tensors ``[batch * beams, ...]`` of any type, row ``b *
-    beams + w`` beam ``w`` of item ``b``; they are kept and must keep their
-    memory.  ``length_dims``: for each state the dimension that holds positions, or
+    beams + w`` beam ``w`` of item ``b``; they are kept, must keep their memory
+    and must not overlap.  ``length_dims``: for each state the dimension that holds positions, or
     ``None``; :meth:`reorder_` can then move the first ``length`` positions only."""
 
     def __init__(self, states, batch: int, beams: int, length_dims=None):
@@ -170,6 +175,7 @@ class BeamStates:
             require_cuda(t, "a state")
             if t.device != self.states[0].device:
                 raise RuntimeError(f"states are on {self.states[0].device} and {t.device}")
+        _check_apart(self.states)
         self.device = self.states[0].device
         n = len(self.states)
         self._c = (_lib.BeamStateC * n)(*(_describe(t, self.batch * self.beams, d) for t, d in zip(self.states, dims)))

@@ -113,3 +113,12 @@ def test_bad_arguments_are_errors_before_any_device_call(lib):
     assert re(st, one, 1, 1, 2, None, -1, None) == bad
     assert re(st, one, 1, 1, 33, one, -1, None) == big
     assert re(st, one, 1, 0, 2, one, -1, None) == _lib.NSM_OK
+
+
+def test_a_state_given_twice_is_refused():
+    t = torch.zeros((4, 6))
+    beam._check_apart([t, torch.zeros((4, 6)), t[:, 3:]])
+    with pytest.raises(RuntimeError, match="must not overlap"):
+        beam._check_apart([t, torch.zeros((4, 6)), t])
+    with pytest.raises(RuntimeError, match="must not overlap"):
+        beam._check_apart([t, t[:, :3]])
