@@ -569,7 +569,9 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
  * are formed and compared in 64 bits.  Outputs [batch]
  * [candidates]: scores, tokens and parents (the beam w); where fewer candidates
  * exist, score -infinity, token -1, parent 0.  1..32 beams, 1..64 candidates.  The
- * workspace needs no initialisation. */
+ * workspace needs no initialisation; nsm_beam_select_workspace_bytes is 0 for sizes
+ * that are refused, and for those that need none (any workspace pointer but NULL
+ * will do). */
 size_t nsm_beam_select_workspace_bytes(int32_t batch, int32_t beams, int32_t vocab, int32_t candidates);
 int nsm_beam_select(const void* logits, int32_t logits_dtype, int64_t batch_stride, int64_t beam_stride,
                     const float* scores, const uint8_t* finished, int32_t batch, int32_t beams, int32_t vocab,

@@ -83,7 +83,7 @@ def _select(logits, code, scores, fin, B, W, V, k, pad_token, dev):
             if len(_WS_BYTES) > 4096:
                 _WS_BYTES.clear()
             need = _WS_BYTES[key] = int(lib.nsm_beam_select_workspace_bytes(B, W, V, k))
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else out_s  # (a pointer that is not used)
         stride = logits.stride()
         status = lib.nsm_beam_select(logits.data_ptr(), code, stride[0], stride[1], scores.data_ptr(), fin, B, W, V, k,
                                      pad_token, out_s.data_ptr(), out_t.data_ptr(), out_p.data_ptr(), ws.data_ptr(),

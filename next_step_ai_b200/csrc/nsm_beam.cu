@@ -16,15 +16,22 @@
 // equal scores included, since blocks are contiguous and in the order of the
 // candidates.  Their values are read again (from L2), scored in 64 bits, and those
 // that reach the k-th block's largest, hardly more than k, are ranked by counting.
-// What bounds the scan is the issue of its instructions for 16-bit logits (about 6 per value)
-// and HBM for fp32.
+// beam_select_kernel is both in one launch, for inputs that a cluster of CTAs per batch item
+// goes through as quickly: a call then costs the host 12.5 us instead of 16.5 (one launch and no
+// workspace), and the GPU 1.3 us more in a graph (9.8 and 11.7 us instead of 8.6 and 10.3 for
+// 1 x 4 x 128256 in fp32 and 24 x 5 x 50257 in fp16).
+//
+// Measured in a graph: 32 x 16 x 128256 in fp32, 32 candidates 41 us (the scan 33: 79% of the
+// copy bandwidth); 16 x 8 x 128256 in bf16 16 us, 9.7 of them the scan, which the issue of its
+// instructions bounds for 16-bit logits (about 6 per value).  The merge is a chain of short
+// steps of one CTA, 5 to 6 us: loads from L2, a double-precision logarithm, ranks.
 //
 // Reordering.  beam_reorder_kernel moves the states in place: a thread owns
 // one 1- to 16-byte column of all beams of a batch item, loads the beams that
 // others go on with, then stores them where they moved.  A beam that stays
 // is not written, and one that nobody else takes is not read.
 #include <algorithm>
-#include <climits>
+#include <atomic>
 
 #include "nsm_common.cuh"
 #include "nsm_internal.h"
@@ -225,22 +232,18 @@ __device__ __forceinline__ void load_block(const T* row, int64_t at, int left, R
   }
 }
 
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(kBsThreads, 4) beam_scan_kernel(ScanParams p) {
-  pdl_wait();
-  pdl_trigger();  // not before: the merge reads the scores before it waits
-  const int lane = threadIdx.x & 31;
-  const int64_t unit = (int64_t)blockIdx.x * kBsWarps + (threadIdx.x >> 5);
-  const int row = (int)(unit / p.segs), sg = (int)(unit - (int64_t)row * p.segs);
+// Piece sg of a row, by one warp: put_top(e, largest value in ordered bits) for each of its
+// entries, put_seg(maximum, sum of exp(value - maximum)).
+template <typename T, bool kVec, typename PutTop, typename PutSeg>
+__device__ __forceinline__ void scan_piece(const ScanParams& p, int row, int sg, PutTop put_top, PutSeg put_seg) {
   // a beam that is out (no score above -infinity) or finished is not read, here or later
-  if (row >= p.rows || !(p.scores[row] > -INFINITY) || (p.finished && p.finished[row])) return;
+  if (!(p.scores[row] > -INFINITY) || (p.finished && p.finished[row])) return;
   const int b = row / p.W, w = row - b * p.W;
   const T* src = reinterpret_cast<const T*>(p.logits) + b * p.batch_stride + w * p.beam_stride;
   const int64_t begin = (int64_t)sg * p.seg_blocks * kBsBlock;
   const int64_t end = min((int64_t)p.V, begin + (int64_t)p.seg_blocks * kBsBlock);
   float m = -INFINITY, s = 0.f, run_top = -INFINITY;
-  int in_run = 0;
-  uint32_t* top = p.top + (int64_t)row * p.entries + sg * (p.seg_blocks / p.run);
+  int in_run = 0, entry = sg * (p.seg_blocks / p.run);
   for (int64_t at = begin; at < end; at += kBsBlock) {  // the SM's other warps cover the wait for a block
     RawTile<T> q;
     load_block<T, kVec>(src, at, (int)min((int64_t)kBsBlock, end - at), q);
@@ -255,16 +258,31 @@ __global__ void __launch_bounds__(kBsThreads, 4) beam_scan_kernel(ScanParams p) 
       run_top = fmaxf(run_top, tm);
     }
     if (++in_run == p.run || at + kBsBlock >= end) {
-      const uint32_t o = __reduce_max_sync(0xffffffffu, order_clean(run_top));
-      if (lane == 0) *top = o;
-      ++top;
+      put_top(entry++, __reduce_max_sync(0xffffffffu, order_clean(run_top)));
       run_top = -INFINITY;
       in_run = 0;
     }
   }
   const float wm = warp_max(m);
-  const float ws = warp_sum(m > -INFINITY ? s * exp2_fast((m - wm) * kLog2e) : 0.f);
-  if (lane == 0) p.seg[(int64_t)row * p.segs + sg] = make_float2(wm, ws);
+  put_seg(wm, warp_sum(m > -INFINITY ? s * exp2_fast((m - wm) * kLog2e) : 0.f));
+}
+
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kBsThreads, 4) beam_scan_kernel(ScanParams p) {
+  pdl_wait();
+  pdl_trigger();  // not before: the merge reads the scores before it waits
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = (int64_t)blockIdx.x * kBsWarps + (threadIdx.x >> 5);
+  const int row = (int)(unit / p.segs), sg = (int)(unit - (int64_t)row * p.segs);
+  if (row >= p.rows) return;
+  scan_piece<T, kVec>(
+      p, row, sg,
+      [&](int e, uint32_t o) {
+        if (lane == 0) p.top[(int64_t)row * p.entries + e] = o;
+      },
+      [&](float m, float s) {
+        if (lane == 0) p.seg[(int64_t)row * p.segs + sg] = make_float2(m, s);
+      });
 }
 
 struct MergeParams {
@@ -483,20 +501,30 @@ __device__ __noinline__ void values_again(const MergeView& v, int blocks, u64 le
   __syncthreads();
 }
 
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(const __grid_constant__ MergeParams mp) {
-  extern __shared__ __align__(16) unsigned char bm_smem[];
+// What the scan noted: in global memory, by the kernel before (pdl_wait first), or in shared
+// memory.
+template <bool kShared>
+struct Notes {
+  const float2* seg;
+  const uint32_t* top;
+  __device__ __forceinline__ float2 load(const float2* at) const { return kShared ? *at : __ldcg(at); }
+  __device__ __forceinline__ uint32_t load(const uint32_t* at) const { return kShared ? *at : __ldcg(at); }
+};
+
+// The k best of batch item b by a CTA.
+template <typename T, bool kVec, bool kShared>
+__device__ __forceinline__ void merge_item(const MergeParams& mp, MergeShared& sh, u64* entries, const Notes<kShared> notes,
+                                           const int b) {
   const ScanParams& p = mp.scan;
-  MergeShared& sh = *reinterpret_cast<MergeShared*>(bm_smem);
-  const MergeView view{mp, sh, reinterpret_cast<u64*>(bm_smem + sizeof(MergeShared)), (int)blockIdx.x};
-  const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = p.W;
+  const MergeView view{mp, sh, entries, b};
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = p.W;
   const int per_beam = p.entries + 1;
   if (threadIdx.x == 0) sh.entries_listed = sh.values_listed = 0;
   if (threadIdx.x < kBmGroups) sh.group[threadIdx.x] = 0;
   __syncthreads();
 
   // 1. a warp per beam: the sums joined, the scores of its blocks' maxima
-  bool waited = false;
+  bool waited = kShared;
   for (int w = warp; w < W; w += kBmWarps) {
     const float sc = p.scores[b * W + w];
     const int alive = !(sc > -INFINITY) ? 0 : p.finished && p.finished[b * W + w] ? 2 : 1;
@@ -505,20 +533,20 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(const __grid_
     u64* entry = view.entry + w * per_beam;
     double lse = 0.0;
     if (alive == 1) {
-      const float2* seg = p.seg + (int64_t)(b * W + w) * p.segs;
-      const uint32_t* top = p.top + (int64_t)(b * W + w) * p.entries;
+      const float2* seg = notes.seg + w * p.segs;
+      const uint32_t* top = notes.top + w * p.entries;
       const float2 none = make_float2(-INFINITY, 0.f);
-      const float2 q0 = lane < p.segs ? __ldcg(seg + lane) : none;
+      const float2 q0 = lane < p.segs ? notes.load(seg + lane) : none;
       uint32_t o[4];  // on their way while the sums are joined
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = lane + 32 * i < p.entries ? __ldcg(top + lane + 32 * i) : 0u;
+      for (int i = 0; i < 4; ++i) o[i] = lane + 32 * i < p.entries ? notes.load(top + lane + 32 * i) : 0u;
       float m = q0.x;
-      for (int i = lane + 32; i < p.segs; i += 32) m = fmaxf(m, __ldcg(seg + i).x);
+      for (int i = lane + 32; i < p.segs; i += 32) m = fmaxf(m, notes.load(seg + i).x);
       m = warp_max(m);
       if (m > -INFINITY) {
         float s = q0.y * exp2_fast((q0.x - m) * kLog2e);
         for (int i = lane + 32; i < p.segs; i += 32) {
-          const float2 q = __ldcg(seg + i);
+          const float2 q = notes.load(seg + i);
           s += q.y * exp2_fast((q.x - m) * kLog2e);
         }
         s = warp_sum(s);
@@ -533,7 +561,7 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(const __grid_
             entry[e] = q;
             put_group(sh, w * per_beam + e, q);
           }
-          if (e + 128 < p.entries) o[i] = __ldcg(top + e + 128);
+          if (e + 128 < p.entries) o[i] = notes.load(top + e + 128);
         }
       }
     } else {
@@ -645,35 +673,146 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(const __grid_
   }
 }
 
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(const __grid_constant__ MergeParams mp) {
+  extern __shared__ __align__(16) unsigned char bm_smem[];
+  const ScanParams& p = mp.scan;
+  const int64_t row = (int64_t)blockIdx.x * p.W;
+  merge_item<T, kVec, false>(mp, *reinterpret_cast<MergeShared*>(bm_smem),
+                             reinterpret_cast<u64*>(bm_smem + sizeof(MergeShared)),
+                             Notes<false>{p.seg + row * p.segs, p.top + row * p.entries}, blockIdx.x);
+}
+
+// Both in one launch: a cluster of CTAs scans a batch item, its first CTA, in whose shared
+// memory all leave their notes, merges.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t in_first_cta(const void* at) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(at)));
+  return r;
+}
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kBmThreads, 1) beam_select_kernel(const __grid_constant__ MergeParams mp, int ctas) {
+  extern __shared__ __align__(16) unsigned char bm_smem[];
+  const ScanParams& p = mp.scan;
+  const int b = blockIdx.x / ctas, rank = blockIdx.x - b * ctas, lane = threadIdx.x & 31;
+  u64* entries = reinterpret_cast<u64*>(bm_smem + sizeof(MergeShared));
+  float2* seg = reinterpret_cast<float2*>(entries + p.W * (p.entries + 1));
+  uint32_t* top = reinterpret_cast<uint32_t*>(seg + p.W * p.segs);
+  cluster_arrive();
+  pdl_wait();
+  const uint32_t seg_at = in_first_cta(seg), top_at = in_first_cta(top);
+  cluster_wait();  // the first CTA is there
+  for (int u = rank * kBmWarps + (threadIdx.x >> 5); u < p.W * p.segs; u += ctas * kBmWarps) {
+    const int w = u / p.segs;
+    scan_piece<T, kVec>(
+        p, b * p.W + w, u - w * p.segs,
+        [&](int e, uint32_t o) {
+          if (lane == 0) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(top_at + (w * p.entries + e) * 4), "r"(o) : "memory");
+        },
+        [&](float m, float s) {
+          if (lane == 0)
+            asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(seg_at + u * 8), "f"(m), "f"(s) : "memory");
+        });
+  }
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  if (rank == 0) merge_item<T, kVec, true>(mp, *reinterpret_cast<MergeShared*>(bm_smem), entries, Notes<true>{seg, top}, b);
+}
+
+constexpr int kSelectMaxSmem = 96 * 1024;
+// Shared memory and clusters beyond the usual, for one of beam_select_kernel's variants.
+cudaError_t beam_select_allow(void (*fn)(MergeParams, int), int device) {
+  static std::atomic<uint64_t> done[6];  // a bit per device
+  void (*const all[6])(MergeParams, int) = {
+      beam_select_kernel<float, false>,  beam_select_kernel<float, true>,         beam_select_kernel<__half, false>,
+      beam_select_kernel<__half, true>, beam_select_kernel<__nv_bfloat16, false>, beam_select_kernel<__nv_bfloat16, true>};
+  const int i = (int)(std::find(all, all + 6, fn) - all);
+  if (done[i].load(std::memory_order_acquire) >> device & 1) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectMaxSmem);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) done[i].fetch_or(1ull << device, std::memory_order_release);
+  return e;
+}
+
 struct BeamPlan {
   int segs = 1, seg_blocks = 1, entries = 1, run = 1;
+  int cluster = 0;  // CTAs of a batch item in one launch; 0: two launches
+  double cost = 0;  // blocks that the slowest warp goes through
   size_t top_off = 0, bytes = 0, merge_smem = 0;
 };
 
 constexpr int kMergeMaxSmem = (int)sizeof(MergeShared) + (kBsMaxBeams * kBsMaxEntries + kBsMaxBeams) * 8;
 
-// Blocks per warp: the split that takes the fewest rounds of blocks when 32 warps fit
-// an SM; a warp costs about half a block beside its blocks.
-BeamPlan beam_plan(int rows, int W, int V, int sm_count) {
-  const int64_t warps = 32LL * sm_count;
+// Blocks per warp: the split that takes the fewest rounds of blocks for so many warps; a
+// warp costs about half a block beside its blocks.
+BeamPlan beam_split(int rows, int W, int V, int64_t warps) {
   BeamPlan pl;
   const int blocks = (int)(((int64_t)V + kBsBlock - 1) / kBsBlock);
   pl.run = (blocks + kBsMaxEntries - 1) / kBsMaxEntries;
   pl.entries = (blocks + pl.run - 1) / pl.run;
-  double best = 1e30;
+  pl.cost = 1e30;
   for (int e = 1; e <= pl.entries; ++e) {  // entries per warp
     const int segs = (pl.entries + e - 1) / e;
     const int64_t rounds = ((int64_t)rows * segs + warps - 1) / warps;
     const double cost = (double)rounds * (e * pl.run + 0.5);
-    if (cost < best) {
-      best = cost;
+    if (cost < pl.cost) {
+      pl.cost = cost;
       pl.seg_blocks = e * pl.run;
       pl.segs = segs;
     }
+    if (rounds == 1) break;  // longer pieces take no fewer rounds
   }
-  pl.top_off = align_up((size_t)rows * pl.segs * sizeof(float2), 256);
-  pl.bytes = pl.top_off + (size_t)rows * pl.entries * 4;
   pl.merge_smem = sizeof(MergeShared) + ((size_t)W * pl.entries + W) * 8;
+  return pl;
+}
+
+// Clusters of `ctas` CTAs of beam_select_kernel that the current device holds at once (an SM
+// holds one of its CTAs; a cluster lies within one group of SMs).
+int clusters_at_once(int ctas, const DeviceInfo& di) {
+  static std::atomic<int> known[64][5];
+  int at = 0;
+  while (1 << at < ctas) ++at;
+  int n = known[di.device][at].load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas * di.sm_count);
+    cfg.blockDim = dim3(kBmThreads);
+    cfg.dynamicSmemBytes = kSelectMaxSmem;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (beam_select_allow(beam_select_kernel<float, true>, di.device) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, beam_select_kernel<float, true>, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = -1;
+    }
+    known[di.device][at].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// One launch where clusters of up to 16 CTAs with 32 warps each fit the GPU at once and take
+// at most a block more per warp than all SMs would.
+BeamPlan beam_plan(int batch, int W, int V, const DeviceInfo& di) {
+  BeamPlan pl = beam_split(batch * W, W, V, 32LL * di.sm_count), best;
+  for (int ctas = 16; ctas >= 1; ctas /= 2) {
+    if (ctas * batch > di.sm_count || clusters_at_once(ctas, di) < batch) continue;
+    BeamPlan one = beam_split(W, W, V, (int64_t)ctas * kBmWarps);
+    one.merge_smem += (size_t)W * one.segs * sizeof(float2) + (size_t)W * one.entries * 4;
+    if (one.cost <= pl.cost + 1.0 && one.merge_smem <= kSelectMaxSmem && (best.cluster == 0 || one.cost <= best.cost)) {
+      best = one;
+      best.cluster = ctas;
+    }
+  }
+  if (best.cluster > 0) return best;
+  pl.top_off = align_up((size_t)batch * W * pl.segs * sizeof(float2), 256);
+  pl.bytes = pl.top_off + (size_t)batch * W * pl.entries * 4;
   return pl;
 }
 
@@ -682,13 +821,16 @@ bool beam_size_ok(int batch, int beams, int vocab, int k) {
          (int64_t)batch * beams <= (1 << 20);
 }
 
-using ScanFn = void (*)(ScanParams);
-using MergeFn = void (*)(MergeParams);
+struct BeamFns {
+  void (*scan)(ScanParams);
+  void (*merge)(MergeParams);
+  void (*both)(MergeParams, int);
+};
 
 template <typename T>
-void beam_pick(bool vec, ScanFn* scan, MergeFn* merge) {
-  *scan = vec ? beam_scan_kernel<T, true> : beam_scan_kernel<T, false>;
-  *merge = vec ? beam_merge_kernel<T, true> : beam_merge_kernel<T, false>;
+BeamFns beam_pick(bool vec) {
+  if (vec) return {beam_scan_kernel<T, true>, beam_merge_kernel<T, true>, beam_select_kernel<T, true>};
+  return {beam_scan_kernel<T, false>, beam_merge_kernel<T, false>, beam_select_kernel<T, false>};
 }
 
 // ---- reordering -------------------------------------------------------------------
@@ -794,7 +936,7 @@ size_t nsm_beam_select_workspace_bytes(int32_t batch, int32_t beams, int32_t voc
   if (!beam_size_ok(batch, beams, vocab, candidates)) return 0;
   DeviceInfo di;
   if (current_device(&di) != NSM_OK) return 0;
-  return beam_plan(batch * beams, beams, vocab, di.sm_count).bytes;
+  return beam_plan(batch, beams, vocab, di).bytes;
 }
 
 int nsm_beam_select(const void* logits, int32_t logits_dtype, int64_t batch_stride, int64_t beam_stride,
@@ -817,8 +959,8 @@ int nsm_beam_select(const void* logits, int32_t logits_dtype, int64_t batch_stri
   const int rc = current_device(&di);
   if (rc != NSM_OK) return rc;
   const int rows = batch * beams;
-  const BeamPlan pl = beam_plan(rows, beams, vocab, di.sm_count);
-  NSM_REQUIRE(((uintptr_t)workspace & 255) == 0 && workspace_bytes >= pl.bytes, NSM_ERR_WORKSPACE,
+  const BeamPlan pl = beam_plan(batch, beams, vocab, di);
+  NSM_REQUIRE(pl.bytes == 0 || (((uintptr_t)workspace & 255) == 0 && workspace_bytes >= pl.bytes), NSM_ERR_WORKSPACE,
               "nsm_beam_select: workspace misaligned or too small (nsm_beam_select_workspace_bytes)");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   auto* ws = static_cast<unsigned char*>(workspace);
@@ -845,19 +987,20 @@ int nsm_beam_select(const void* logits, int32_t logits_dtype, int64_t batch_stri
   mp.out_parents = out_parents;
   // 16-byte loads when every row starts on 16 bytes, else one value per lane
   const bool vec = (((uintptr_t)logits | (uintptr_t)(batch_stride * es) | (uintptr_t)(beam_stride * es)) & 15) == 0;
-  ScanFn scan;
-  MergeFn merge;
-  if (logits_dtype == NSM_F32)
-    beam_pick<float>(vec, &scan, &merge);
-  else if (logits_dtype == NSM_F16)
-    beam_pick<__half>(vec, &scan, &merge);
-  else
-    beam_pick<__nv_bfloat16>(vec, &scan, &merge);
+  const BeamFns f = logits_dtype == NSM_F32   ? beam_pick<float>(vec)
+                    : logits_dtype == NSM_F16 ? beam_pick<__half>(vec)
+                                              : beam_pick<__nv_bfloat16>(vec);
+  if (pl.cluster > 0) {
+    NSM_CHECK_CUDA(beam_select_allow(f.both, di.device));
+    NSM_CHECK_CUDA(launch_pdl_cluster(f.both, dim3(batch * pl.cluster), dim3(kBmThreads), pl.merge_smem, s, pl.cluster, mp,
+                                      pl.cluster));
+    return NSM_OK;
+  }
   const int64_t warps = (int64_t)rows * pl.segs;
-  NSM_CHECK_CUDA(launch_pdl(scan, dim3((unsigned)((warps + kBsWarps - 1) / kBsWarps)), dim3(kBsThreads), 0, s, sp));
+  NSM_CHECK_CUDA(launch_pdl(f.scan, dim3((unsigned)((warps + kBsWarps - 1) / kBsWarps)), dim3(kBsThreads), 0, s, sp));
   static SmemOnce once[6];
-  NSM_CHECK_CUDA(once[logits_dtype * 2 + vec].set(merge, kMergeMaxSmem, di.device));
-  NSM_CHECK_CUDA(launch_pdl(merge, dim3(batch), dim3(kBmThreads), pl.merge_smem, s, mp));
+  NSM_CHECK_CUDA(once[logits_dtype * 2 + vec].set(f.merge, kMergeMaxSmem, di.device));
+  NSM_CHECK_CUDA(launch_pdl(f.merge, dim3(batch), dim3(kBmThreads), pl.merge_smem, s, mp));
   return NSM_OK;
 }
 

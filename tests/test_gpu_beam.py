@@ -432,3 +432,16 @@ def test_small_vocabularies(dev, W, V, k):
     s = torch.zeros((3, W), device=dev)
     same = x[:, :1].expand(3, W, V)
     _check(beam_select(same, s, num_candidates=k), same, s, k, exact=True)
+
+
+@pytest.mark.parametrize("B", [1, 7, 8, 15, 16, 33, 34, 74, 75, 148, 149])
+def test_batches_in_one_launch_and_in_two(dev, B):
+    """The sizes at which a selection goes from clusters of 16 CTAs per item to fewer, and to
+    two launches: what an item gets does not depend on its neighbours but for rounding."""
+    from next_step_ai_b200 import beam_select
+
+    x, s, gen = _inputs(B, 3, 5003, FH, dev, B)
+    _check(beam_select(x, s, num_candidates=6), x, s, 6)
+    x[:] = x[:1, :1].clone()                           # every beam alike: ties by beam, then token
+    s = torch.zeros_like(s)
+    _check(beam_select(x, s, num_candidates=6), x, s, 6, exact=True)
