@@ -137,27 +137,6 @@ __device__ __forceinline__ float raw_max(const RawTile<T>& q) {
   }
 }
 
-// Two fp32 values in one register pair: one instruction works on both.
-__device__ __forceinline__ u64 pair2(float a, float b) {
-  u64 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpair2(u64 v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ u64 add2(u64 a, u64 b) {
-  u64 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
-  u64 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // sum of exp(value - top) over the thread's values
 template <typename T, bool kClean>
 __device__ __forceinline__ float raw_exp_sum(const RawTile<T>& q, float top) {

@@ -649,9 +649,9 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
     const uint32_t lanebase = (uint32_t)lane * 4u;
     uint32_t full_bar = smem_u32(&bars.full[wg][0]);
     const uint32_t done_bar = smem_u32(&bars.done[wg][0]);
-    float acc[NC];
-#pragma unroll
-    for (int c = 0; c < NC; ++c) acc[c] = 0.f;
+    // sums of two columns each (16 columns 41.5 -> 40.0 us, 32 44.4 -> 43.4), or of one
+    unsigned long long acc[(NC + 1) / 2] = {};
+    float acc1 = 0.f;
     bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t parity) {
       if (ok && !mbar_wait(bar, parity, p.wait_limit)) {
@@ -677,10 +677,15 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
             uint32_t r[kLd];
             tmem_ld<kLd>(mine + d_col + g * C::kN + c0, r);
             tmem_wait_ld<kLd>(r);
+            if constexpr (NC == 1) {
+              acc1 = fmaf(s[g] * xs[0], __uint_as_float(r[0]), acc1);
+            } else {
 #pragma unroll
-            for (int c = 0; c < kLd; ++c) {
-              const float sc = C::kOwnX ? s[g] * xs[c0 + c] : s[g];  // (x's are powers of two)
-              acc[c0 + c] = fmaf(sc, __uint_as_float(r[c]), acc[c0 + c]);
+              for (int c = 0; c < kLd; c += 2) {
+                unsigned long long sc = pair2(s[g], s[g]);
+                if constexpr (C::kOwnX) sc = mul2(sc, pair2(xs[c0 + c], xs[c0 + c + 1]));  // (x's are powers of two)
+                acc[(c0 + c) / 2] = fma2(sc, pair2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), acc[(c0 + c) / 2]);
+              }
             }
           }
         }
@@ -692,9 +697,11 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
       float* dst = p.part + ((int64_t)(open * p.max_segs + seg) * p.cols) * kL4BlockRows + wg * kL4TileRows + row;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        if (c < p.cols) dst[(int64_t)c * kL4BlockRows] = ok ? acc[c] : __int_as_float(0x7fc00000);
-        acc[c] = 0.f;
+        const float2 v = NC == 1 ? make_float2(acc1, 0.f) : unpair2(acc[c / 2]);
+        if (c < p.cols) dst[(int64_t)c * kL4BlockRows] = !ok ? __int_as_float(0x7fc00000) : c % 2 ? v.y : v.x;
+        if (c % 2 == 1) acc[c / 2] = 0;
       }
+      acc1 = 0.f;
     };
     int st = 0, w_phase = 0, xst = 0, x_phase = 0;  // ring positions
     for (int u = u0; u < u1; ++u) {
