@@ -829,8 +829,10 @@ __global__ void __launch_bounds__(kL4BlockRows) lin4_finalize_kernel(const float
   __shared__ float sums[kShare][kRows];
   const int i = threadIdx.x % kRows, q = threadIdx.x / kRows;
   const int n = blockIdx.x * kRows + i, rb = n / kL4BlockRows, r = blockIdx.y;
-  const int first = stream_owner(units, ctas, rb * steps);
-  const int segs = stream_owner(units, ctas, (rb + 1) * steps - 1) - first + 1;
+  __shared__ int owner[2];  // the first and last CTA of the row block (64-bit divisions: by two threads)
+  if (threadIdx.x < 2) owner[threadIdx.x] = stream_owner(units, ctas, rb * steps + (threadIdx.x ? steps - 1 : 0));
+  __syncthreads();
+  const int segs = owner[1] - owner[0] + 1;
   pdl_wait();
   const float* src = part + ((int64_t)rb * max_segs * cols + r) * kL4BlockRows + n % kL4BlockRows;
   auto load = [&](int k) {
