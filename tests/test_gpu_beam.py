@@ -445,3 +445,24 @@ def test_batches_in_one_launch_and_in_two(dev, B):
     x[:] = x[:1, :1].clone()                           # every beam alike: ties by beam, then token
     s = torch.zeros_like(s)
     _check(beam_select(x, s, num_candidates=6), x, s, 6, exact=True)
+
+
+def test_logits_shared_far_apart_and_other_layouts(dev):
+    """Beams that share their logits (stride 0), rows more than 2^31 values apart, scores and
+    flags that are views, bytes as flags."""
+    from next_step_ai_b200 import beam_select
+
+    x, s, gen = _inputs(2, 4, 3001, BF, dev, 77)
+    shared = x[:, :1].expand(2, 4, 3001)
+    _check(beam_select(shared, s, num_candidates=9), shared, s, 9)
+    far = torch.empty(2 ** 31 + 16384, dtype=BF, device=dev)
+    view = torch.as_strided(far, (2, 4, 3001), (2 ** 31, 3001, 1))
+    view.copy_(x)
+    f = torch.rand((2, 4), device=dev, generator=gen) < 0.4
+    want = beam_select(x.contiguous(), s, num_candidates=9, finished=f, pad_token=5)
+    wide = torch.zeros((4, 2, 2), device=dev)
+    wide[..., 0] = s.t()
+    flags = f.t().contiguous().t().to(torch.uint8) * 7
+    got = beam_select(view, wide[..., 0].t(), num_candidates=9, finished=flags, pad_token=5)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    _check(got, x, s, 9, f, 5)

@@ -321,3 +321,52 @@ def test_a_row_gives_the_same_bits_alone_and_among_others(dev, kind, N, K):
     y = layer(x, out_dtype=FS)
     for n in (1, 3, 8, 16, 17):
         assert torch.equal(layer(x[:n], out_dtype=FS), y[:n])
+
+
+def test_graphs_with_many_rows(dev):
+    """Two graphs of one layer whose calls go through the kernel that lays x out, one of them
+    in three passes, replayed on two streams at once."""
+    from next_step_ai_b200.linear4bit import Linear4bit
+
+    N, K = 1030, 2048
+    p, sc, _, zeros, b = _make(N, K, 128, "zeros", dev, 31, FH, BF)
+    layer = Linear4bit(p, sc, out_features=N, in_features=K, group_size=128, zeros=zeros, bias=b)
+    W = _dense(p, sc, None, zeros, N, K, 128)
+    xs = [torch.zeros((r, K), device=dev, dtype=t) for r, t in ((9, FS), (70, BF))]
+    graphs, outs = [], []
+    for x in xs:
+        layer(x)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(layer(x))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for seed in range(3):
+        for x in xs:
+            x.copy_(torch.randn(x.shape, device=dev, generator=torch.Generator(device=dev).manual_seed(seed)))
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(xs, outs):
+            _check(y, x, W, b, None)
+
+
+def test_offsets_past_32_bits(dev):
+    """A weight of more than 2^32 bytes (its last rows), and rows of x that lie further apart."""
+    from next_step_ai_b200.linear4bit import Linear4bit
+
+    N, K = 131072 + 133, 65536 + 130
+    p = torch.randint(0, 256, (N, K // 2), dtype=torch.uint8, device=dev)
+    groups = -(-K // 128)
+    sc = (torch.rand((N, groups), device=dev) + 0.5).to(BF)
+    layer = Linear4bit(p, sc, out_features=N, in_features=K, group_size=128)
+    far = torch.empty(2 ** 31 + K, dtype=BF, device=dev)
+    x = torch.as_strided(far, (2, K), (2 ** 31, 1))
+    x.copy_(torch.randn((2, K), device=dev))
+    y = layer(x, out_dtype=FS)
+    for a in (0, 65536, N - 200):
+        W = _dense(p[a:a + 200], sc[a:a + 200], None, None, 200, K, 128)
+        _check(y[:, a:a + 200], x, W, None, None)
