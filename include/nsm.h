@@ -527,7 +527,8 @@ int nsm_lm_head_nf4(const void* x, int32_t x_dtype, int32_t tokens, const uint8_
  * to 22 bits for fp32 ones.  A result does not depend on the other rows of the
  * call and has the same bits every time (and for any number of rows, but for x's
  * values below that border).  The workspace needs no initialisation; calls that
- * share one must not overlap on the GPU.  A wait inside the kernel that runs out
+ * share one must not overlap on the GPU, unless nsm_linear4bit_workspace_bytes says
+ * 256: such a call does not touch it.  A wait inside the kernel that runs out
  * (nsm_set_copy_wait_limit) leaves NaN in the outputs it concerns. */
 typedef struct nsm_linear4bit_weights {
   const uint8_t* packed; /* tiled, from nsm_linear4bit_pack */

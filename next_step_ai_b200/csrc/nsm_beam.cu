@@ -31,7 +31,6 @@
 // others go on with, then stores them where they moved.  A beam that stays
 // is not written, and one that nobody else takes is not read.
 #include <algorithm>
-#include <atomic>
 
 #include "nsm_common.cuh"
 #include "nsm_internal.h"
@@ -664,13 +663,6 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(const __grid_
 
 // Both in one launch: a cluster of CTAs scans a batch item, its first CTA, in whose shared
 // memory all leave their notes, merges.
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ uint32_t in_first_cta(const void* at) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(at)));
-  return r;
-}
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kBmThreads, 1) beam_select_kernel(const __grid_constant__ MergeParams mp, int ctas) {
   extern __shared__ __align__(16) unsigned char bm_smem[];
@@ -681,7 +673,7 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_select_kernel(const __grid
   uint32_t* top = reinterpret_cast<uint32_t*>(seg + p.W * p.segs);
   cluster_arrive();
   pdl_wait();
-  const uint32_t seg_at = in_first_cta(seg), top_at = in_first_cta(top);
+  const uint32_t seg_at = in_cluster_cta(smem_u32(seg), 0), top_at = in_cluster_cta(smem_u32(top), 0);
   cluster_wait();  // the first CTA is there
   for (int u = rank * kBmWarps + (threadIdx.x >> 5); u < p.W * p.segs; u += ctas * kBmWarps) {
     const int w = u / p.segs;
@@ -702,19 +694,7 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_select_kernel(const __grid
 }
 
 constexpr int kSelectMaxSmem = 96 * 1024;
-// Shared memory and clusters beyond the usual, for one of beam_select_kernel's variants.
-cudaError_t beam_select_allow(void (*fn)(MergeParams, int), int device) {
-  static std::atomic<uint64_t> done[6];  // a bit per device
-  void (*const all[6])(MergeParams, int) = {
-      beam_select_kernel<float, false>,  beam_select_kernel<float, true>,         beam_select_kernel<__half, false>,
-      beam_select_kernel<__half, true>, beam_select_kernel<__nv_bfloat16, false>, beam_select_kernel<__nv_bfloat16, true>};
-  const int i = (int)(std::find(all, all + 6, fn) - all);
-  if (done[i].load(std::memory_order_acquire) >> device & 1) return cudaSuccess;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectMaxSmem);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess) done[i].fetch_or(1ull << device, std::memory_order_release);
-  return e;
-}
+ClusterOnce select_once[6];  // of beam_select_kernel's variants: dtype * 2 + kVec
 
 struct BeamPlan {
   int segs = 1, seg_blocks = 1, entries = 1, run = 1;
@@ -748,32 +728,11 @@ BeamPlan beam_split(int rows, int W, int V, int64_t warps) {
   return pl;
 }
 
-// Clusters of `ctas` CTAs of beam_select_kernel that the current device holds at once (an SM
-// holds one of its CTAs; a cluster lies within one group of SMs).
 int clusters_at_once(int ctas, const DeviceInfo& di) {
-  static std::atomic<int> known[64][5];
-  int at = 0;
-  while (1 << at < ctas) ++at;
-  int n = known[di.device][at].load(std::memory_order_relaxed);
-  if (n == 0) {
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)ctas;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas * di.sm_count);
-    cfg.blockDim = dim3(kBmThreads);
-    cfg.dynamicSmemBytes = kSelectMaxSmem;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (beam_select_allow(beam_select_kernel<float, true>, di.device) != cudaSuccess ||
-        cudaOccupancyMaxActiveClusters(&n, beam_select_kernel<float, true>, &cfg) != cudaSuccess || n < 1) {
-      cudaGetLastError();
-      n = -1;
-    }
-    known[di.device][at].store(n, std::memory_order_relaxed);
-  }
-  return n;
+  static ClustersAtOnce known;
+  constexpr auto kern = beam_select_kernel<float, true>;
+  if (select_once[2 * NSM_F32 + 1].set(kern, kSelectMaxSmem, di.device) != cudaSuccess) return -1;
+  return known.get(kern, kBmThreads, kSelectMaxSmem, ctas, di);
 }
 
 // One launch where clusters of up to 16 CTAs with 32 warps each fit the GPU at once and take
@@ -970,7 +929,7 @@ int nsm_beam_select(const void* logits, int32_t logits_dtype, int64_t batch_stri
                     : logits_dtype == NSM_F16 ? beam_pick<__half>(vec)
                                               : beam_pick<__nv_bfloat16>(vec);
   if (pl.cluster > 0) {
-    NSM_CHECK_CUDA(beam_select_allow(f.both, di.device));
+    NSM_CHECK_CUDA(select_once[logits_dtype * 2 + vec].set(f.both, kSelectMaxSmem, di.device));
     NSM_CHECK_CUDA(launch_pdl_cluster(f.both, dim3(batch * pl.cluster), dim3(kBmThreads), pl.merge_smem, s, pl.cluster, mp,
                                       pl.cluster));
     return NSM_OK;

@@ -152,6 +152,14 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int lim
   }
   return false;
 }
+// A cluster's barrier, and the address of a place in shared memory in its CTA `rank`.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t in_cluster_cta(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
 // Two fp32 values in one register pair: one instruction works on both.
 __device__ __forceinline__ unsigned long long pair2(float a, float b) {
   unsigned long long r;

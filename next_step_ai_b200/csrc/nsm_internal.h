@@ -151,7 +151,52 @@ inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, siz
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
-// The same in clusters of `cluster` CTAs.
+// The same for kernels launched in clusters of up to 16 CTAs.
+struct ClusterOnce {
+  SmemOnce smem;
+  std::atomic<unsigned long long> wide{0};
+  template <typename Kernel>
+  cudaError_t set(Kernel kern, int bytes, int device) {
+    cudaError_t e = smem.set(kern, bytes, device);
+    const unsigned long long bit = 1ull << (device & 63);
+    if (e != cudaSuccess || (wide.load(std::memory_order_acquire) & bit)) return e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) wide.fetch_or(bit, std::memory_order_release);
+    return e;
+  }
+};
+
+// Clusters of `ctas` (1, 2, 4, 8 or 16) CTAs of a kernel, of which an SM holds one, that a device
+// runs at once: a cluster lies within one group of SMs.  Asked once, after ClusterOnce::set.
+struct ClustersAtOnce {
+  std::atomic<int> known[64][5] = {};
+  template <typename Kernel>
+  int get(Kernel kern, int threads, int bytes, int ctas, const DeviceInfo& di) {
+    int at = 0;
+    while (1 << at < ctas) ++at;
+    std::atomic<int>& slot = known[di.device & 63][at];
+    int n = slot.load(std::memory_order_relaxed);
+    if (n != 0) return n;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(ctas * di.sm_count));
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)bytes;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = -1;
+    }
+    slot.store(n, std::memory_order_relaxed);
+    return n;
+  }
+};
+
+// launch_pdl in clusters of `cluster` CTAs.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pdl_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                                       int cluster, Args&&... args) {

@@ -11,7 +11,7 @@
 // row, and a warp's 16-byte loads are 512 contiguous bytes.  Scales and zero points lie
 // as [row tile][tile][128 rows][granules], a granule being the group or 128 columns.
 //
-// Two or three launches, linked by programmatic dependent launch:
+// One to three launches, linked by programmatic dependent launch:
 //  1. for more than 8 columns of x, lin4_prep_kernel: per row of x a power-of-two scale that
 //     brings the largest finite |x| to [2^14, 2^15), and x as fp16: exact for fp16, for bf16 exact
 //     down to 2^-31 of the row's largest value (below that off by at most 2^-39 of it); an
@@ -32,7 +32,8 @@
 //     threads the same but for the sums.  Each CTA leaves one fp32 partial per row block that it
 //     touched;
 //  3. lin4_finalize_kernel: the partials of a row block in a fixed order (the same
-//     bits every time), times the scale of x, + bias, in the output's type.
+//     bits every time), times the scale of x, + bias, in the output's type.  Small weights
+//     go without it: there a cluster of CTAs has a row block, and its sums join in shared memory.
 //
 // Measured, 16384 x 16384 with weights larger than L2: NF4, one row of x in bf16, 32 us; integers
 // with groups of 128, 30 us for one row and 44 us for 32.  In its steady state a unit of NF4
@@ -277,6 +278,13 @@ struct Lin4Params {
   float* part;  // [row block][segment][column of x][512]
   int row_tiles, steps, scale_steps, div, cols;
   int units, ctas, max_segs, wait_limit;
+  // One launch, a cluster of CTAs per row block (0: partials and lin4_finalize_kernel)
+  int cluster, N;
+  const float* scale;  // of x's rows, from lin4_prep_kernel
+  const void* bias;
+  void* out;
+  int64_t out_stride;
+  int bias_dt, out_dt;
 };
 
 __device__ __forceinline__ uint32_t hsub2_u32(uint32_t a, uint32_t b) {
@@ -399,6 +407,7 @@ struct Lin4Config {
   static constexpr int kBars = kX + kL4XStages * kXBytes + 1024;  // the last tile of x is read 128 bytes over
   static constexpr int kSmem = kBars + 512;
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
+  static_assert(kX - kRing >= kL4BlockRows * NC * 4, "a cluster's sums fit the rings");
 };
 
 struct Lin4Bars {
@@ -414,7 +423,7 @@ struct Lin4Bars {
 };
 static_assert(sizeof(Lin4Bars) <= 512, "barriers");
 
-template <int MODE, int NPG, int NC>
+template <int MODE, int NPG, int NC, bool kCluster>
 __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_constant__ Lin4Params p) {
   extern __shared__ __align__(1024) uint32_t l4_smem[];
   using C = Lin4Config<MODE, NPG, NC>;
@@ -428,8 +437,16 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
   unsigned char* smem = reinterpret_cast<unsigned char*>(l4_smem);
   Lin4Bars& bars = *reinterpret_cast<Lin4Bars*>(smem + C::kBars);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = threadIdx.x & 127;
-  const int u0 = stream_begin(p.units, p.ctas, blockIdx.x), u1 = stream_begin(p.units, p.ctas, blockIdx.x + 1);
-  pdl_trigger();
+  int u0, u1;
+  if constexpr (kCluster) {  // (no trigger: what comes next is no kernel of ours)
+    const int block = blockIdx.x / p.cluster, rank = blockIdx.x - block * p.cluster;
+    u0 = block * p.steps + p.steps * rank / p.cluster;
+    u1 = block * p.steps + p.steps * (rank + 1) / p.cluster;
+  } else {
+    u0 = stream_begin(p.units, p.ctas, blockIdx.x);
+    u1 = stream_begin(p.units, p.ctas, blockIdx.x + 1);
+    pdl_trigger();
+  }
 
   // warps 0-15: the warpgroups; 16-19: one that issues MMAs for each; 20-23: bring the tiles
   const int my_warp = __shfl_sync(0xffffffffu, warp, 0);
@@ -744,7 +761,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
           add_round(slots - kLag, was % kSlotsPerScale == kLast, s + was * NPG / kSlots, xs);
         } else if (open >= 0) {
           add_round(slots - kLag, was % kSlotsPerScale == kLast, ps + was * NPG / kSlots, pxs);
-          if (was == kSlots - 1 && open != rb) flush();
+          if (!kCluster && was == kSlots - 1 && open != rb) flush();  // (a cluster's CTA has one row block)
         }
       };
 #pragma unroll
@@ -803,10 +820,47 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
 #pragma unroll
       for (int t = kSlots - kLag; t < kSlots; ++t)
         add_round(slots - kSlots + t, t % kSlotsPerScale == kSlotsPerScale - 1, ps + t * NPG / kSlots, pxs);
-      flush();
+      if (!kCluster) flush();
     }
     __syncwarp();
     tmem_fence_before();
+    if constexpr (kCluster) {
+      // The cluster's CTAs share the row block's outputs: each gets the sums of its slice of rows
+      // into its weight rings, which nobody reads any more, and adds them in the CTAs' order.
+      const int slice = kL4BlockRows / p.cluster, block = blockIdx.x / p.cluster, rank = blockIdx.x - block * p.cluster;
+      const int mine_at = wg * kL4TileRows + row, to = mine_at / slice;
+      float* const sums = reinterpret_cast<float*>(smem + C::kRing);  // [CTA][column of x][row of the slice]
+      cluster_arrive();
+      cluster_wait();
+      const uint32_t dst = in_cluster_cta(smem_u32(sums + rank * p.cols * slice + mine_at % slice), to);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const float2 v = NC == 1 ? make_float2(acc1, 0.f) : unpair2(acc[c / 2]);
+        const float e = !ok ? __int_as_float(0x7fc00000) : c % 2 ? v.y : v.x;
+        if (c < p.cols) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + c * slice * 4), "f"(e) : "memory");
+      }
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();
+      for (int o = threadIdx.x; o < slice * p.rows; o += kL4Groups * 128) {
+        const int r = o / slice, i = o - r * slice, n = block * kL4BlockRows + rank * slice + i;
+        if (n >= p.N) continue;
+        float v = 0.f;
+        for (int k = 0; k < p.cluster; ++k) {
+          const float* at = sums + (k * p.cols + r) * slice + i;
+          v += p.cols > p.rows ? at[0] + at[p.rows * slice] : at[0];  // the remainders of an fp32 x
+        }
+        if (!C::kOwnX) v *= __ldcg(p.scale + r);
+        if (p.bias) v += load_as_f32(p.bias, p.bias_dt, n);
+        store_from_f32(p.out, p.out_dt, (int64_t)r * p.out_stride + n, v);
+      }
+    }
+  }
+  if (kCluster && my_warp >= 4 * kL4Groups) {
+    cluster_arrive();
+    cluster_wait();
+    cluster_arrive();
+    cluster_wait();
   }
   __syncthreads();
   tmem_fence_after();
@@ -869,24 +923,10 @@ __global__ void __launch_bounds__(kL4BlockRows) lin4_finalize_kernel(const float
 
 struct Lin4Plan {
   bool own_x = false;  // few columns: the kernel reads x itself
+  int cluster = 0;     // CTAs of a row block in one launch, 0: partials and lin4_finalize_kernel
   int cols = 0, col_groups = 1, units = 0, ctas = 0, max_segs = 0;
   size_t scale_off = 0, part_off = 0, bytes = 0;
 };
-
-Lin4Plan lin4_plan(const Lin4Shape& sh, int rows, int x_dtype, int sm_count) {
-  Lin4Plan pl;
-  pl.cols = x_dtype == NSM_F32 ? 2 * rows : rows;
-  pl.units = sh.row_blocks * sh.steps;
-  pl.ctas = std::max(1, std::min({sm_count, pl.units, sh.row_blocks * (kL4MaxSegs - 2)}));
-  const int least = pl.units / pl.ctas;  // units of the shortest run
-  pl.max_segs = (sh.steps - 1 + least - 1) / least + 1;
-  pl.col_groups = pl.cols <= 8 ? 1 : pl.cols <= 16 ? 2 : 4;
-  pl.own_x = pl.cols <= 8;
-  pl.scale_off = pl.own_x ? 0 : align_up((size_t)pl.col_groups * 8 * sh.kp * 2, 256);
-  pl.part_off = pl.scale_off + (pl.own_x ? 0 : align_up((size_t)rows * 4, 256));
-  pl.bytes = pl.part_off + (size_t)sh.row_blocks * pl.max_segs * pl.cols * kL4BlockRows * 4;
-  return pl;
-}
 
 bool lin4_size_ok(int N, int K, int group) {
   return N > 0 && K > 0 && K % 2 == 0 && group > 0 && group % 32 == 0 && N <= (1 << 24) && K <= (1 << 20) &&
@@ -903,19 +943,71 @@ struct Lin4Fn {
 // Columns of x that the sums hold: the next of 1, 2, 4, 8, 16, 32.
 int lin4_col_case(int cols) { return cols <= 1 ? 0 : cols <= 2 ? 1 : cols <= 4 ? 2 : cols <= 8 ? 3 : cols <= 16 ? 4 : 5; }
 
-template <int MODE, int NPG, int NC>
+template <int MODE, int NPG, int NC, bool kCluster>
 constexpr Lin4Fn lin4_fn() {
-  return {lin4_kernel<MODE, NPG, NC>, Lin4Config<MODE, NPG, NC>::kSmem};
+  return {lin4_kernel<MODE, NPG, NC, kCluster>, Lin4Config<MODE, NPG, NC>::kSmem};
 }
-template <int MODE, int NPG>
+template <int MODE, int NPG, bool kCluster>
 Lin4Fn lin4_pick_cols(int c) {
-  constexpr Lin4Fn fns[6] = {lin4_fn<MODE, NPG, 1>(), lin4_fn<MODE, NPG, 2>(),  lin4_fn<MODE, NPG, 4>(),
-                             lin4_fn<MODE, NPG, 8>(), lin4_fn<MODE, NPG, 16>(), lin4_fn<MODE, NPG, 32>()};
+  constexpr Lin4Fn fns[6] = {lin4_fn<MODE, NPG, 1, kCluster>(), lin4_fn<MODE, NPG, 2, kCluster>(),
+                             lin4_fn<MODE, NPG, 4, kCluster>(), lin4_fn<MODE, NPG, 8, kCluster>(),
+                             lin4_fn<MODE, NPG, 16, kCluster>(), lin4_fn<MODE, NPG, 32, kCluster>()};
   return fns[c];
 }
-template <int MODE>
+template <int MODE, bool kCluster>
 Lin4Fn lin4_pick_npg(int npg, int c) {
-  return npg == 1 ? lin4_pick_cols<MODE, 1>(c) : npg == 2 ? lin4_pick_cols<MODE, 2>(c) : lin4_pick_cols<MODE, 4>(c);
+  return npg == 1   ? lin4_pick_cols<MODE, 1, kCluster>(c)
+         : npg == 2 ? lin4_pick_cols<MODE, 2, kCluster>(c)
+                    : lin4_pick_cols<MODE, 4, kCluster>(c);
+}
+template <bool kCluster>
+Lin4Fn lin4_pick(int mode, int npg, int c) {
+  return mode == kCode        ? lin4_pick_npg<kCode, kCluster>(npg, c)
+         : mode == kCodeExact ? lin4_pick_npg<kCodeExact, kCluster>(npg, c)
+         : mode == kInt       ? lin4_pick_npg<kInt, kCluster>(npg, c)
+                              : lin4_pick_npg<kIntZeros, kCluster>(npg, c);
+}
+
+ClusterOnce lin4_once[2][4][3][6];  // of lin4_kernel's variants
+
+int lin4_clusters_at_once(int ctas, const DeviceInfo& di) {
+  static ClustersAtOnce known;
+  const Lin4Fn f = lin4_fn<kCode, 1, 1, true>();  // as all of them: one CTA per SM
+  if (lin4_once[1][kCode][0][0].set(f.fn, f.smem, di.device) != cudaSuccess) return -1;
+  return known.get(f.fn, kL4Threads, f.smem, ctas, di);
+}
+
+// In one launch, a row block is a cluster's, cut evenly over its CTAs, and the sums join in shared
+// memory: no finalize kernel and no workspace of partials.  The host then takes 8.5 us per call
+// instead of 12, the GPU 0.4 to 0.7 us more (4096 x 4096 10.0 in a graph instead of 9.3), so it is taken
+// where calls one after another wait for the host: runs of at most four units (0.94 us each), two
+// longer than an even cut's, of clusters that fit the GPU at once (14336 x 4096, eight units instead
+// of seven: 17.8 us instead of 17.2).  The choice depends on the weight alone, so a row's bits do not
+// depend on the number of rows.
+Lin4Plan lin4_plan(const Lin4Shape& sh, int rows, int x_dtype, const DeviceInfo& di) {
+  Lin4Plan pl;
+  pl.cols = x_dtype == NSM_F32 ? 2 * rows : rows;
+  pl.units = sh.row_blocks * sh.steps;
+  pl.ctas = std::max(1, std::min({di.sm_count, pl.units, sh.row_blocks * (kL4MaxSegs - 2)}));
+  const int least = pl.units / pl.ctas;  // units of the shortest run
+  pl.max_segs = (sh.steps - 1 + least - 1) / least + 1;
+  pl.col_groups = pl.cols <= 8 ? 1 : pl.cols <= 16 ? 2 : 4;
+  pl.own_x = pl.cols <= 8;
+  pl.scale_off = pl.own_x ? 0 : align_up((size_t)pl.col_groups * 8 * sh.kp * 2, 256);
+  pl.part_off = pl.scale_off + (pl.own_x ? 0 : align_up((size_t)rows * 4, 256));
+  const int longest = (pl.units + pl.ctas - 1) / pl.ctas;
+  int best = std::min(longest + 2, 4);
+  for (int c = 1; c <= 16; c *= 2) {
+    const int mine = (sh.steps + c - 1) / c;
+    if (c > sh.steps || c * sh.row_blocks > di.sm_count) break;
+    if (mine < best + (pl.cluster == 0) && lin4_clusters_at_once(c, di) >= sh.row_blocks) {
+      best = mine;
+      pl.cluster = c;
+    }
+  }
+  pl.bytes = std::max<size_t>(
+      256, pl.part_off + (pl.cluster > 0 ? 0 : (size_t)sh.row_blocks * pl.max_segs * pl.cols * kL4BlockRows * 4));
+  return pl;
 }
 
 }  // namespace
@@ -975,7 +1067,7 @@ size_t nsm_linear4bit_workspace_bytes(int32_t rows, int32_t x_dtype, int32_t out
   if (!lin4_size_ok(out_features, in_features, 32) || rows <= 0 || rows > lin4_max_rows(x_dtype)) return 0;
   DeviceInfo di;
   if (current_device(&di) != NSM_OK) return 0;
-  return lin4_plan(lin4_shape(out_features, in_features, 32), rows, x_dtype, di.sm_count).bytes;
+  return lin4_plan(lin4_shape(out_features, in_features, 32), rows, x_dtype, di).bytes;
 }
 
 int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_stride,
@@ -1004,7 +1096,7 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
   const int rc = current_device(&di);
   if (rc != NSM_OK) return rc;
   const Lin4Shape sh = lin4_shape(w->out_features, w->in_features, w->group_size);
-  const Lin4Plan pl = lin4_plan(sh, rows, x_dtype, di.sm_count);
+  const Lin4Plan pl = lin4_plan(sh, rows, x_dtype, di);
   NSM_REQUIRE(((uintptr_t)workspace & 255) == 0 && workspace_bytes >= pl.bytes, NSM_ERR_WORKSPACE,
               "nsm_linear4bit: workspace misaligned or too small (nsm_linear4bit_workspace_bytes)");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -1018,12 +1110,9 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
   // half an fp16 rounding), which halves the table reads that bound the kernel
   const int mode = w->code ? (out_dtype == NSM_F32 ? kCodeExact : kCode) : (w->zeros ? kIntZeros : kInt);
   const int cc = lin4_col_case(pl.cols);
-  const Lin4Fn f = mode == kCode        ? lin4_pick_npg<kCode>(sh.npg, cc)
-                   : mode == kCodeExact ? lin4_pick_npg<kCodeExact>(sh.npg, cc)
-                   : mode == kInt       ? lin4_pick_npg<kInt>(sh.npg, cc)
-                                        : lin4_pick_npg<kIntZeros>(sh.npg, cc);
-  static SmemOnce once[4][3][6];
-  NSM_CHECK_CUDA(once[mode][sh.npg / 2][cc].set(f.fn, f.smem, di.device));
+  const bool cluster = pl.cluster > 0;
+  const Lin4Fn f = cluster ? lin4_pick<true>(mode, sh.npg, cc) : lin4_pick<false>(mode, sh.npg, cc);
+  NSM_CHECK_CUDA(lin4_once[cluster][mode][sh.npg / 2][cc].set(f.fn, f.smem, di.device));
   if (!pl.own_x) {
     const int slices = std::max(1, std::min(8, sh.kp / 2048));
     lin4_prep_kernel<<<dim3(slices, rows), 256, 0, s>>>(x, x_dtype, x_row_stride, sh.K, sh.kp, rows, pl.col_groups,
@@ -1051,6 +1140,19 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
   p.ctas = pl.ctas;
   p.max_segs = pl.max_segs;
   p.wait_limit = copy_wait_spins();
+  p.cluster = pl.cluster;
+  p.N = sh.N;
+  p.scale = scale;
+  p.bias = w->bias;
+  p.bias_dt = w->bias_dtype;
+  p.out = out;
+  p.out_dt = out_dtype;
+  p.out_stride = out_row_stride;
+  if (cluster) {
+    NSM_CHECK_CUDA(launch_pdl_cluster(f.fn, dim3(sh.row_blocks * pl.cluster), dim3(kL4Threads), (size_t)f.smem, s,
+                                      pl.cluster, p));
+    return NSM_OK;
+  }
   NSM_CHECK_CUDA(launch_pdl(f.fn, dim3(pl.ctas), dim3(kL4Threads), (size_t)f.smem, s, p));
   const bool many = pl.max_segs > 4;
   const int share = many && 4LL * sh.N * rows <= 2048LL * di.sm_count ? 4 : 1;

@@ -86,6 +86,7 @@ class Linear4bit:
                                           ptr(self.bias), dtype_code(self.bias.dtype) if bias is not None else 0, N, K, gs)
         self._ref = ctypes.byref(self._c)
         self._ws_bytes: dict[tuple[int, int], int] = {}
+        self._spare = torch.empty(256, dtype=torch.uint8, device=self.device)  # for calls that need no workspace
 
     # ---- construction
     @classmethod
@@ -182,7 +183,7 @@ class Linear4bit:
             need = self._ws_bytes.get((n, xc))
             if need is None:
                 need = self._ws_bytes[(n, xc)] = int(lib.nsm_linear4bit_workspace_bytes(n, xc, N, self.in_features))
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            ws = self._spare if need == 256 else torch.empty(need, dtype=torch.uint8, device=dev)
             status = lib.nsm_linear4bit(xp, xc, n, stride, self._ref, op, oc, N, ws.data_ptr(), need, stream)
             if status:
                 _lib.check(status, "nsm_linear4bit")

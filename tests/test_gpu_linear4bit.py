@@ -370,3 +370,21 @@ def test_offsets_past_32_bits(dev):
     for a in (0, 65536, N - 200):
         W = _dense(p[a:a + 200], sc[a:a + 200], None, None, 200, K, 128)
         _check(y[:, a:a + 200], x, W, None, None)
+
+
+@pytest.mark.parametrize("N,K", [(512, 128), (513, 2048), (2048, 2050), (4096, 4096), (4100, 4096), (9216, 1024),
+                                 (37888, 256), (38000, 256), (75776, 128), (75777, 128)])
+def test_weights_in_one_launch_and_in_two(dev, N, K):
+    """The sizes at which a row block goes from a cluster of 16 CTAs to fewer, and to partials: one,
+    eight, nine and 32 rows, and fp32 rows in two columns each."""
+    from next_step_ai_b200.linear4bit import Linear4bit
+
+    for kind in ("code", "zeros"):
+        p, sc, code, zeros, b = _make(N, K, 64, kind, dev, N + K, FS, FS)
+        layer = Linear4bit(p, sc, out_features=N, in_features=K, group_size=64, code=code, zeros=zeros, bias=b)
+        W = _dense(p, sc, code, zeros, N, K, 64)
+        for rows, xd in ((1, BF), (8, FH), (9, BF), (32, BF), (4, FS), (16, FS)):
+            x = torch.randn((rows, K), device=dev).to(xd)
+            y = layer(x, out_dtype=FS)
+            _check(y, x, W, b, code)
+            assert torch.equal(y, layer(x, out_dtype=FS))
