@@ -466,3 +466,18 @@ def test_logits_shared_far_apart_and_other_layouts(dev):
     got = beam_select(view, wide[..., 0].t(), num_candidates=9, finished=flags, pad_token=5)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     _check(got, x, s, 9, f, 5)
+
+
+@pytest.mark.parametrize("B,W,V,k,dtype", [(28, 11, 1429, 15, BF), (8, 16, 1712, 29, BF), (21, 7, 1370, 12, FS),
+                                           (1, 5, 3041, 10, FH), (160, 5, 3296, 9, FS), (2, 3, 40000, 64, FH)])
+def test_few_blocks_with_many_values_above_the_last(dev, B, W, V, k, dtype):
+    """As many blocks of the vocabulary as candidates, some of them far below the others: the
+    last one's largest value says little about the candidates."""
+    from next_step_ai_b200 import beam_select
+
+    x, s, gen = _inputs(B, W, V, dtype, dev, V + k)
+    _check(beam_select(x, s * 20, num_candidates=k), x, s * 20, k)
+    down = torch.sort(x.float(), dim=-1, descending=True).values.to(dtype)
+    _check(beam_select(down, s, num_candidates=k), down, s, k)
+    f = torch.rand((B, W), device=dev, generator=gen) < 0.4
+    _check(beam_select(down, s, num_candidates=k, finished=f, pad_token=3), down, s, k, f, 3)
