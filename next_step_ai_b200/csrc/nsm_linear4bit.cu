@@ -36,7 +36,7 @@
 //     go without it: there a cluster of CTAs has a row block, and its sums join in shared memory.
 //
 // Measured, 16384 x 16384 with weights larger than L2: NF4, one row of x in bf16, 32 us; integers
-// with groups of 128, 30 us for one row and 44 us for 32.  In its steady state a unit of NF4
+// with groups of 128, 30 us for one row and 41 us for 32.  In its steady state a unit of NF4
 // takes 0.94 us and one of integers 0.88 us with 32 rows, 85% and 87% of the copy bandwidth; the
 // rest is a start of 3 us, the last CTAs' tail with the partials (3 us), and prep.  Where an
 // fp32 output keeps the codebook to 22 bits, the two table reads per byte from shared memory
