@@ -524,7 +524,8 @@ int nsm_lm_head_nf4(const void* x, int32_t x_dtype, int32_t tokens, const uint8_
  * fp32; x enters as fp16 scaled by a power of two (fp32 x as value + remainder):
  * bf16 is exact down to 2^-31 of the row's largest value, smaller ones are off by
  * at most 2^-39 of it.  The codebook enters as fp16 for fp16 / bf16 outputs and
- * to 22 bits for fp32 ones.  A result does not depend on the other rows of the
+ * to 22 bits for fp32 ones (a value below 2^-8 of the largest is off by at most 2^-29 of
+ * that).  A result does not depend on the other rows of the
  * call and has the same bits every time (and for any number of rows, but for x's
  * values below that border).  The workspace needs no initialisation; calls that
  * share one must not overlap on the GPU, unless nsm_linear4bit_workspace_bytes says

@@ -164,6 +164,32 @@ __device__ __forceinline__ float x_scale_for(float m, float& inv) {
   return __uint_as_float((uint32_t)(e - 14) << 23);
 }
 
+// A codebook entry (scaled) as two fp16, value and remainder (in the upper half), 22 bits.  The
+// value is cut towards zero and the remainder is never 0 beside a value that is not, so that both
+// have one sign: an infinite x times the two is infinite, not NaN.  That costs a value at most
+// 2^-24, 2^-30 of the largest (one below 2^-24 itself, 2^-29 of it).
+__device__ __forceinline__ uint32_t split_code(float c) {
+  const uint32_t sign = __float_as_uint(c) >> 31 << 15;
+  uint32_t h = __half_as_ushort(__float2half_rz(c)), r = 0;
+  if (c != 0.f) {
+    if ((h & 0x7fffu) == 0) h = sign | 1u;
+    const float rem = c - __half2float(__ushort_as_half((unsigned short)h));  // NaN beside an infinity
+    r = __half_as_ushort(__float2half_rn(rem));
+    if (!(fabsf(rem) > 0.f) || (r & 0x7fffu) == 0 || (r & 0x8000u) != sign) r = sign | 1u;
+  }
+  return h | r << 16;
+}
+// The entry as one fp16; what is not 0 stays so, for infinite x.
+__device__ __forceinline__ uint32_t round_code(float c) {
+  const uint32_t h = __half_as_ushort(__float2half_rn(c));
+  return c != 0.f && (h & 0x7fffu) == 0 ? h | 1u : h;
+}
+// The sums of an fp32 x's values and of its remainders.  Infinite weights make the first infinite
+// or NaN, which it then is; the second's sign says nothing.
+__device__ __forceinline__ float join_remainder(float value, float rem) {
+  return fabsf(value) <= 3.4028234e38f ? value + rem : value;
+}
+
 // Eight columns of a row of x on their way to an operand tile.
 struct XRun {
   uint32_t r[8];  // fp32 values, or four words of 16-bit pairs
@@ -501,15 +527,11 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
     const float code = __ldg(p.code + (lane & 15));
     const float mine = fabsf(code) <= 3.4e38f ? fabsf(code) : 0.f;
     const float scaled = code * code_scale_of(warp_max(mine));
+    const uint32_t halves = MODE == kCodeExact ? split_code(scaled) : round_code(scaled);
     uint4* lut4 = reinterpret_cast<uint4*>(smem);
     for (int e = my_warp; e < 256; e += kL4Groups * 5) {  // a warp per byte: 8 lanes fill a table's 32 words
-      const float c0 = __shfl_sync(0xffffffffu, scaled, e >> 4), c1 = __shfl_sync(0xffffffffu, scaled, e & 15);
-      __half h0 = __float2half_rn(c0), h1 = __float2half_rn(c1);
-      if (lane & 8) {
-        h0 = __float2half_rn(c0 - __half2float(h0));
-        h1 = __float2half_rn(c1 - __half2float(h1));
-      }
-      const uint32_t v = (uint32_t)__half_as_ushort(h0) | ((uint32_t)__half_as_ushort(h1) << 16);
+      const uint32_t c0 = __shfl_sync(0xffffffffu, halves, e >> 4), c1 = __shfl_sync(0xffffffffu, halves, e & 15);
+      const uint32_t v = __byte_perm(c0, c1, lane & 8 ? 0x7632 : 0x5410);
       if (lane < (MODE == kCodeExact ? 16 : 8)) lut4[e * 16 + lane] = make_uint4(v, v, v, v);
     }
   }
@@ -848,7 +870,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
         float v = 0.f;
         for (int k = 0; k < p.cluster; ++k) {
           const float* at = sums + (k * p.cols + r) * slice + i;
-          v += p.cols > p.rows ? at[0] + at[p.rows * slice] : at[0];  // the remainders of an fp32 x
+          v += p.cols > p.rows ? join_remainder(at[0], at[p.rows * slice]) : at[0];
         }
         if (!C::kOwnX) v *= __ldcg(p.scale + r);
         if (p.bias) v += load_as_f32(p.bias, p.bias_dt, n);
@@ -891,7 +913,7 @@ __global__ void __launch_bounds__(kL4BlockRows) lin4_finalize_kernel(const float
   const float* src = part + ((int64_t)rb * max_segs * cols + r) * kL4BlockRows + n % kL4BlockRows;
   auto load = [&](int k) {
     const float* at = src + (int64_t)k * cols * kL4BlockRows;
-    return cols > rows ? __ldcg(at) + __ldcg(at + (int64_t)rows * kL4BlockRows) : __ldcg(at);  // the remainders of an fp32 x
+    return cols > rows ? join_remainder(__ldcg(at), __ldcg(at + (int64_t)rows * kL4BlockRows)) : __ldcg(at);
   };
   float v = 0.f;
   if (kShare > 1) {

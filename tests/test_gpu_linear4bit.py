@@ -388,3 +388,53 @@ def test_weights_in_one_launch_and_in_two(dev, N, K):
             y = layer(x, out_dtype=FS)
             _check(y, x, W, b, code)
             assert torch.equal(y, layer(x, out_dtype=FS))
+
+
+def _infinite_check(y, x, W):
+    """Infinite, and of that sign, where the definition is; NaN where that is; else finite."""
+    ref = x.double() @ W.t()
+    assert torch.equal(torch.isnan(y), torch.isnan(ref))
+    inf = torch.isinf(ref)
+    assert torch.equal(torch.isinf(y), inf) and torch.equal(y[inf].double(), ref[inf])
+
+
+@pytest.mark.parametrize("rows", [1, 12])
+@pytest.mark.parametrize("xd,od", [(BF, FS), (FS, FS), (BF, BF), (FH, FH), (FS, FH)])
+def test_infinite_x_with_a_codebook(dev, rows, xd, od):
+    """One infinity in a row: an infinity of the weight's sign, or NaN where the weight is 0."""
+    from next_step_ai_b200.linear4bit import Linear4bit
+
+    N, K = 300, 384
+    p, sc, code, _, _ = _make(N, K, 64, "code", dev, 41)
+    code = code.clone()
+    code[2] = 2.0 ** -33                               # next to nothing, but not nothing
+    layer = Linear4bit(p, sc, out_features=N, in_features=K, group_size=64, code=code)
+    W = _dense(p, sc, code, None, N, K, 64)
+    for value in (float("inf"), -float("inf")):
+        x = torch.randn((rows, K), device=dev).to(xd)
+        x[0, 77] = value
+        x[-1, 200] = value
+        x[rows // 2, 77] = value
+        _infinite_check(layer(x, out_dtype=od), x, W)
+
+
+@pytest.mark.parametrize("rows", [1, 12])
+@pytest.mark.parametrize("xd,od", [(BF, FS), (FS, FS), (BF, BF), (FS, BF)])
+def test_infinite_codebook_entries(dev, rows, xd, od):
+    """An infinite entry gives infinities where a weight uses it, and touches nothing else."""
+    from next_step_ai_b200.linear4bit import Linear4bit
+
+    N, K = 48, 128
+    p, sc, code, _, _ = _make(N, K, 64, "code", dev, 9)
+    code = code.clone()
+    code[15] = float("inf")
+    q = _dense(p, torch.ones_like(sc), torch.arange(16.0, device=dev), None, N, K, 64)
+    p = torch.where((q[:, 0::2] == 15) | (q[:, 1::2] == 15), 0, p.reshape(N, K // 2)).contiguous()
+    p[3, 7] = 0xF1
+    W = _dense(p, sc, code, None, N, K, 64)
+    x = (torch.rand((rows, K), device=dev) + 0.5).to(xd)
+    x[0, 14] *= -1.0
+    layer = Linear4bit(p, sc, out_features=N, in_features=K, group_size=64, code=code)
+    _infinite_check(layer(x, out_dtype=od), x, W)
+    x[-1, 14] = float("inf")
+    _infinite_check(layer(x, out_dtype=od), x, W)
