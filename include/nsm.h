@@ -523,9 +523,10 @@ int nsm_lm_head_nf4(const void* x, int32_t x_dtype, int32_t tokens, const uint8_
  * contiguous).  x, bias and out may be fp32 / fp16 / bf16.  Accumulation is
  * fp32; x enters as fp16 scaled by a power of two (fp32 x as value + remainder):
  * bf16 is exact down to 2^-31 of the row's largest value, smaller ones are off by
- * at most 2^-39 of it.  The codebook enters as fp16 for fp16 / bf16 outputs and
- * to 22 bits for fp32 ones (a value below 2^-8 of the largest is off by at most 2^-29 of
- * that).  A result does not depend on the other rows of the
+ * at most 2^-39 of it.  The codebook enters to 22 bits, as two fp16 (a value
+ * below 2^-8 of the largest is off by at most 2^-29 of that).  nsm_linear4bit_code16 is the
+ * same with the codebook rounded to fp16 (2^-11 of a value), which takes two thirds of the time
+ * on large weights; integers are exact in both.  A result does not depend on the other rows of the
  * call and has the same bits every time (and for any number of rows, but for x's
  * values below that border).  The workspace needs no initialisation; calls that
  * share one must not overlap on the GPU, unless nsm_linear4bit_workspace_bytes says
@@ -553,6 +554,9 @@ size_t nsm_linear4bit_workspace_bytes(int32_t rows, int32_t x_dtype, int32_t out
 int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_stride,
                    const nsm_linear4bit_weights* weights, void* out, int32_t out_dtype, int64_t out_row_stride,
                    void* workspace, size_t workspace_bytes, nsm_stream_t stream);
+int nsm_linear4bit_code16(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_stride,
+                          const nsm_linear4bit_weights* weights, void* out, int32_t out_dtype, int64_t out_row_stride,
+                          void* workspace, size_t workspace_bytes, nsm_stream_t stream);
 
 /* ---- beam search: selection and reordering -------------------------------
  * What follows the logits of a head (nsm_lm_head_nf4, nsm_linear4bit) when

@@ -23,8 +23,8 @@
 //     128 columns; the units, row block by row block, are cut into equal contiguous runs,
 //     one per CTA, so no CTA finishes late.  Bulk copies bring each warpgroup's tile and
 //     scales into its own ring, and x into a ring that all share.  A warpgroup turns its
-//     tile into fp16 (a byte -> half2 table for codebooks, mask and subtract for
-//     integers: both exact but for the codebook's rounding) and stores it to tensor
+//     tile into fp16 (a byte -> half2 table for codebooks, and a second one for what fp16
+//     leaves of a value; mask and subtract for integers, exact) and stores it to tensor
 //     memory; a warp of its own multiplies it with x (tcgen05.mma, M = 128 rows, N = the
 //     columns of x, fp32 accumulation), and then the warpgroup adds scale * product to its
 //     fp32 sums in registers, after it has converted what comes next.  With weights as the M
@@ -35,12 +35,11 @@
 //     bits every time), times the scale of x, + bias, in the output's type.  Small weights
 //     go without it: there a cluster of CTAs has a row block, and its sums join in shared memory.
 //
-// Measured, 16384 x 16384 with weights larger than L2: NF4, one row of x in bf16, 32 us; integers
-// with groups of 128, 30 us for one row and 41 us for 32.  In its steady state a unit of NF4
-// takes 0.94 us and one of integers 0.88 us with 32 rows, 85% and 87% of the copy bandwidth; the
-// rest is a start of 3 us, the last CTAs' tail with the partials (3 us), and prep.  Where an
-// fp32 output keeps the codebook to 22 bits, the two table reads per byte from shared memory
-// bound a unit at 1.64 us (48 us in all).
+// Measured, 16384 x 16384 with weights larger than L2: NF4, one row of x in bf16, 48 us; integers
+// with groups of 128, 30 us for one row and 41 us for 32.  The codebook's 22 bits take two table
+// reads per byte, and shared memory bounds a unit at 1.64 us.  With the codebook rounded to
+// fp16 (32 us) a unit takes 0.94 us, one of integers 0.88 us with 32 rows: 90% and 91% of the copy
+// bandwidth.  The rest is a start of 3 us, the last CTAs' tail with the partials (3 us), and prep.
 #include <algorithm>
 
 #include "nsm_common.cuh"
@@ -60,9 +59,9 @@ constexpr int kL4MaxCols = 32;                        // fp16 columns of x in on
 constexpr int kL4MaxSegs = 32;                        // CTAs that share one row block
 constexpr uint32_t kL4TmemGroup = 128;                // columns of tensor memory per warpgroup
 
-// Kinds of weights: codebook rounded to fp16; codebook as fp16 value +
-// remainder (22 bits, two table reads and two MMAs: outputs in fp32); integers
-// with the zero point 8; integers with a zero point per group.
+// Kinds of weights: codebook rounded to fp16 (where the caller asks for it); codebook as
+// fp16 value + remainder (22 bits, two table reads and two MMAs); integers with the zero
+// point 8; integers with a zero point per group.
 enum { kCode = 0, kCodeExact = 1, kInt = 2, kIntZeros = 3 };
 
 struct Lin4Shape {
@@ -1092,9 +1091,14 @@ size_t nsm_linear4bit_workspace_bytes(int32_t rows, int32_t x_dtype, int32_t out
   return lin4_plan(lin4_shape(out_features, in_features, 32), rows, x_dtype, di).bytes;
 }
 
-int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_stride,
-                   const nsm_linear4bit_weights* w, void* out, int32_t out_dtype, int64_t out_row_stride,
-                   void* workspace, size_t workspace_bytes, nsm_stream_t stream) {
+}  // extern "C"
+
+namespace nsm {
+namespace {
+
+int lin4_run(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_stride, const nsm_linear4bit_weights* w,
+             bool code16, void* out, int32_t out_dtype, int64_t out_row_stride, void* workspace,
+             size_t workspace_bytes, nsm_stream_t stream) {
   auto dtype_ok = [](int d) { return d == NSM_F32 || d == NSM_F16 || d == NSM_BF16; };
   NSM_REQUIRE(w != nullptr, NSM_ERR_INVALID_ARG, "nsm_linear4bit: NULL weights");
   NSM_REQUIRE(dtype_ok(x_dtype) && dtype_ok(out_dtype) && (w->bias == nullptr || dtype_ok(w->bias_dtype)),
@@ -1127,10 +1131,10 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
   float* scale = reinterpret_cast<float*>(ws + pl.scale_off);
   float* part = reinterpret_cast<float*>(ws + pl.part_off);
 
-  // fp32 outputs keep the codebook's values to 22 bits; fp16 and bf16 ones round
-  // it to fp16 (2^-12 of a value at most, random over the columns: about 1e-4 of the output,
-  // half an fp16 rounding), which halves the table reads that bound the kernel
-  const int mode = w->code ? (out_dtype == NSM_F32 ? kCodeExact : kCode) : (w->zeros ? kIntZeros : kInt);
+  // The codebook's values keep 22 bits.  Rounded to fp16 (2^-11 of a value at most, random over
+  // the columns: about 1e-4 of the output) they take half the table reads, which bound the
+  // kernel: that is the caller's choice (nsm_linear4bit_code16).
+  const int mode = w->code ? (code16 ? kCode : kCodeExact) : (w->zeros ? kIntZeros : kInt);
   const int cc = lin4_col_case(pl.cols);
   const bool cluster = pl.cluster > 0;
   const Lin4Fn f = cluster ? lin4_pick<true>(mode, sh.npg, cc) : lin4_pick<false>(mode, sh.npg, cc);
@@ -1184,6 +1188,25 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
                             (const float*)(pl.own_x ? nullptr : scale), pl.units, pl.ctas, sh.steps, pl.max_segs, pl.cols,
                             (int)rows, sh.N, w->bias, (int)w->bias_dtype, out, (int)out_dtype, out_row_stride));
   return NSM_OK;
+}
+
+}  // namespace
+}  // namespace nsm
+
+extern "C" {
+
+int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_stride,
+                   const nsm_linear4bit_weights* w, void* out, int32_t out_dtype, int64_t out_row_stride,
+                   void* workspace, size_t workspace_bytes, nsm_stream_t stream) {
+  return lin4_run(x, x_dtype, rows, x_row_stride, w, false, out, out_dtype, out_row_stride, workspace, workspace_bytes,
+                  stream);
+}
+
+int nsm_linear4bit_code16(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_stride,
+                          const nsm_linear4bit_weights* w, void* out, int32_t out_dtype, int64_t out_row_stride,
+                          void* workspace, size_t workspace_bytes, nsm_stream_t stream) {
+  return lin4_run(x, x_dtype, rows, x_row_stride, w, true, out, out_dtype, out_row_stride, workspace, workspace_bytes,
+                  stream);
 }
 
 }  // extern "C"

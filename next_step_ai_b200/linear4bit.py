@@ -31,13 +31,16 @@ class Linear4bit:
     (uint8, the scales' shape) their zero points, 8 when it is ``None``.  The
     layer keeps copies in its own layout: the arguments may be freed.
 
+    A codebook is held to 22 bits; ``fp16_code=True`` rounds it to fp16 (11 bits), which
+    takes about two thirds of the time on large weights.
+
     Calls on different streams may overlap; a call inside a CUDA graph capture
     takes its scratch memory from the capture's own pool.
     """
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, *, out_features: int, in_features: int,
                  group_size: int = 64, code: torch.Tensor | None = None, zeros: torch.Tensor | None = None,
-                 bias: torch.Tensor | None = None):
+                 bias: torch.Tensor | None = None, fp16_code: bool = False):
         for name, t in (("packed", packed), ("scales", scales), ("zeros", zeros), ("code", code), ("bias", bias)):
             if t is None:
                 continue
@@ -56,6 +59,8 @@ class Linear4bit:
             raise RuntimeError(f"scales has {scales.numel()} values for a [{N}, {K}] weight with group_size {gs}")
         if code is not None and zeros is not None:
             raise RuntimeError("a weight with a codebook has no zero points")
+        if fp16_code and code is None:
+            raise RuntimeError("fp16_code is for weights with a codebook")
         if code is not None and code.numel() != 16:
             raise RuntimeError(f"code has {code.numel()} entries, expected 16")
         if zeros is not None and (zeros.dtype != torch.uint8 or zeros.numel() != N * groups):
@@ -85,28 +90,31 @@ class Linear4bit:
         self._c = _lib.Linear4bitWeightsC(ptr(self.packed), ptr(self.scales), ptr(self.zeros), ptr(self.code),
                                           ptr(self.bias), dtype_code(self.bias.dtype) if bias is not None else 0, N, K, gs)
         self._ref = ctypes.byref(self._c)
+        self._fn = lib.nsm_linear4bit_code16 if fp16_code else lib.nsm_linear4bit
         self._ws_bytes: dict[tuple[int, int], int] = {}
         self._spare = torch.empty(256, dtype=torch.uint8, device=self.device)  # for calls that need no workspace
 
     # ---- construction
     @classmethod
-    def from_param(cls, p, device: torch.device | str = "cuda", bias: torch.Tensor | None = None) -> "Linear4bit":
+    def from_param(cls, p, device: torch.device | str = "cuda", bias: torch.Tensor | None = None,
+                   fp16_code: bool = False) -> "Linear4bit":
         """From a ``checkpoint.Nf4Param`` (host tensors)."""
         if p.in_features % p.blocksize:
             raise RuntimeError(f"{p.name}: quant blocks of {p.blocksize} do not divide the {p.in_features} columns of a row")
         dev = torch.device(device)
         return cls(p.packed.to(dev), p.absmax.to(dev), out_features=p.out_features, in_features=p.in_features,
-                   group_size=p.blocksize, code=p.code.to(dev), bias=bias.to(dev) if bias is not None else None)
+                   group_size=p.blocksize, code=p.code.to(dev), bias=bias.to(dev) if bias is not None else None,
+                   fp16_code=fp16_code)
 
     @classmethod
     def from_checkpoint(cls, ckpt, name: str, device: torch.device | str = "cuda",
-                        bias: torch.Tensor | None = None) -> "Linear4bit":
+                        bias: torch.Tensor | None = None, fp16_code: bool = False) -> "Linear4bit":
         """A quantised weight of an ``Nf4Checkpoint``."""
-        return cls.from_param(ckpt.load_param(name), device, bias)
+        return cls.from_param(ckpt.load_param(name), device, bias, fp16_code)
 
     @classmethod
     def from_dense(cls, weight: torch.Tensor, device: torch.device | str = "cuda", group_size: int = 64,
-                   kind: str = "nf4", bias: torch.Tensor | None = None) -> "Linear4bit":
+                   kind: str = "nf4", bias: torch.Tensor | None = None, fp16_code: bool = False) -> "Linear4bit":
         """A dense ``[N, K]`` weight quantised on the device: ``kind`` ``"nf4"``
         (nearest code value, absmax per group) or ``"int4"`` (round to -7..7,
         absmax / 7 per group).  ``group_size`` must divide ``K``."""
@@ -130,7 +138,7 @@ class Linear4bit:
         else:
             raise RuntimeError(f"unknown kind of 4-bit weight {kind!r} (nf4 or int4)")
         return cls(packed, scales, out_features=N, in_features=K, group_size=group_size, code=code,
-                   bias=bias.to(dev) if bias is not None else None)
+                   bias=bias.to(dev) if bias is not None else None, fp16_code=fp16_code)
 
     # ---- forward
     def max_rows_per_call(self, dtype: torch.dtype) -> int:
@@ -184,7 +192,7 @@ class Linear4bit:
             if need is None:
                 need = self._ws_bytes[(n, xc)] = int(lib.nsm_linear4bit_workspace_bytes(n, xc, N, self.in_features))
             ws = self._spare if need == 256 else torch.empty(need, dtype=torch.uint8, device=dev)
-            status = lib.nsm_linear4bit(xp, xc, n, stride, self._ref, op, oc, N, ws.data_ptr(), need, stream)
+            status = self._fn(xp, xc, n, stride, self._ref, op, oc, N, ws.data_ptr(), need, stream)
             if status:
                 _lib.check(status, "nsm_linear4bit")
             rows -= n

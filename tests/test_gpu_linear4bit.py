@@ -438,3 +438,54 @@ def test_infinite_codebook_entries(dev, rows, xd, od):
     _infinite_check(layer(x, out_dtype=od), x, W)
     x[-1, 14] = float("inf")
     _infinite_check(layer(x, out_dtype=od), x, W)
+
+
+def _one_column_rows(dev, rows, K, dtype):
+    """Rows with a single 1.0 each, in different columns."""
+    x = torch.zeros((rows, K), device=dev, dtype=dtype)
+    at = (torch.arange(rows, device=dev) * 37 + 5) % K
+    x[torch.arange(rows, device=dev), at] = 1.0
+    return x, at
+
+
+@pytest.mark.parametrize("N,K,rows", [(700, 320, 1), (700, 320, 12), (4096, 4096, 8), (1024, 8192, 32)])
+@pytest.mark.parametrize("xd,od", [(BF, BF), (FH, FH), (BF, FH), (FS, FS)])
+def test_one_column_gives_the_weight_rounded_once(dev, N, K, rows, xd, od):
+    """A row of x with a single 1.0 gives a column of W: off by the output's rounding, 2^-22 for
+    the codebook as two fp16, and 2^-23 for the product with the scale (at most 2^-24 each of
+    two roundings); the other columns add exact zeros."""
+    from next_step_ai_b200.linear4bit import Linear4bit
+
+    p, sc, code, _, _ = _make(N, K, 64, "code", dev, N + rows)
+    layer = Linear4bit(p, sc, out_features=N, in_features=K, group_size=64, code=code)
+    W = _dense(p, sc, code, None, N, K, 64)
+    x, at = _one_column_rows(dev, rows, K, xd)
+    ref = W[:, at].t()
+    rel = 2.0 ** -22 + 2.0 ** -23
+    bound = (torch.finfo(od).eps / 2 * (1 + rel) + rel) * ref.abs()
+    assert bool(((layer(x, out_dtype=od).double() - ref).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("od", [BF, FH, FS])
+def test_codebook_rounded_to_fp16_where_asked(dev, od):
+    """``fp16_code``: the definition with a codebook that fp16 rounded, in any output type; a power
+    of two before the rounding keeps it out of the subnormal numbers."""
+    from next_step_ai_b200.linear4bit import Linear4bit
+
+    for N, K, rows in ((700, 322, 1), (4096, 4096, 8), (1030, 2048, 32)):
+        p, sc, code, _, b = _make(N, K, 64, "code", dev, N + rows, FS, FS)
+        mk = dict(out_features=N, in_features=K, group_size=64, code=code, bias=b)
+        layer = Linear4bit(p, sc, fp16_code=True, **mk)
+        x = torch.randn((rows, K), device=dev, dtype=BF)
+        y = layer(x, out_dtype=od)
+        _check(y, x, _dense(p, sc, (code * 64).half().float() / 64, None, N, K, 64), b, code)
+        if od == FS:
+            assert not torch.equal(y, Linear4bit(p, sc, **mk)(x, out_dtype=od))
+        x[0, 9] = float("inf")
+        _infinite_check(layer(x, out_dtype=od)[:1], x[:1], _dense(p, sc, code, None, N, K, 64))
+    with pytest.raises(RuntimeError, match="with a codebook"):
+        Linear4bit(p, sc, out_features=N, in_features=K, group_size=64, fp16_code=True)
+    w = torch.randn((64, 128), device=dev)
+    a, c = Linear4bit.from_dense(w, fp16_code=True), Linear4bit.from_dense(w)
+    x = torch.randn((2, 128), device=dev)
+    assert not torch.equal(a(x), c(x))
