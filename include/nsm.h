@@ -554,6 +554,10 @@ size_t nsm_linear4bit_workspace_bytes(int32_t rows, int32_t x_dtype, int32_t out
 int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_stride,
                    const nsm_linear4bit_weights* weights, void* out, int32_t out_dtype, int64_t out_row_stride,
                    void* workspace, size_t workspace_bytes, nsm_stream_t stream);
+/* Tries of each wait inside these kernels, instead of nsm_set_copy_wait_limit's: 0 = that one
+ * (the default); -1 = none, so that every wait gives up at once (to test what follows then).
+ * Process-wide, for later launches. */
+int nsm_linear4bit_set_wait_limit(int32_t tries);
 int nsm_linear4bit_code16(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_stride,
                           const nsm_linear4bit_weights* weights, void* out, int32_t out_dtype, int64_t out_row_stride,
                           void* workspace, size_t workspace_bytes, nsm_stream_t stream);

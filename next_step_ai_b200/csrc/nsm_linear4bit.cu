@@ -58,6 +58,7 @@ constexpr int kL4BlockRows = kL4TileRows * kL4Groups;  // rows of a unit
 constexpr int kL4MaxCols = 32;                        // fp16 columns of x in one call
 constexpr int kL4MaxSegs = 32;                        // CTAs that share one row block
 constexpr uint32_t kL4TmemGroup = 128;                // columns of tensor memory per warpgroup
+constexpr int kL4BarBytes = 640;                      // of Lin4Bars
 
 // Kinds of weights: codebook rounded to fp16 (where the caller asks for it); codebook as
 // fp16 value + remainder (22 bits, two table reads and two MMAs); integers with the zero
@@ -430,7 +431,7 @@ struct Lin4Config {
   static constexpr int kLut = kIsCode ? kLutBytes : 0;
   static constexpr int kRing = kLut, kX = kRing + kL4Groups * kStages * kStageBytes;
   static constexpr int kBars = kX + kL4XStages * kXBytes + 1024;  // the last tile of x is read 128 bytes over
-  static constexpr int kSmem = kBars + 512;
+  static constexpr int kSmem = kBars + kL4BarBytes;
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
   static_assert(kX - kRing >= kL4BlockRows * NC * 4, "a cluster's sums fit the rings");
 };
@@ -445,8 +446,10 @@ struct Lin4Bars {
   unsigned long long dead[2];               // where a warp arrives instead of at `full` after a failure
   float x_scale[kL4XStages][8];             // kOwnX: what a tile's columns of x were divided by
   uint32_t tmem;
+  int asked[kL4XStages];   // by the warps that bring tiles, at their end: the last unit whose weights each asked for
+  int failed[kL4XStages];  // and whether a wait of theirs ran out
 };
-static_assert(sizeof(Lin4Bars) <= 512, "barriers");
+static_assert(sizeof(Lin4Bars) <= kL4BarBytes, "barriers");
 
 template <int MODE, int NPG, int NC, bool kCluster>
 __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_constant__ Lin4Params p) {
@@ -608,11 +611,24 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
       }
     }
     // Nothing may arrive in shared memory that is gone: the last commits (they come after the
-    // copies they waited for), and after a failure the copies under way.
+    // copies they waited for), and after a failure the copies under way.  The units that use a
+    // warp's last copies may be another's to wait for, so a failure of one is a failure of all;
+    // and where another has filled the same place of the ring since, these were waited for.
     if (lane == 0 && x_last >= 0 && ok) ok = mbar_wait(free, x_last & 1, p.wait_limit);
     ok = __shfl_sync(0xffffffffu, ok, 0);
-    if (!ok) {
-      if (lane < kL4Groups && w_last >= 0 && (u0 + w_last) / p.steps * kL4Groups + lane < p.row_tiles)
+    if (lane == 0) {
+      bars.asked[st] = w_last;
+      bars.failed[st] = !ok;
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(kL4XStages * 32) : "memory");
+    bool failed = false, newest = w_last >= 0;
+#pragma unroll
+    for (int o = 0; o < kL4XStages; ++o) {
+      failed |= bars.failed[o] != 0;
+      newest &= !(bars.asked[o] > w_last && bars.asked[o] % C::kStages == w_last % C::kStages);
+    }
+    if (failed) {
+      if (lane < kL4Groups && newest && (u0 + w_last) / p.steps * kL4Groups + lane < p.row_tiles)
         mbar_wait(smem_u32(&bars.w_full[lane][w_last % C::kStages]), (w_last / C::kStages) & 1);
       if (!C::kOwnX && lane == 0 && x_last >= 0) mbar_wait(full, x_last & 1);
     }
@@ -942,6 +958,13 @@ __global__ void __launch_bounds__(kL4BlockRows) lin4_finalize_kernel(const float
   store_from_f32(out, out_dt, (int64_t)r * out_stride + n, v);
 }
 
+// Tries of a wait: 0 = copy_wait_spins(), -1 = none.
+std::atomic<int> g_lin4_wait{0};
+int lin4_wait_limit() {
+  const int tries = g_lin4_wait.load(std::memory_order_relaxed);
+  return tries == 0 ? copy_wait_spins() : std::max(tries, 0);
+}
+
 struct Lin4Plan {
   bool own_x = false;  // few columns: the kernel reads x itself
   int cluster = 0;     // CTAs of a row block in one launch, 0: partials and lin4_finalize_kernel
@@ -1051,6 +1074,12 @@ size_t nsm_linear4bit_scale_count(int32_t out_features, int32_t in_features, int
 }
 
 int nsm_linear4bit_max_rows(int32_t x_dtype) { return lin4_max_rows(x_dtype); }
+
+int nsm_linear4bit_set_wait_limit(int32_t tries) {
+  NSM_REQUIRE(tries >= -1, NSM_ERR_INVALID_ARG, "nsm_linear4bit_set_wait_limit: tries must be >= -1");
+  g_lin4_wait.store(tries, std::memory_order_relaxed);
+  return NSM_OK;
+}
 
 int nsm_linear4bit_pack(const uint8_t* packed, int64_t packed_row_bytes, const void* scales, int32_t scale_dtype,
                         const uint8_t* zeros, int32_t out_features, int32_t in_features, int32_t group_size,
@@ -1165,7 +1194,7 @@ int lin4_run(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_stride,
   p.units = pl.units;
   p.ctas = pl.ctas;
   p.max_segs = pl.max_segs;
-  p.wait_limit = copy_wait_spins();
+  p.wait_limit = lin4_wait_limit();
   p.cluster = pl.cluster;
   p.N = sh.N;
   p.scale = scale;

@@ -1,0 +1,65 @@
+"""``nsm_linear4bit`` when its waits run out: without a GPU fault, every wait gives up at
+once (``nsm_linear4bit_set_wait_limit(-1)``).  Copies that were asked for are waited for
+with the ordinary limit before a CTA ends, and the next call is as if nothing had been."""
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+BF, FH, FS = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from next_step_ai_b200 import _lib
+
+    _lib.load()
+    return torch.device("cuda", 0)
+
+
+@pytest.fixture
+def no_tries(dev):
+    """Sets the limit to none; the ordinary one is back after the test."""
+    from next_step_ai_b200 import _lib
+
+    lib = _lib.load()
+
+    def set_to(tries):
+        torch.cuda.synchronize()
+        _lib.check(lib.nsm_linear4bit_set_wait_limit(tries), "nsm_linear4bit_set_wait_limit")
+
+    yield set_to
+    set_to(0)
+
+
+def _layer(dev, N, K, kind, fp16_code=False):
+    from next_step_ai_b200.linear4bit import Linear4bit
+    from next_step_ai_b200.nf4 import nf4_code
+
+    gen = torch.Generator(device=dev).manual_seed(N + K)
+    p = torch.randint(0, 256, (N, K // 2), dtype=torch.uint8, device=dev, generator=gen)
+    sc = (torch.rand((N, -(-K // 64)), device=dev, generator=gen) + 0.5) * 0.02
+    z = torch.randint(0, 16, sc.shape, dtype=torch.uint8, device=dev, generator=gen) if kind == "zeros" else None
+    return Linear4bit(p, sc, out_features=N, in_features=K, group_size=64, zeros=z, fp16_code=fp16_code,
+                      code=nf4_code(dev) if kind == "code" else None)
+
+
+# a cluster's CTAs and partials; the kernel's own tiles of x and those laid out before; rings of
+# three and four places; fewer units than places, and many
+@pytest.mark.parametrize("N,K", [(40, 128), (600, 2048), (4096, 4096), (4096, 16384), (20000, 1024)])
+@pytest.mark.parametrize("kind,fp16_code", [("code", False), ("code", True), ("zeros", False), ("sym", False)])
+@pytest.mark.parametrize("rows,xd", [(1, BF), (8, FH), (9, BF), (16, FS)])
+def test_waits_that_give_up_at_once(dev, no_tries, N, K, kind, fp16_code, rows, xd):
+    layer = _layer(dev, N, K, kind, fp16_code)
+    x = torch.randn((rows, K), device=dev).to(xd)
+    want = layer(x)
+    no_tries(-1)
+    y = layer(x)
+    no_tries(0)
+    assert bool(torch.isnan(y).all())
+    assert torch.equal(layer(x), want)

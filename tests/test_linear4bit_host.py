@@ -74,3 +74,9 @@ def test_quant_blocks_across_rows_are_refused():
     p = Nf4Param("w", torch.zeros(96, dtype=torch.uint8), torch.zeros(3), torch.zeros(16), 2, 96, 64, "nf4", "float16")
     with pytest.raises(RuntimeError, match="do not divide"):
         linear4bit.Linear4bit.from_param(p, "cpu")
+
+
+def test_wait_limit_is_validated(lib):
+    assert lib.nsm_linear4bit_set_wait_limit(-2) == _lib.NSM_ERR_INVALID_ARG
+    assert lib.nsm_linear4bit_set_wait_limit(1000) == _lib.NSM_OK
+    assert lib.nsm_linear4bit_set_wait_limit(0) == _lib.NSM_OK
