@@ -531,7 +531,8 @@ int nsm_lm_head_nf4(const void* x, int32_t x_dtype, int32_t tokens, const uint8_
  * values below that border).  The workspace needs no initialisation; calls that
  * share one must not overlap on the GPU, unless nsm_linear4bit_workspace_bytes says
  * 256: such a call does not touch it.  A wait inside the kernel that runs out
- * (nsm_set_copy_wait_limit) leaves NaN in the outputs it concerns. */
+ * (nsm_set_copy_wait_limit) leaves NaN in the outputs it concerns, and NSM_ERR_TIMEOUT in
+ * the device's error word (nsm_linear4bit_error). */
 typedef struct nsm_linear4bit_weights {
   const uint8_t* packed; /* tiled, from nsm_linear4bit_pack */
   const float* scales;   /* tiled */
@@ -554,6 +555,10 @@ size_t nsm_linear4bit_workspace_bytes(int32_t rows, int32_t x_dtype, int32_t out
 int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_stride,
                    const nsm_linear4bit_weights* weights, void* out, int32_t out_dtype, int64_t out_row_stride,
                    void* workspace, size_t workspace_bytes, nsm_stream_t stream);
+/* The error word of these kernels on the current device: *code_out = NSM_ERR_TIMEOUT when a
+ * wait of an earlier call ran out, else 0; the word is cleared.  Synchronises `stream`.  The
+ * calls do not clear the word, so one check after several covers them all. */
+int nsm_linear4bit_error(int32_t* code_out, nsm_stream_t stream);
 /* Tries of each wait inside these kernels, instead of nsm_set_copy_wait_limit's: 0 = that one
  * (the default); -1 = none, so that every wait gives up at once (to test what follows then).
  * Process-wide, for later launches. */

@@ -47,7 +47,7 @@ EXPORTED = (
     "nsm_decode_token", "nsm_token_profile",
     "nsm_linear4bit_packed_bytes", "nsm_linear4bit_scale_count", "nsm_linear4bit_max_rows", "nsm_linear4bit_pack",
     "nsm_linear4bit_workspace_bytes", "nsm_linear4bit", "nsm_linear4bit_code16",
-    "nsm_linear4bit_set_wait_limit",
+    "nsm_linear4bit_set_wait_limit", "nsm_linear4bit_error",
     "nsm_beam_select_workspace_bytes", "nsm_beam_select", "nsm_beam_states_bytes", "nsm_beam_states_set",
     "nsm_beam_reorder",
 )
@@ -174,6 +174,7 @@ _SIGS = {
     "nsm_linear4bit": (c_int, [c_void_p, c_int32, c_int32, c_int64, POINTER(Linear4bitWeightsC), c_void_p, c_int32,
                                c_int64, c_void_p, c_size_t, c_void_p]),
     "nsm_linear4bit_set_wait_limit": (c_int, [c_int32]),
+    "nsm_linear4bit_error": (c_int, [POINTER(c_int32), c_void_p]),
     "nsm_linear4bit_code16": (c_int, [c_void_p, c_int32, c_int32, c_int64, POINTER(Linear4bitWeightsC), c_void_p, c_int32,
                                c_int64, c_void_p, c_size_t, c_void_p]),
     "nsm_beam_select_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32]),

@@ -261,6 +261,13 @@ class BeamSearch:
         self.length += 1
         return tokens
 
+    def error(self) -> int:
+        """The head's error word, read and cleared (``Linear4bit.error``; 0 for a head that
+        has none).  Not 0: logits were NaN, which no candidate comes from, so the tokens since
+        the last check are not the best ones.  Synchronises; once after a decode is enough."""
+        read = getattr(self.head, "error", None)
+        return int(read()) if read is not None else 0
+
     def sequences(self) -> torch.Tensor:
         """The tokens so far, ``[batch, beams, length]``, best beam first."""
         return self.history.view(self.batch, self.beams, -1)[:, :, :self.length]

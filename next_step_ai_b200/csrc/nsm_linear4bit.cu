@@ -292,6 +292,9 @@ __global__ void __launch_bounds__(256) lin4_prep_kernel(const void* x, int dt, i
 }
 
 // ---- products -------------------------------------------------------------------
+__device__ int g_lin4_error;  // a wait ran out: NSM_ERR_TIMEOUT until nsm_linear4bit_error reads it
+__device__ __forceinline__ void lin4_failed() { atomicCAS(&g_lin4_error, 0, NSM_ERR_TIMEOUT); }
+
 struct Lin4Params {
   const uint8_t* w;
   const float* s;
@@ -544,7 +547,8 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
 
   // Every wait is bounded.  After one that ran out nothing more is copied, multiplied or handed
   // on, so the waits that depend on it run out too, and the warpgroups that saw one leave NaN in
-  // their partials.  Copies and MMAs under way are waited for before the CTA ends.
+  // their partials and record NSM_ERR_TIMEOUT.  Copies and MMAs under way are waited for before
+  // the CTA ends.
   if (bringing) {
     // ---- tiles: each of these warps fills one place of x's ring, and when all MMAs that read it
     // are done, so that all warpgroups have read their weights of that unit too, the place of those
@@ -628,6 +632,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
       newest &= !(bars.asked[o] > w_last && bars.asked[o] % C::kStages == w_last % C::kStages);
     }
     if (failed) {
+      if (lane == 0) lin4_failed();
       if (lane < kL4Groups && newest && (u0 + w_last) / p.steps * kL4Groups + lane < p.row_tiles)
         mbar_wait(smem_u32(&bars.w_full[lane][w_last % C::kStages]), (w_last / C::kStages) & 1);
       if (!C::kOwnX && lane == 0 && x_last >= 0) mbar_wait(full, x_last & 1);
@@ -859,6 +864,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
         add_round(slots - kSlots + t, t % kSlotsPerScale == kSlotsPerScale - 1, ps + t * NPG / kSlots, pxs);
       if (!kCluster) flush();
     }
+    if (!ok) lin4_failed();
     __syncwarp();
     tmem_fence_before();
     if constexpr (kCluster) {
@@ -1074,6 +1080,19 @@ size_t nsm_linear4bit_scale_count(int32_t out_features, int32_t in_features, int
 }
 
 int nsm_linear4bit_max_rows(int32_t x_dtype) { return lin4_max_rows(x_dtype); }
+
+int nsm_linear4bit_error(int32_t* code_out, nsm_stream_t stream) {
+  NSM_REQUIRE(code_out != nullptr, NSM_ERR_INVALID_ARG, "nsm_linear4bit_error: code_out is NULL");
+  void* word = nullptr;
+  NSM_CHECK_CUDA(cudaGetSymbolAddress(&word, g_lin4_error));
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  int32_t v = 0;
+  NSM_CHECK_CUDA(cudaMemcpyAsync(&v, word, sizeof(int32_t), cudaMemcpyDeviceToHost, s));
+  NSM_CHECK_CUDA(cudaMemsetAsync(word, 0, sizeof(int32_t), s));
+  NSM_CHECK_CUDA(cudaStreamSynchronize(s));
+  *code_out = v;
+  return NSM_OK;
+}
 
 int nsm_linear4bit_set_wait_limit(int32_t tries) {
   NSM_REQUIRE(tries >= -1, NSM_ERR_INVALID_ARG, "nsm_linear4bit_set_wait_limit: tries must be >= -1");

@@ -148,6 +148,16 @@ class Linear4bit:
         return sum(t.numel() * t.element_size() for t in (self.packed, self.scales, self.zeros, self.code, self.bias)
                    if t is not None)
 
+    def error(self) -> int:
+        """Read and clear the error word of the layers on this device (``NSM_ERR_TIMEOUT``:
+        a wait inside a kernel ran out and outputs of a call since the last check are NaN;
+        0: all is well).  Synchronises."""
+        code = ctypes.c_int32(0)
+        with torch.cuda.device(self.device):
+            _lib.check(self._lib.nsm_linear4bit_error(ctypes.byref(code), stream_handle(self.device)),
+                       "nsm_linear4bit_error")
+        return int(code.value)
+
     def __call__(self, x: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
         return self.forward(x, out_dtype)
 

@@ -63,3 +63,49 @@ def test_waits_that_give_up_at_once(dev, no_tries, N, K, kind, fp16_code, rows, 
     no_tries(0)
     assert bool(torch.isnan(y).all())
     assert torch.equal(layer(x), want)
+
+
+@pytest.mark.parametrize("N,K,rows,xd", [(4096, 4096, 1, BF), (4096, 4096, 9, BF), (4096, 16384, 1, FS),
+                                         (4096, 16384, 16, FS)])
+@pytest.mark.parametrize("kind", ["code", "zeros"])
+def test_a_failed_wait_is_recorded(dev, no_tries, N, K, rows, xd, kind):
+    """The word keeps the failure over later calls, of any layer on the device, and until it is read."""
+    from next_step_ai_b200 import _lib
+
+    layer, other = _layer(dev, N, K, kind), _layer(dev, 40, 128, kind)
+    x = torch.randn((rows, K), device=dev).to(xd)
+    layer.error()
+    layer(x)
+    assert layer.error() == 0
+    no_tries(-1)
+    layer(x)
+    no_tries(0)
+    layer(x)
+    assert other.error() == _lib.NSM_ERR_TIMEOUT
+    assert other.error() == 0 and layer.error() == 0
+
+
+def test_a_search_tells_of_its_heads_failure(dev, no_tries):
+    """A failed head's NaN logits are no candidates: the search says so, and a head without an error
+    word has none."""
+    from next_step_ai_b200 import BeamSearch, _lib
+
+    head = _layer(dev, 1000, 256, "code")
+    search = BeamSearch(head, 2, 3, max_tokens=8)
+    head.error()
+    hidden = torch.randn((6, 256), device=dev, dtype=BF)
+    search.step(hidden)
+    assert search.error() == 0
+    no_tries(-1)
+    search.step(hidden)
+    no_tries(0)
+    search.step(hidden)
+    assert search.error() == _lib.NSM_ERR_TIMEOUT and search.error() == 0
+
+    class Plain:
+        device = dev
+
+        def __call__(self, hidden, out_dtype):
+            return torch.zeros((hidden.shape[0], 50), device=dev, dtype=out_dtype)
+
+    assert BeamSearch(Plain(), 2, 3, max_tokens=8).error() == 0

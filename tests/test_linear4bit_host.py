@@ -80,3 +80,7 @@ def test_wait_limit_is_validated(lib):
     assert lib.nsm_linear4bit_set_wait_limit(-2) == _lib.NSM_ERR_INVALID_ARG
     assert lib.nsm_linear4bit_set_wait_limit(1000) == _lib.NSM_OK
     assert lib.nsm_linear4bit_set_wait_limit(0) == _lib.NSM_OK
+
+
+def test_error_word_needs_somewhere_to_go(lib):
+    assert lib.nsm_linear4bit_error(None, None) == _lib.NSM_ERR_INVALID_ARG
