@@ -522,13 +522,13 @@ int nsm_lm_head_nf4(const void* x, int32_t x_dtype, int32_t tokens, const uint8_
  * x rows are x_row_stride elements apart, out rows out_row_stride (each row
  * contiguous).  x, bias and out may be fp32 / fp16 / bf16.  Accumulation is
  * fp32; x enters as fp16 scaled by a power of two (fp32 x as value + remainder):
- * bf16 is exact down to 2^-31 of the row's largest value, smaller ones are off by
- * at most 2^-39 of it.  The codebook enters to 22 bits, as two fp16 (a value
+ * bf16 is exact down to 2^-30 of the row's largest value, smaller ones are off by
+ * at most 2^-38 of it.  The codebook enters to 22 bits, as two fp16 (a value
  * below 2^-8 of the largest is off by at most 2^-29 of that).  nsm_linear4bit_code16 is the
  * same with the codebook rounded to fp16 (2^-11 of a value), which takes two thirds of the time
  * on large weights; integers are exact in both.  A result does not depend on the other rows of the
  * call and has the same bits every time (and for any number of rows, but for x's
- * values below that border).  The workspace needs no initialisation; calls that
+ * values below that border and for results below 2^-100).  The workspace needs no initialisation; calls that
  * share one must not overlap on the GPU, unless nsm_linear4bit_workspace_bytes says
  * 256: such a call does not touch it.  A wait inside the kernel that runs out
  * (nsm_set_copy_wait_limit) leaves NaN in the outputs it concerns, and NSM_ERR_TIMEOUT in

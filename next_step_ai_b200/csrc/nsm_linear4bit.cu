@@ -17,8 +17,8 @@
 //     down to 2^-31 of the row's largest value (below that off by at most 2^-39 of it); an
 //     fp32 x becomes two fp16 columns, value and remainder: 22 bits.  x is written as the 8 x
 //     16-byte core matrices of a K-major tensor-core operand.  For up to 8 columns lin4_kernel
-//     does this itself, with a scale for each 128 columns of a row: one launch and 5 us less at
-//     16384 columns;
+//     does this itself, with a scale for each 128 columns of a row, that brings their largest to
+//     [2^13, 2^15): one launch and 5 us less at 16384 columns;
 //  2. lin4_kernel: one CTA per SM, four warpgroups of 128 rows each.  A unit is 512 rows x
 //     128 columns; the units, row block by row block, are cut into equal contiguous runs,
 //     one per CTA, so no CTA finishes late.  Bulk copies bring each warpgroup's tile and
@@ -140,11 +140,12 @@ __global__ void lin4_pack_scales_kernel(const void* __restrict__ scales, int dt,
 }
 
 // ---- activations ----------------------------------------------------------------
-// Power of two that brings the largest |code| (m) to [64, 128): the remainders of the
-// exact codebook then stay normal fp16 numbers.
+// An even power of two (see x_scale_root) that brings the largest |code| (m) to [64, 256): the
+// remainders of the exact codebook then stay normal fp16 numbers.
 __device__ __forceinline__ float code_scale_of(float m) {
   if (!(m > 0.f)) return 1.f;
-  return ldexpf(1.f, max(-120, min(120, 6 - ilogbf(m))));
+  const int e = 6 - ilogbf(m);
+  return ldexpf(1.f, max(-120, min(120, e + (e & 1))));
 }
 __device__ __forceinline__ float code_scale(const float* code) {
   float m = 0.f;
@@ -162,6 +163,20 @@ __device__ __forceinline__ float x_scale_for(float m, float& inv) {
   const int e = max(16, (int)(__float_as_uint(m) >> 23));
   inv = __uint_as_float((uint32_t)(268 - e) << 23);
   return __uint_as_float((uint32_t)(e - 14) << 23);
+}
+
+// Of a tile of x: what its products are multiplied by is 2^(2 j), and half of it, 2^j, goes to the
+// product and half to the weights' scale.  As one factor it would make that scale subnormal for a
+// tiny x, and the product infinite for a large one.  Scales s and inv of x (powers of two) are
+// moved so that the exponent is even; icode, what the codebook's scale takes back, has one.
+__device__ __forceinline__ float x_scale_root(float& s, float& inv, float icode) {
+  const int e = (int)(__float_as_uint(s) >> 23) - 127;
+  if (e & 1) {
+    s *= 2.f;
+    inv *= 0.5f;
+  }
+  const int j = ((int)(__float_as_uint(s) >> 23) - 127 + (int)(__float_as_uint(icode) >> 23) - 127) / 2;
+  return __uint_as_float((uint32_t)(127 + j) << 23);
 }
 
 // A codebook entry (scaled) as two fp16, value and remainder (in the upper half), 22 bits.  The
@@ -447,7 +462,7 @@ struct Lin4Bars {
   unsigned long long x_free[kL4XStages];    // all warpgroups' MMAs that read it are done
   unsigned long long drained[kL4Groups];    // all of the warpgroup's MMAs are done
   unsigned long long dead[2];               // where a warp arrives instead of at `full` after a failure
-  float x_scale[kL4XStages][8];             // kOwnX: what a tile's columns of x were divided by
+  float x_scale[kL4XStages][8];             // kOwnX: of a tile's columns of x (x_scale_root)
   uint32_t tmem;
   int asked[kL4XStages];   // by the warps that bring tiles, at their end: the last unit whose weights each asked for
   int failed[kL4XStages];  // and whether a wait of theirs ran out
@@ -593,14 +608,15 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
             for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             s = x_scale_for(m, inv);
           }
+          const float root = x_scale_root(s, inv, icode);
           v[q].to_half(p.x_dtype, inv, hi, lo);
           if (r < p.rows) {
             // core matrices of 8 columns of x by 8 of the weight: [k / 8][c][k % 8]
             *reinterpret_cast<uint4*>(dst + ((lane & 15) * 8 + r) * 16) = hi;
-            if ((lane & 15) == 0) bars.x_scale[st][r] = s * icode;
+            if ((lane & 15) == 0) bars.x_scale[st][r] = root;
             if (p.x_dtype == NSM_F32) {
               *reinterpret_cast<uint4*>(dst + ((lane & 15) * 8 + p.rows + r) * 16) = lo;
-              if ((lane & 15) == 0) bars.x_scale[st][p.rows + r] = s * icode;
+              if ((lane & 15) == 0) bars.x_scale[st][p.rows + r] = root;
             }
           }
         }
@@ -737,13 +753,17 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
             tmem_ld<kLd>(mine + d_col + g * C::kN + c0, r);
             tmem_wait_ld<kLd>(r);
             if constexpr (NC == 1) {
-              acc1 = fmaf(s[g] * xs[0], __uint_as_float(r[0]), acc1);
+              acc1 = fmaf(s[g] * xs[0], __uint_as_float(r[0]) * xs[0], acc1);
             } else {
 #pragma unroll
               for (int c = 0; c < kLd; c += 2) {
-                unsigned long long sc = pair2(s[g], s[g]);
-                if constexpr (C::kOwnX) sc = mul2(sc, pair2(xs[c0 + c], xs[c0 + c + 1]));  // (x's are powers of two)
-                acc[(c0 + c) / 2] = fma2(sc, pair2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), acc[(c0 + c) / 2]);
+                unsigned long long sc = pair2(s[g], s[g]), d = pair2(__uint_as_float(r[c]), __uint_as_float(r[c + 1]));
+                if constexpr (C::kOwnX) {  // (powers of two: exact)
+                  const unsigned long long root = pair2(xs[c0 + c], xs[c0 + c + 1]);
+                  sc = mul2(sc, root);
+                  d = mul2(d, root);
+                }
+                acc[(c0 + c) / 2] = fma2(sc, d, acc[(c0 + c) / 2]);
               }
             }
           }

@@ -489,3 +489,47 @@ def test_codebook_rounded_to_fp16_where_asked(dev, od):
     a, c = Linear4bit.from_dense(w, fp16_code=True), Linear4bit.from_dense(w)
     x = torch.randn((2, 128), device=dev)
     assert not torch.equal(a(x), c(x))
+
+
+@pytest.mark.parametrize("xd", [BF, FS])
+@pytest.mark.parametrize("kind,mul", [("code", 1.0), ("code", 1.7e-3), ("sym", 1.0)])
+def test_tiny_x(dev, xd, kind, mul):
+    """Rows down to 1e-35: as exact as others (a result is at least 2^-120 or so, a normal number),
+    whether the kernel lays x out itself (one row, eight) or not.  The two give the same bits where
+    results are 2^-100 and more.  Below, sums on the way may be subnormal numbers in the first
+    (those of an fp32 x's remainders, 2^-11 of the others and less, before the rest): they round by
+    up to 2^-150, and that can turn a later rounding, of a sum of any size, by a whole step of its
+    own.  Both stay within the definition's bound."""
+    from next_step_ai_b200.linear4bit import Linear4bit
+
+    N, K = 300, 512
+    p, sc, code, _, _ = _make(N, K, 64, kind, dev, 51)
+    code = code * mul if code is not None else None
+    sc = sc / mul
+    layer = Linear4bit(p, sc, out_features=N, in_features=K, group_size=64, code=code)
+    W = _dense(p, sc, code, None, N, K, 64)
+    many = 16 if xd == FS else 32
+    for size in (1e-27, 1e-30, 1e-32, 1e-33, 1e-34, 1e-35):
+        x = (torch.randn((many, K), device=dev) * size).to(xd)
+        y = layer(x, out_dtype=FS)
+        # (the definition's bound times 2^60: _check allows a smallest normal number otherwise)
+        _check(y.double().mul(2.0 ** 60).float(), x.float() * 2.0 ** 60, W, None, code)
+        for n in (1, 3, many // 4):
+            own, same = layer(x[:n], out_dtype=FS), y[:n].abs() >= 2.0 ** -100
+            assert size < 1e-27 or bool(same.any())
+            assert torch.equal(own[same], y[:n][same])
+            _check(own.double().mul(2.0 ** 60).float(), x[:n].float() * 2.0 ** 60, W, None, code)
+
+
+def test_large_x_with_small_scales(dev):
+    """Products of x and the codebook past fp32's range, brought back by the scales."""
+    from next_step_ai_b200.linear4bit import Linear4bit
+
+    N, K = 130, 256
+    p, sc, code, _, _ = _make(N, K, 64, "code", dev, 52)
+    code, sc = code * 2.0 ** 20, sc * 2.0 ** -40
+    layer = Linear4bit(p, sc, out_features=N, in_features=K, group_size=64, code=code)
+    W = _dense(p, sc, code, None, N, K, 64)
+    for xd, rows in ((BF, 1), (BF, 9), (FS, 2), (FS, 16)):
+        x = (torch.randn((rows, K), device=dev) * 2.0 ** 120).to(xd)
+        _check(layer(x, out_dtype=FS), x, W, None, code)
