@@ -86,7 +86,7 @@ class Linear4bit:
                                                gs, int(code is not None), self.packed.data_ptr(), self.scales.data_ptr(),
                                                ptr(self.zeros), stream_handle(self.device)), "nsm_linear4bit_pack")
             self.code = code.reshape(-1).to(torch.float32, copy=True) if code is not None else None
-            self.bias = bias.reshape(-1).contiguous() if bias is not None else None
+            self.bias = bias.reshape(-1).clone(memory_format=torch.contiguous_format) if bias is not None else None
         self._c = _lib.Linear4bitWeightsC(ptr(self.packed), ptr(self.scales), ptr(self.zeros), ptr(self.code),
                                           ptr(self.bias), dtype_code(self.bias.dtype) if bias is not None else 0, N, K, gs)
         self._ref = ctypes.byref(self._c)

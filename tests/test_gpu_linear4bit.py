@@ -533,3 +533,29 @@ def test_large_x_with_small_scales(dev):
     for xd, rows in ((BF, 1), (BF, 9), (FS, 2), (FS, 16)):
         x = (torch.randn((rows, K), device=dev) * 2.0 ** 120).to(xd)
         _check(layer(x, out_dtype=FS), x, W, None, code)
+
+
+@pytest.mark.parametrize("kind", ["code", "zeros"])
+def test_arguments_may_be_overwritten(dev, kind):
+    """The layer holds copies of all that it was made from, in calls and in a captured graph."""
+    from next_step_ai_b200.linear4bit import Linear4bit
+
+    N, K = 300, 256
+    made = _make(N, K, 64, kind, dev, 61, FS, FS)
+    p, sc, code, zeros, b = made
+    layer = Linear4bit(p, sc, out_features=N, in_features=K, group_size=64, code=code, zeros=zeros, bias=b)
+    x = torch.randn((3, K), device=dev, dtype=BF)
+    want = layer(x, out_dtype=FS)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = layer(x, out_dtype=FS)
+    for t in made:
+        if t is not None:
+            t.fill_(3)
+    assert torch.equal(layer(x, out_dtype=FS), want)
+    g.replay()
+    assert torch.equal(y, want)
+    strided = torch.randn((N, 2), device=dev)
+    a = Linear4bit(p, sc, out_features=N, in_features=K, group_size=64, bias=strided[:, 0])
+    c = Linear4bit(p, sc, out_features=N, in_features=K, group_size=64, bias=strided[:, 0].contiguous())
+    assert torch.equal(a(x), c(x)) and a.bias.is_contiguous()
