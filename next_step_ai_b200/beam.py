@@ -152,14 +152,47 @@ def _check_apart(states) -> None:
         raise RuntimeError("two states begin at the same address: states must not overlap")
 
 
+def _run_starts(c: _lib.BeamStateC, rows: int) -> torch.Tensor:
+    """The addresses of a state's runs."""
+    at = torch.tensor(c.data, dtype=torch.int64)
+    for n, step in ((rows, c.row_stride), (c.outer0, c.outer0_stride), (c.outer1, c.outer1_stride)):
+        at = at[..., None] + torch.arange(n, dtype=torch.int64) * step
+    return at.reshape(-1)
+
+
+def _check_disjoint(described, rows: int) -> None:
+    """No byte belongs to two states: different states move at the same time.  States whose
+    extents meet are compared run by run, so that parts of one buffer may lie in between
+    each other."""
+    def end(c):
+        return (c.data + (rows - 1) * c.row_stride + (c.outer0 - 1) * c.outer0_stride + (c.outer1 - 1) * c.outer1_stride
+                + c.run_bytes)
+
+    meeting: list[list] = []
+    reach = 0
+    for c in sorted(described, key=lambda c: c.data):
+        if c.data >= reach:
+            meeting.append([])
+        meeting[-1].append(c)
+        reach = max(reach, end(c))
+    for group in meeting:
+        if len(group) < 2:
+            continue
+        first = [_run_starts(c, rows) for c in group]
+        starts, order = torch.cat(first).sort()
+        ends = torch.cat([s + c.run_bytes for s, c in zip(first, group)])[order]
+        if bool((starts[1:] < ends[:-1]).any()):
+            raise RuntimeError("two states share memory: states must not overlap")
+
+
 class BeamStates:
     """The per-beam states of a decode (caches, histories, residuals), reordered in
     place and in one launch after each selection.
 
     ``states``: CUDA tensors ``[batch * beams, ...]`` of any type, row ``b *
     beams + w`` beam ``w`` of item ``b``; they are kept, must keep their memory
-    and must not overlap.  ``length_dims``: for each state the dimension that holds positions, or
-    ``None``; :meth:`reorder_` can then move the first ``length`` positions only."""
+    and must not overlap (states that share a byte are refused).  ``length_dims``: for each
+    state the dimension that holds positions, or ``None``; :meth:`reorder_` can then move the first ``length`` positions only."""
 
     def __init__(self, states, batch: int, beams: int, length_dims=None):
         self.states = list(states)
@@ -178,7 +211,9 @@ class BeamStates:
         _check_apart(self.states)
         self.device = self.states[0].device
         n = len(self.states)
-        self._c = (_lib.BeamStateC * n)(*(_describe(t, self.batch * self.beams, d) for t, d in zip(self.states, dims)))
+        described = [_describe(t, self.batch * self.beams, d) for t, d in zip(self.states, dims)]
+        _check_disjoint(described, self.batch * self.beams)
+        self._c = (_lib.BeamStateC * n)(*described)
         self.max_length = min((c.positions for c in self._c if c.position_bytes), default=None)
         self._lib = lib = _lib.load()
         with torch.cuda.device(self.device):

@@ -122,3 +122,29 @@ def test_a_state_given_twice_is_refused():
         beam._check_apart([t, torch.zeros((4, 6)), t])
     with pytest.raises(RuntimeError, match="must not overlap"):
         beam._check_apart([t, t[:, :3]])
+
+
+def _check(states, rows=4):
+    beam._check_disjoint([beam._describe(t, rows, d) for t, d in states], rows)
+
+
+def test_states_that_share_memory_are_refused():
+    z = torch.zeros
+    t, kv, cache = z((4, 6)), z((4, 2, 3, 5, 8)), z((4, 3, 2, 5, 8))
+    # parts of a buffer side by side, or in between each other, in any order
+    _check([(t[:, 3:], None), (z((4, 6)), None), (t[:, :3], 1)])
+    _check([(kv[:, 0], 2), (kv[:, 1], 2)])
+    _check([(cache[:, :, 1], 2), (cache[:, :, 0], 2)])
+    _check([(z((8, 5))[:4], None), (z((8, 5))[4:], None)])
+    _check([(t[:, 0], None), (t[:, 2], None), (t[:, 1], None), (t[:, 3:], 1)])
+    whole = z(96)
+    _check([(whole[:48].view(4, 12)[:, :6], None), (whole[48:].view(4, 12), None)])
+    _check([(t[:1, :3], None), (t[:1, 3:], None)], rows=1)
+    for states in ([(t, None), (t[:, 3:], None)], [(t[:, 3:], 1), (z((4, 6)), None), (t, 1)],
+                   [(t[:, :4], None), (t[:, 3:], None)], [(kv, None), (kv[:, 1], 2)],
+                   [(cache[:, :, 1], 2), (cache[:, 1:], None)], [(whole[:48].view(4, 12), None), (whole[44:92].view(4, 12), None)],
+                   [(whole[:24].view(4, 6), None), (z((4, 6)), None), (whole.view(torch.uint8)[93:97].view(4, 1), None)]):
+        with pytest.raises(RuntimeError, match="share memory"):
+            _check(states)
+    with pytest.raises(RuntimeError, match="share memory"):
+        _check([(t[:1], None), (t[:1, 5:], None)], rows=1)

@@ -481,3 +481,21 @@ def test_few_blocks_with_many_values_above_the_last(dev, B, W, V, k, dtype):
     _check(beam_select(down, s, num_candidates=k), down, s, k)
     f = torch.rand((B, W), device=dev, generator=gen) < 0.4
     _check(beam_select(down, s, num_candidates=k, finished=f, pad_token=3), down, s, k, f, 3)
+
+
+def test_states_that_share_memory(dev):
+    """Parts of one buffer are put in order as states of their own; parts that share bytes are refused."""
+    from next_step_ai_b200 import BeamStates
+
+    B, W = 2, 3
+    kv = torch.randn((B * W, 2, 4, 8, 6), device=dev)
+    want = kv.clone()
+    parents = torch.tensor([[1, 1, 0], [2, 0, 2]], device=dev)
+    rows = (parents + W * torch.arange(B, device=dev)[:, None]).reshape(-1)
+    BeamStates([kv[:, 1], kv[:, 0]], B, W, [2, 2]).reorder_(parents, length=5)
+    want[:, :, :, :5] = want[rows][:, :, :, :5]
+    assert torch.equal(kv, want)
+    with pytest.raises(RuntimeError, match="share memory"):
+        BeamStates([kv, kv[:, 1]], B, W)
+    with pytest.raises(RuntimeError, match="share memory"):
+        BeamStates([kv[:, 0], kv[:, :, 2:]], B, W)
