@@ -271,7 +271,7 @@ struct MergeParams {
   int64_t* out_parents;
 };
 
-// A candidate is (beam << 32 | token), a block (its index among [W][entries + 1]): smaller
+// A candidate is (beam * V + token), a block (its index among [W][entries + 1]): smaller
 // comes first among equal scores.  A finished beam has one block, of one candidate.
 struct MergeShared {
   u64 key[kBmCap];  // scores in ordered bits, larger is better
@@ -281,47 +281,119 @@ struct MergeShared {
   uint32_t group[kBmGroups], cut;
   u64 best_key[kBsMaxK];   // the k best blocks
   int best_id[kBsMaxK];
-  int sum[kBmWarps];
   int entries_listed, values_listed, hits;
 };
 
-__device__ __forceinline__ int block_sum(int v, MergeShared& sh) {
-  v = __reduce_add_sync(0xffffffffu, v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh.sum[threadIdx.x >> 5] = v;
-  __syncthreads();
-  int s = 0;
+// The k-th largest of the values in [lo, hi] that `each` runs over (it calls its argument with
+// every value), where none is above hi and lo > 0.  need: how many of those equal to it are among
+// the k; 0 when all that are at least the result are, which are k, or fewer if there are fewer.
+// Every round counts the values in up to 2048 equal parts of the range and goes on with the part
+// that holds the k-th.  kNarrow: the range is cut to the values seen too, so that equal values end
+// it after one or two rounds.  Uses the candidates' list.
+constexpr int kBmBins = 2048;
+template <bool kNarrow, typename Each>
+__device__ __forceinline__ u64 kth_value(MergeShared& sh, int k, u64 lo, u64 hi, Each each, int& need) {
+  static_assert(kBmBins * 4 <= (int)sizeof(sh.key) && kBmBins == 2 * kBmThreads, "two parts per thread");
+  int* const count = reinterpret_cast<int*>(sh.key);
+  u64* const seen = sh.id;  // the least and largest value, then what the next round goes on with
+  int* const warp_count = reinterpret_cast<int*>(sh.id + 8);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = 2 * threadIdx.x;
+  int above = 0;
+  for (;;) {
+    const u64 span = hi - lo;
+    const int shift = max(0, 64 - 11 - __clzll((long long)span));
+    __syncthreads();
+    count[mine] = count[mine + 1] = 0;
+    if (threadIdx.x == 0) {
+      seen[0] = ~0ull;
+      seen[1] = 0;
+      seen[2] = seen[3] = 0;  // unless a part has the k-th: all there are
+      seen[4] = 1;
+    }
+    __syncthreads();
+    u64 least = ~0ull, most = 0, last = lo - 1;
+    int part = 0, run = 0, in = 0;  // a thread's values are often equal, or lie in one part: added up first
+    each([&](u64 v) {
+      if (v != last) {
+        last = v;
+        in = v - lo <= span;
+        if (!in) return;
+        const int at = (int)((v - lo) >> shift);
+        if (at != part) {
+          if (run > 0) atomicAdd(&count[part], run);
+          part = at;
+          run = 0;
+        }
+        if (kNarrow) {
+          least = min(least, v);
+          most = max(most, v);
+        }
+      }
+      run += in;
+    });
+    if (run > 0) atomicAdd(&count[part], run);
+    __syncwarp();
+    if (kNarrow) {
 #pragma unroll
-  for (int w = 0; w < kBmWarps; ++w) s += sh.sum[w];
-  return s;
+      for (int o = 16; o > 0; o >>= 1) {
+        least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+      }
+      if (lane == 0 && least <= most) {
+        atomicMin(&seen[0], least);
+        atomicMax(&seen[1], most);
+      }
+    }
+    __syncthreads();
+    const int c[2] = {count[mine], count[mine + 1]};
+    int n = c[0] + c[1];  // of this thread's parts and all above, in the warp
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int from = __shfl_down_sync(0xffffffffu, n, o);
+      if (lane + o < 32) n += from;
+    }
+    if (lane == 0) warp_count[warp] = n;
+    __syncthreads();
+    static_assert(kBmWarps == 32, "a lane per warp");
+    n += above + __reduce_add_sync(0xffffffffu, lane > warp ? warp_count[lane] : 0) - c[0] - c[1];
+#pragma unroll
+    for (int i = 1; i >= 0; --i) {
+      if (n < k && n + c[i] >= k) {
+        const u64 at = lo + ((u64)(mine + i) << shift), last_of = at + ((1ull << shift) - 1);
+        seen[2] = kNarrow ? max(at, seen[0]) : at;
+        seen[3] = (hi - at) >> shift ? last_of : hi;
+        if (kNarrow) seen[3] = min(seen[3], seen[1]);
+        seen[4] = (u64)n << 1 | (u64)(n + c[i] == k);
+      }
+      n += c[i];
+    }
+    __syncthreads();
+    lo = seen[2];
+    hi = seen[3];
+    above = (int)(seen[4] >> 1);
+    const bool all = seen[4] & 1;
+    if (all || lo == hi) {
+      need = all ? 0 : k - above;
+      __syncthreads();
+      return lo;
+    }
+  }
 }
 
-// The k-th best (key, id) of what `each` runs over (it calls its argument with
-// every key and id), bit by bit: exactly k are at least that good if there are k.
+// The k-th best (key, id) of what `each` runs over (it calls its argument with every key in
+// [lo, hi] and its id, below id_end): exactly k are at least that good if there are k.
 template <typename Each>
-__device__ __forceinline__ void kth_best(MergeShared& sh, int k, Each each, u64& ck, u64& cf) {
-  ck = 0;
+__device__ __forceinline__ void kth_best(MergeShared& sh, int k, u64 lo, u64 hi, u64 id_end, Each each, u64& ck, u64& cf) {
+  int need;
+  ck = kth_value<true>(sh, k, lo, hi, [&](auto use) { each([&](u64 key, u64) { use(key); }); }, need);
   cf = ~0ull;
-  bool done = false;
-  for (int bit = 63; bit >= 0 && !done; --bit) {
-    const u64 tr = ck | (1ull << bit);
-    int c = 0;
-    each([&](u64 key, u64) { c += key >= tr; });
-    c = block_sum(c, sh);
-    if (c >= k) ck = tr;
-    done = c == k;
-  }
-  if (done) return;
-  u64 low = 0;  // of ~id
-  for (int bit = 63; bit >= 0 && !done; --bit) {
-    const u64 tr = low | (1ull << bit);
-    int c = 0;
-    each([&](u64 key, u64 id) { c += key > ck || (key == ck && ~id >= tr); });
-    c = block_sum(c, sh);
-    if (c >= k) low = tr;
-    done = c == k;
-  }
-  cf = ~low;
+  if (need == 0) return;
+  const u64 key_k = ck;  // ids are different: the need-th smallest has need at least as small
+  cf = ~kth_value<false>(sh, need, ~id_end, ~0ull, [&](auto use) {
+    each([&](u64 key, u64 id) {
+      if (key == key_k) use(~id);
+    });
+  }, need);
 }
 
 // Calls found(rank, key, id) for the k best of the n in sh.key / sh.id; eight
@@ -369,7 +441,8 @@ __device__ __forceinline__ uint32_t group_threshold(MergeShared& sh, int k) {
   return sh.cut;
 }
 
-// What the steps of the merge share.
+// What the steps of the merge share.  The functions that are not inlined copy it: through a
+// reference every use in their loops would be a load.
 struct MergeView {
   const MergeParams& mp;
   MergeShared& sh;
@@ -379,12 +452,19 @@ struct MergeView {
   __device__ __forceinline__ u64 score_key(int w, float v) const {
     return order_f64(sh.score[w] + ((double)v - sh.lse[w]));
   }
+  __device__ __forceinline__ u64 candidate(int w, int64_t token) const { return (u64)w * (unsigned)mp.scan.V + (u64)token; }
+  // Above every candidate and block.
+  __device__ __forceinline__ u64 id_end() const { return (u64)mp.scan.W * (unsigned)max(mp.scan.V, mp.scan.entries + 1); }
   __device__ __forceinline__ void append(int* count, u64 key, u64 id) const {
     const int e = atomicAdd(count, 1);
     if (e < kBmCap) {
       sh.key[e] = key;
       sh.id[e] = id;
     }
+  }
+  // More than the list holds: it is made again, and nothing more need be put in.
+  __device__ __forceinline__ bool over(const int* count) const {
+    return *reinterpret_cast<const volatile int*>(count) > kBmCap;
   }
   template <typename T>
   __device__ __forceinline__ const T* row(int w) const {
@@ -396,7 +476,11 @@ struct MergeView {
 // costs their number squared): by the groups' threshold, and if very many scores are equal
 // exactly.
 constexpr int kBmRank = 256;
-__device__ __noinline__ void shrink_list(const MergeView& v, int* count) {
+constexpr int kBmMany = kBsBlock - 1;  // candidates listed (one value after the other): no block of equal values
+static_assert(kBmMany + kBsMaxBeams <= kBmCap, "the list, with the finished beams' candidates");
+__device__ __noinline__ void shrink_list(const MergeView& view, int* count) {
+  const MergeParams mp = view.mp;
+  const MergeView v{mp, view.sh, view.entry, view.b};
   MergeShared& sh = v.sh;
   constexpr int kMine = kBmCap / kBmThreads;
   u64 key[kMine], id[kMine];
@@ -415,7 +499,7 @@ __device__ __noinline__ void shrink_list(const MergeView& v, int* count) {
   u64 ck = (u64)group_threshold(sh, v.mp.k) << 32, cf = ~0ull;
   for (int exact = 0; exact < 2; ++exact) {
     if (exact) {
-      kth_best(sh, v.mp.k, [&](auto use) {
+      kth_best(sh, v.mp.k, max(ck, 1ull), ~0ull, v.id_end(), [&](auto use) {
 #pragma unroll
         for (int i = 0; i < kMine; ++i)
           if (key[i]) use(key[i], id[i]);
@@ -433,10 +517,12 @@ __device__ __noinline__ void shrink_list(const MergeView& v, int* count) {
 }
 
 // The k best blocks when very many have equal maxima.
-__device__ __noinline__ void entries_again(const MergeView& v) {
+__device__ __noinline__ void entries_again(const MergeView& view) {
+  const MergeParams mp = view.mp;
+  const MergeView v{mp, view.sh, view.entry, view.b};
   const int n = v.mp.scan.W * (v.mp.scan.entries + 1);
   u64 ck, cf;
-  kth_best(v.sh, v.mp.k, [&](auto use) {
+  kth_best(v.sh, v.mp.k, 1ull, ~0ull, v.id_end(), [&](auto use) {
     for (int i = threadIdx.x; i < n; i += kBmThreads)
       if (v.entry[i]) use(v.entry[i], (u64)i);
   }, ck, cf);
@@ -449,28 +535,94 @@ __device__ __noinline__ void entries_again(const MergeView& v) {
   __syncthreads();
 }
 
-// The k best of the blocks' values when very many scores are equal.
-template <typename T>
-__device__ __noinline__ void values_again(const MergeView& v, int blocks, u64 least) {
+// Block i % run of the chosen entry i / run: its beam w and where it begins; false where there
+// are no values (a finished beam, the last entry's end).
+__device__ __forceinline__ bool find_chosen(const MergeView& v, int i, int& w, int64_t& at) {
   const ScanParams& p = v.mp.scan;
+  const int j = p.run == 1 ? i : i / p.run, per_beam = p.entries + 1;
+  const int id = v.sh.best_id[j];
+  w = id / per_beam;
+  at = ((int64_t)(id - w * per_beam) * p.run + (i - j * p.run)) * kBsBlock;
+  return v.sh.alive[w] != 2 && at < p.V;
+}
+
+// Eight values per lane of a block of `left`: block_pos's 8 part .. 8 part + 7.
+constexpr int kBmPer = 8, kBmParts = kBsPer / kBmPer;
+template <typename T, bool kVec>
+__device__ __forceinline__ void load_part(const T* block, int left, int part, uint32_t* r) {
+  constexpr int n = 16 / sizeof(T);
+  if (kVec && left >= kBsBlock) {
+#pragma unroll
+    for (int c = 0; c < kBmPer / n; ++c) {
+      const uint4 u = *(reinterpret_cast<const uint4*>(block) + (part * (kBmPer / n) + c) * 32 + (threadIdx.x & 31));
+      r[4 * c] = u.x;
+      r[4 * c + 1] = u.y;
+      r[4 * c + 2] = u.z;
+      r[4 * c + 3] = u.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < kBmPer; ++e) {
+    const int pos = block_pos<T, kVec>(part * kBmPer + e, false);
+    const uint32_t b = pos < left ? raw_bits<T>(block[pos]) : kMinusInf<T>;
+    uint32_t& word = r[e * (int)sizeof(T) / 4];
+    word = sizeof(T) == 2 && e % 2 ? word | b << 16 : b;
+  }
+}
+
+// The k best of the blocks' values when very many reach `least`: equal scores, or large values
+// next to each other.  Every pass reads the blocks again, from L2, a warp per quarter of a block and
+// the next quarter under way.  With every word of 1 x 4 x 128256 masked by the lowest value but one,
+// 8 candidates, the call takes 41 us (ordinary logits 12.5; five passes over 8192 values); of
+// 1 x 32 x 128256, 64 candidates, 125 us (20.6; over 65536 values, by the issue of some 50
+// instructions each).
+template <typename T, bool kVec>
+__device__ __noinline__ void values_again(const MergeView& view, int blocks, u64 least) {
+  const MergeParams mp = view.mp;
+  const MergeView v{mp, view.sh, view.entry, view.b};
+  const ScanParams& p = mp.scan;
+  const int lane = threadIdx.x & 31;
+  struct Part {
+    uint32_t r[kBmPer * sizeof(T) / 4];
+    int64_t at;
+    int w, left;  // left: 0 = no values, -1 = a finished beam's candidate
+  };
+  auto load = [&](int i, Part& q) {
+    q.left = 0;
+    if (i >= blocks * p.run * kBmParts) return;
+    if (!find_chosen(v, i / kBmParts, q.w, q.at)) {
+      if (v.sh.alive[q.w] == 2 && i % (p.run * kBmParts) == 0) q.left = -1;
+      q.at = i / (p.run * kBmParts);
+      return;
+    }
+    q.left = (int)min((int64_t)kBsBlock, p.V - q.at);
+    load_part<T, kVec>(v.row<T>(q.w) + q.at, q.left, i % kBmParts, q.r);
+  };
   auto each = [&](auto use) {
-    const int64_t per = (int64_t)p.run * kBsBlock;
-    for (int64_t i = threadIdx.x; i < blocks * per; i += kBmThreads) {
-      const int j = (int)(i / per), id = v.sh.best_id[j], w = id / (p.entries + 1);
-      if (v.sh.alive[w] == 2) {
-        if (i == j * per) use(v.sh.best_key[j], (u64)w << 32 | (u64)v.mp.pad);
-        continue;
+    Part next;
+    load(threadIdx.x >> 5, next);
+    for (int i = threadIdx.x >> 5; i < blocks * p.run * kBmParts; i += kBmWarps) {
+      const Part q = next;
+      load(i + kBmWarps, next);
+      if (q.left < 0 && lane == 0) use(v.sh.best_key[q.at], v.candidate(q.w, v.mp.pad));
+      if (q.left <= 0) continue;
+      float last = -INFINITY;
+      u64 key = 0;
+#pragma unroll
+      for (int e = 0; e < kBmPer; ++e) {
+        const float x = clean(raw_value<T>(q.r[e * (int)sizeof(T) / 4], e));
+        if (x != last) {  // equal values follow each other where there are very many
+          key = x > -INFINITY ? v.score_key(q.w, x) : 0ull;
+          last = x;
+        }
+        if (key >= least)
+          use(key, v.candidate(q.w, q.at + block_pos<T, kVec>(i % kBmParts * kBmPer + e, q.left >= kBsBlock)));
       }
-      const int64_t pos = (id - w * (p.entries + 1)) * per + (i - j * per);
-      if (pos >= p.V) continue;
-      const float x = clean(to_f32<T>(v.row<T>(w)[pos]));
-      if (x == -INFINITY) continue;
-      const u64 key = v.score_key(w, x);
-      if (key >= least) use(key, (u64)w << 32 | (u64)pos);
     }
   };
   u64 ck, cf;
-  kth_best(v.sh, v.mp.k, each, ck, cf);
+  kth_best(v.sh, v.mp.k, least, v.sh.best_key[0], v.id_end(), each, ck, cf);
   if (threadIdx.x == 0) v.sh.values_listed = 0;
   __syncthreads();
   each([&](u64 key, u64 id) {
@@ -561,7 +713,7 @@ __device__ __forceinline__ void merge_item(const MergeParams& mp, MergeShared& s
   const uint32_t cut = group_threshold(sh, mp.k);
   for (int i = threadIdx.x; i < W * per_beam; i += kBmThreads) {
     const u64 q = view.entry[i];
-    if (q && (uint32_t)(q >> 32) >= cut) view.append(&sh.entries_listed, q, i);
+    if (q && (uint32_t)(q >> 32) >= cut && !view.over(&sh.entries_listed)) view.append(&sh.entries_listed, q, i);
   }
   __syncthreads();
   if (sh.entries_listed > kBmCap) entries_again(view);
@@ -575,14 +727,10 @@ __device__ __forceinline__ void merge_item(const MergeParams& mp, MergeShared& s
 
   // 3. their values that reach the k-th block's largest score
   u64 least = blocks == mp.k ? sh.best_key[blocks - 1] : 1ull;
-  auto load_chosen = [&](int i, RawTile<T>& q, int& w, int64_t& at) {  // false: no values there
-    const int j = p.run == 1 ? i : i / p.run;
-    const int id = sh.best_id[j];
-    w = id / per_beam;
-    at = ((int64_t)(id - w * per_beam) * p.run + (i - j * p.run)) * kBsBlock;
-    if (sh.alive[w] == 2 || at >= p.V) return false;
-    load_block<T, kVec>(view.row<T>(w), at, (int)min((int64_t)kBsBlock, p.V - at), q);
-    return true;
+  auto load_chosen = [&](int i, RawTile<T>& q, int& w, int64_t& at) {
+    const bool has = find_chosen(view, i, w, at);
+    if (has) load_block<T, kVec>(view.row<T>(w), at, (int)min((int64_t)kBsBlock, p.V - at), q);
+    return has;
   };
   // Where there are fewer blocks than candidates (a small vocabulary, a heavy mask), or too many values
   // reach that score (few blocks, large values next to each other), a threshold from the lanes'
@@ -591,7 +739,7 @@ __device__ __forceinline__ void merge_item(const MergeParams& mp, MergeShared& s
     if (refine) {
       __syncthreads();
       if (threadIdx.x < kBmGroups) sh.group[threadIdx.x] = 0;
-      if (threadIdx.x == 0) sh.values_listed = 0;
+      if (threadIdx.x == 0) sh.values_listed = sh.hits = 0;
       __syncthreads();
       for (int i = warp; i < blocks * p.run; i += kBmWarps) {
         RawTile<T> q;
@@ -613,7 +761,7 @@ __device__ __forceinline__ void merge_item(const MergeParams& mp, MergeShared& s
       int64_t at;
       if (!load_chosen(i, q, w, at)) {
         if (sh.alive[w] == 2 && lane == 0 && i % p.run == 0)
-          view.append(&sh.values_listed, sh.best_key[i / p.run], (u64)w << 32 | (u64)mp.pad);
+          view.append(&sh.values_listed, sh.best_key[i / p.run], view.candidate(w, mp.pad));
         continue;
       }
       const int left = (int)min((int64_t)kBsBlock, p.V - at);
@@ -626,12 +774,11 @@ __device__ __forceinline__ void merge_item(const MergeParams& mp, MergeShared& s
 #pragma unroll
       for (int e = 0; e < kBsPer; ++e)
         if (clean(raw_value<T>(q, e)) >= thr) hits |= 1u << e;
-      if (!refine) {
-        const int n = __reduce_add_sync(0xffffffffu, __popc(hits));
-        int before = 0;
-        if (lane == 0 && n > 0) before = atomicAdd(&sh.hits, n);
-        if (__shfl_sync(0xffffffffu, before, 0) + n > kBmRank) continue;  // too many: another threshold
-      }
+      const int n = __reduce_add_sync(0xffffffffu, __popc(hits));
+      int before = 0;
+      if (lane == 0 && n > 0) before = atomicAdd(&sh.hits, n);
+      // too many: another threshold, or, where that was it, the search that needs no list
+      if (__shfl_sync(0xffffffffu, before, 0) + n > (refine ? kBmMany : kBmRank)) continue;
       while (hits) {  // few
         const int at_e = __ffs(hits) - 1;
         hits &= hits - 1;
@@ -641,20 +788,21 @@ __device__ __forceinline__ void merge_item(const MergeParams& mp, MergeShared& s
           if (e == at_e * (int)sizeof(T) / 4) word = q.r[e];
         const u64 key = view.score_key(w, clean(raw_value<T>(word, at_e)));
         if (key >= least)
-          view.append(&sh.values_listed, key, (u64)w << 32 | (u64)(at + block_pos<T, kVec>(at_e, left >= kBsBlock)));
+          view.append(&sh.values_listed, key, view.candidate(w, at + block_pos<T, kVec>(at_e, left >= kBsBlock)));
       }
     }
     __syncthreads();
     if (refine || sh.hits <= kBmRank) break;
   }
-  if (sh.values_listed > kBmCap) values_again<T>(view, blocks, least);
+  if (sh.hits > kBmMany) values_again<T, kVec>(view, blocks, least);
   if (sh.values_listed > kBmRank) shrink_list(view, &sh.values_listed);
   const int n = sh.values_listed;
   const int64_t out = (int64_t)b * mp.k;
   rank_list(sh, n, mp.k, [&](int rank, u64 key, u64 id) {
     mp.out_scores[out + rank] = (float)unorder_f64(key);
-    mp.out_tokens[out + rank] = (int64_t)(id & 0xffffffffu);
-    mp.out_parents[out + rank] = (int64_t)(id >> 32);
+    const u64 w = id / (unsigned)p.V;
+    mp.out_tokens[out + rank] = (int64_t)(id - w * (unsigned)p.V);
+    mp.out_parents[out + rank] = (int64_t)w;
   });
   for (int r = n + threadIdx.x; r < mp.k; r += kBmThreads) {  // too few candidates
     mp.out_scores[out + r] = -INFINITY;
