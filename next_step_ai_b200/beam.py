@@ -8,8 +8,6 @@ share most of their blocks), a head (``Nf4LmHead``, ``Linear4bit``) and these.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
@@ -152,36 +150,47 @@ def _check_apart(states) -> None:
         raise RuntimeError("two states begin at the same address: states must not overlap")
 
 
-def _run_starts(c: _lib.BeamStateC, rows: int) -> torch.Tensor:
-    """The addresses of a state's runs."""
-    at = torch.tensor(c.data, dtype=torch.int64)
-    for n, step in ((rows, c.row_stride), (c.outer0, c.outer0_stride), (c.outer1, c.outer1_stride)):
-        at = at[..., None] + torch.arange(n, dtype=torch.int64) * step
-    return at.reshape(-1)
-
-
 def _check_disjoint(described, rows: int) -> None:
     """No byte belongs to two states: different states move at the same time.  States whose
     extents meet are compared run by run, so that parts of one buffer may lie in between
     each other."""
-    def end(c):
-        return (c.data + (rows - 1) * c.row_stride + (c.outer0 - 1) * c.outer0_stride + (c.outer1 - 1) * c.outer1_stride
-                + c.run_bytes)
+    # where a state begins, its run, and the (count, stride) of its rows and outer dimensions
+    sets = [(c.data, c.run_bytes, [(n, s) for n, s in ((rows, c.row_stride), (c.outer0, c.outer0_stride),
+                                                       (c.outer1, c.outer1_stride)) if n > 1]) for c in described]
+
+    def end(e):
+        return e[0] + e[1] + sum((n - 1) * s for n, s in e[2])
 
     meeting: list[list] = []
     reach = 0
-    for c in sorted(described, key=lambda c: c.data):
-        if c.data >= reach:
+    for e in sorted(sets, key=lambda e: e[0]):
+        if e[0] >= reach:
             meeting.append([])
-        meeting[-1].append(c)
-        reach = max(reach, end(c))
+        meeting[-1].append(e)
+        reach = max(reach, end(e))
     for group in meeting:
         if len(group) < 2:
             continue
-        first = [_run_starts(c, rows) for c in group]
-        starts, order = torch.cat(first).sort()
-        ends = torch.cat([s + c.run_bytes for s, c in zip(first, group)])[order]
-        if bool((starts[1:] < ends[:-1]).any()):
+        # A stride that all have, and that all of them fit into without it: what lies at different
+        # multiples of it is apart, and one multiple is as the others.
+        again = True
+        while again:
+            again = False
+            for step in {s for _, s in group[0][2]}:
+                if all(any(s == step for _, s in e[2]) for e in group):
+                    rest = [(at, run, [d for d in dims if d[1] != step]) for at, run, dims in group]
+                    if max(end(e) for e in rest) - min(e[0] for e in rest) <= step:
+                        group, again = rest, True
+                        break
+        starts, ends = [], []
+        for at, run, dims in group:
+            first = torch.tensor([at], dtype=torch.int64)
+            for n, s in dims:
+                first = (first[:, None] + torch.arange(n, dtype=torch.int64) * s).reshape(-1)
+            starts.append(first)
+            ends.append(first + run)
+        first, order = torch.cat(starts).sort()
+        if bool((first[1:] < torch.cat(ends)[order][:-1]).any()):
             raise RuntimeError("two states share memory: states must not overlap")
 
 

@@ -148,3 +148,42 @@ def test_states_that_share_memory_are_refused():
             _check(states)
     with pytest.raises(RuntimeError, match="share memory"):
         _check([(t[:1], None), (t[:1, 5:], None)], rows=1)
+
+
+def test_shared_memory_is_found_run_by_run():
+    """Random parts of one buffer: refused where an element belongs to two of them, and only there."""
+    gen = torch.Generator().manual_seed(7)
+    pick = lambda n: int(torch.randint(0, n, (1,), generator=gen))  # noqa: E731
+    seen = [0, 0]
+    for _ in range(400):
+        shape = [4, 1 + pick(4), 1 + pick(4), 1 + pick(6)]
+        order = [0, 1, 2, 3] if pick(3) else [1, 0, 2, 3]
+        buf = torch.arange(4 * shape[1] * shape[2] * shape[3]).reshape([shape[i] for i in order]).permute(order)
+        states = []
+        for _ in range(2 + pick(2)):
+            cut = [slice(None)]
+            for n in buf.shape[1:]:
+                a = pick(n)
+                cut.append(slice(a, a + 1 + pick(n - a)))
+            states.append(buf[tuple(cut)])
+        used = torch.cat([s.reshape(-1) for s in states])
+        shared = used.unique().numel() != used.numel()
+        seen[shared] += 1
+        if shared:
+            with pytest.raises(RuntimeError, match="share memory"):
+                _check([(s, None) for s in states])
+        else:
+            _check([(s, None) for s in states])
+    assert min(seen) > 40
+
+
+def test_large_interleaved_states_are_checked_at_once():
+    """The keys and values of one buffer, in between each other at every position: not looked through
+    one by one (2^26 of them)."""
+    data, es, rows, heads, positions, dim = 1 << 40, 2, 256, 64, 4096, 128
+    one = [_lib.BeamStateC(data + part * dim * es, heads * positions * 2 * dim * es, 1, 0, heads * positions, 2 * dim * es,
+                           dim * es, 0, 0) for part in range(2)]
+    beam._check_disjoint(one, rows)
+    one[1].data -= 2
+    with pytest.raises(RuntimeError, match="share memory"):
+        beam._check_disjoint(one, rows)
