@@ -581,7 +581,9 @@ int nsm_linear4bit_code16(const void* x, int32_t x_dtype, int32_t rows, int64_t 
  * candidate, pad_token at its own score; its logits are not read either.  A logit
  * of -infinity or NaN is no candidate; +infinity counts as the largest finite
  * value.  The logsumexp is taken from fp32 sums (equal rows give equal bits); scores
- * are formed and compared in 64 bits.  Outputs [batch]
+ * are formed and compared in 64 bits.  (Where the largest logit is 2^53 or more in
+ * magnitude, as in a row of nothing but the type's lowest value, 64 bits lose the logarithm of
+ * the sum: its words have the beam's own score.)  Outputs [batch]
  * [candidates]: scores, tokens and parents (the beam w); where fewer candidates
  * exist, score -infinity, token -1, parent 0.  1..32 beams, 1..64 candidates.  The
  * workspace needs no initialisation; nsm_beam_select_workspace_bytes is 0 for sizes

@@ -28,7 +28,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, num_candidates: i
     the beams.  ``finished [batch, beams]`` (bool): such a beam is one candidate,
     ``pad_token`` at its own score.  A logit of -infinity or NaN is no
     candidate; where too few exist: score -infinity, token -1, parent 0.
-    Scores are formed and compared in 64 bits, with log-sum-exps of fp32 sums."""
+    Scores are formed and compared in 64 bits, with log-sum-exps of fp32 sums.  (In a
+    row of nothing but the type's lowest value 64 bits lose the logarithm of the sum: its words
+    have the beam's own score.  Mask with -infinity what may not come.)"""
     require_cuda(logits, "logits")
     dev = logits.device
     if scores.dim() != 2 or scores.dtype != torch.float32 or scores.device != dev:

@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) lin4_kernel(const __grid_consta
   Lin4Bars& bars = *reinterpret_cast<Lin4Bars*>(smem + C::kBars);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = threadIdx.x & 127;
   int u0, u1;
-  if constexpr (kCluster) {  // (no trigger: what comes next is no kernel of ours)
+  if constexpr (kCluster) {  // (no trigger: what comes next reads what this kernel writes)
     const int block = blockIdx.x / p.cluster, rank = blockIdx.x - block * p.cluster;
     u0 = block * p.steps + p.steps * rank / p.cluster;
     u1 = block * p.steps + p.steps * (rank + 1) / p.cluster;
@@ -1049,11 +1049,12 @@ int lin4_clusters_at_once(int ctas, const DeviceInfo& di) {
 
 // In one launch, a row block is a cluster's, cut evenly over its CTAs, and the sums join in shared
 // memory: no finalize kernel and no workspace of partials.  The host then takes 8.5 us per call
-// instead of 12, the GPU 0.4 to 0.7 us more (4096 x 4096 10.0 in a graph instead of 9.3), so it is taken
-// where calls one after another wait for the host: runs of at most four units (0.94 us each), two
-// longer than an even cut's, of clusters that fit the GPU at once (14336 x 4096, eight units instead
-// of seven: 17.8 us instead of 17.2).  The choice depends on the weight alone, so a row's bits do not
-// depend on the number of rows.
+// instead of 12, the GPU 0.4 to 0.7 us more (4096 x 4096 with the codebook in fp16 10.0 in a graph
+// instead of 9.3), so it is taken where calls one after another wait for the host: runs of at most
+// four units (0.94 us each; 1.64 with the codebook to 22 bits, where calls take 12.3 us), two longer
+// than an even cut's, of clusters that fit the GPU at once (14336 x 4096, eight units instead of
+// seven: 17.8 us instead of 17.2).  The choice depends on the weight's sizes alone, so a row's bits do
+// not depend on the number of rows, nor the workspace on the codebook.
 Lin4Plan lin4_plan(const Lin4Shape& sh, int rows, int x_dtype, const DeviceInfo& di) {
   Lin4Plan pl;
   pl.cols = x_dtype == NSM_F32 ? 2 * rows : rows;
