@@ -556,8 +556,9 @@ int nsm_linear4bit(const void* x, int32_t x_dtype, int32_t rows, int64_t x_row_s
                    const nsm_linear4bit_weights* weights, void* out, int32_t out_dtype, int64_t out_row_stride,
                    void* workspace, size_t workspace_bytes, nsm_stream_t stream);
 /* The error word of these kernels on the current device: *code_out = NSM_ERR_TIMEOUT when a
- * wait of an earlier call ran out, else 0; the word is cleared.  Synchronises `stream`.  The
- * calls do not clear the word, so one check after several covers them all. */
+ * wait of an earlier call ran out, else 0; the word is cleared.  Synchronises `stream` (calls on
+ * other streams must be done).  The calls do not clear the word, so one check after several
+ * covers them all. */
 int nsm_linear4bit_error(int32_t* code_out, nsm_stream_t stream);
 /* Tries of each wait inside these kernels, instead of nsm_set_copy_wait_limit's: 0 = that one
  * (the default); -1 = none, so that every wait gives up at once (to test what follows then).

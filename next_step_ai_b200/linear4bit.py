@@ -151,7 +151,7 @@ class Linear4bit:
     def error(self) -> int:
         """Read and clear the error word of the layers on this device (``NSM_ERR_TIMEOUT``:
         a wait inside a kernel ran out and outputs of a call since the last check are NaN;
-        0: all is well).  Synchronises."""
+        0: all is well).  Synchronises the current stream; calls on others must be done."""
         code = ctypes.c_int32(0)
         with torch.cuda.device(self.device):
             _lib.check(self._lib.nsm_linear4bit_error(ctypes.byref(code), stream_handle(self.device)),

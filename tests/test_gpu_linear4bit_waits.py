@@ -109,3 +109,26 @@ def test_a_search_tells_of_its_heads_failure(dev, no_tries):
             return torch.zeros((hidden.shape[0], 50), device=dev, dtype=out_dtype)
 
     assert BeamSearch(Plain(), 2, 3, max_tokens=8).error() == 0
+
+
+@pytest.mark.parametrize("tries", [1, 2, 8])
+@pytest.mark.parametrize("N,K,rows,xd", [(4096, 4096, 1, BF), (4096, 16384, 1, BF), (4096, 16384, 8, FH),
+                                         (4096, 16384, 9, BF), (20000, 2048, 16, FS), (700, 16384, 32, BF)])
+@pytest.mark.parametrize("kind", ["code", "zeros"])
+def test_few_tries(dev, no_tries, tries, N, K, rows, xd, kind):
+    """Waits that may run out in the middle of a run, or not: an output is right or NaN, and where any
+    is NaN the failure is recorded."""
+    from next_step_ai_b200 import _lib
+
+    layer = _layer(dev, N, K, kind)
+    x = torch.randn((rows, K), device=dev).to(xd)
+    want = layer(x)
+    layer.error()
+    no_tries(tries)
+    got = [layer(x) for _ in range(10)]
+    no_tries(0)
+    code = layer.error()
+    lost = [torch.isnan(y) for y in got]
+    assert all(torch.equal(torch.where(m, want, y), want) for m, y in zip(lost, got))
+    assert code == (_lib.NSM_ERR_TIMEOUT if any(bool(m.any()) for m in lost) else code)
+    assert torch.equal(layer(x), want) and layer.error() == 0
